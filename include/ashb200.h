@@ -45,6 +45,9 @@ extern "C" {
 /* dtype / interpolation codes of the grid entry points */
 #define ASHB_F32 0
 #define ASHB_F64 1
+/* further value types of the layer and row entry points */
+#define ASHB_F16 2
+#define ASHB_BF16 3
 #define ASHB_LINEAR 0
 #define ASHB_SMOOTH_STEP 1
 
@@ -739,6 +742,92 @@ int ashb_routed_backward_backward(ashb_map* map, int interp, const void* const* 
                                   int64_t counts_offset, int64_t inbox_z_offset, int64_t out_y_offset,
                                   int64_t out_gx_offset, int64_t inbox_g_offset, int64_t region_capacity, int world,
                                   int rank, void* stream);
+
+/* ---------------------------------------------------------------- rows in 8 bits */
+
+/* Formats of a stored row: e4m3 codes or int8 codes, one byte a value, with one float32 scale a row.
+ *   scale = max(amax * rn(1 / most), 2^-126), code = rn(value * rn(1 / scale)), most = 448 or 127
+ * A row that holds an infinity or a NaN reads back as NaN throughout. */
+#define ASHB_E4M3 1
+#define ASHB_INT8 2
+
+/* One table of rows: values of `dtype` (ASHB_F32, ASHB_F16, ASHB_BF16) on one side, codes and scales on the other.
+ * Device pointers.  Writing: src values [n][width], dst codes [capacity][width].  Reading: src codes, dst values.
+ * format 0 (insertion only): rows of `width` BYTES copied as they are, scales and dtype unused. */
+typedef struct ashb_row_table {
+    const void* src;
+    void* dst;
+    float* scales;
+    int64_t width;
+    int32_t format;
+    int32_t dtype;
+} ashb_row_table;
+
+/* ashb_map_insert_values with tables that may be kept in 8 bits: the row of every NEW key is quantised as it is
+ * written.  `tables` is a HOST array of at most 16. */
+int ashb_map_insert_rows(ashb_map* map, const int32_t* keys_dev, int64_t n, int n_tables, const ashb_row_table* tables,
+                         void* stream);
+
+/* ashb_map_find, and the rows of tables kept in 8 bits: row i of a table's dst is what the row of key i reads back as, zeros
+ * for a miss.  indices_dev may be NULL. */
+int ashb_map_find_rows(ashb_map* map, const int32_t* keys_dev, int64_t n, int64_t* indices_dev, uint8_t* masks_dev,
+                       int n_tables, const ashb_row_table* tables, void* stream);
+
+/* Rows in order into codes and scales (current device). */
+int ashb_quantize_rows(int64_t n, const ashb_row_table* table, void* stream);
+
+/* Rows read back, in order (numbers_dev NULL) or row numbers_dev[i] (int64; zeros outside 0 .. n_rows - 1) (current
+ * device). */
+int ashb_read_rows(int64_t n, const int64_t* numbers_dev, int64_t n_rows, const ashb_row_table* table, void* stream);
+
+/* ---------------------------------------------------------------- norms and layers (current device) */
+
+/* Root-mean-square norm of rows of x, or of x + residual (then written to `sum`, required): y = s rstd weight with
+ * rstd = (mean(s^2) + eps)^(-1/2), statistics in float32.  Either y [rows][width] of the same type, or e4m3 codes
+ * [rows][width] and scales [rows].  x and residual may have a row stride (elements); all else is contiguous.  rstd
+ * (float32 [rows]) may be NULL. */
+int ashb_rms_norm_forward(int dtype, const void* x_dev, int64_t x_stride, const void* residual_dev, int64_t residual_stride,
+                          const void* weight_dev, int64_t rows, int64_t width, float eps, void* y_dev, uint8_t* codes_dev,
+                          float* scales_dev, void* sum_dev, float* rstd_dev, void* stream);
+
+/* Its gradient: dx (which is the residual's too) and dweight, from dy, the gradient dsum of `sum` (NULL: none), s (x, or
+ * `sum`), and rstd.  The weight's gradient is summed in a fixed order.  _workspace: bytes of device scratch. */
+int64_t ashb_rms_norm_workspace(int64_t rows, int64_t width);
+int ashb_rms_norm_backward(int dtype, const void* dy_dev, const void* dsum_dev, const void* s_dev, const void* weight_dev,
+                           const float* rstd_dev, int64_t rows, int64_t width, void* dx_dev, void* dweight_dev,
+                           void* workspace_dev, int64_t workspace_bytes, void* stream);
+
+/* operand type of a layer given as e4m3 rows with a float32 scale each */
+#define ASHB_E4M3_ROWS 8
+#define ASHB_ACT_NONE 0
+#define ASHB_ACT_RELU 1
+#define ASHB_ACT_SILU 2   /* z / (1 + e^-z) */
+#define ASHB_ACT_GELU 3   /* z (1 + erf(z / sqrt 2)) / 2 */
+#define ASHB_ACT_SIN 4    /* sin(omega z) */
+
+/* Dense layer: y = act(x weight^T + bias) + residual, x [rows][inputs] and weight [outputs][inputs] with row strides
+ * (values), y [rows][outputs] contiguous; bias [outputs] and residual may be NULL.  type: ASHB_F32, ASHB_F16, ASHB_BF16 --
+ * of x, weight, bias, residual and y alike -- or ASHB_E4M3_ROWS: x and weight are e4m3 codes with x_scales [rows] and
+ * weight_scales [outputs], bias, residual and y of out_type.  Sums are float32 (float32 operands are multiplied as exact
+ * sums of three bf16 parts).  slope (may be NULL): act'(z) [rows][outputs] in y's type, for the backward pass. */
+int ashb_linear_forward(int type, const void* x_dev, int64_t x_stride, const float* x_scales_dev, const void* weight_dev,
+                        int64_t weight_stride, const float* weight_scales_dev, const void* bias_dev, const void* residual_dev,
+                        int64_t residual_stride, int64_t rows, int64_t inputs, int64_t outputs, int activation, float omega,
+                        int out_type, void* y_dev, void* slope_dev, void* stream);
+
+/* Gradients of the same from dy [rows][outputs] (contiguous): dx [rows][inputs], dweight [outputs][inputs] and dbias
+ * [outputs], each NULL where not wanted (the residual's is dy).  slope_kind 0: no activation, slope NULL; 1: slope holds
+ * act'(z); 2: relu without a residual, slope is the output y.  Sums run in a fixed order.  _workspace: bytes of device
+ * scratch (256-byte aligned). */
+int64_t ashb_linear_workspace(int type, int64_t rows, int64_t inputs, int64_t outputs, int slope_kind, int want_dweight,
+                              int want_dbias);
+int ashb_linear_backward(int type, const void* dy_dev, const void* slope_dev, int slope_kind, const void* x_dev,
+                         int64_t x_stride, const void* weight_dev, int64_t weight_stride, int64_t rows, int64_t inputs,
+                         int64_t outputs, void* dx_dev, void* dweight_dev, void* dbias_dev, void* workspace_dev,
+                         int64_t workspace_bytes, void* stream);
+
+/* How many waits inside the layer kernels ran out on the current device (0 in a healthy run).  Synchronises. */
+int ashb_layer_timeouts(unsigned int* out);
 
 /* ---------------------------------------------------------------- runtime knobs */
 

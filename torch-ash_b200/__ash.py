@@ -130,11 +130,33 @@ _lib.ashb_routed_backward.argtypes = [_vp, _int, _vp, _vp, _int, _int, _c.c_doub
 _lib.ashb_routed_send_g.argtypes = [_vp, _i64, _vp, _i64] + _ROUTED_LAYOUT + [_vp]
 _lib.ashb_routed_backward_backward.argtypes = [_vp, _int, _vp, _vp, _c.c_double, _vp, _int, _vp, _vp, _i64, _i64] + _ROUTED_LAYOUT + [_vp]
 _lib.ashb_routed_unpack_grad_x.argtypes = [_vp, _i64, _vp, _i64] + _ROUTED_LAYOUT + [_vp]
+_lib.ashb_map_insert_rows.argtypes = [_vp, _vp, _i64, _int, _vp, _vp]
+_lib.ashb_map_find_rows.argtypes = [_vp, _vp, _i64, _vp, _vp, _int, _vp, _vp]
+_lib.ashb_quantize_rows.argtypes = [_i64, _vp, _vp]
+_lib.ashb_read_rows.argtypes = [_i64, _vp, _i64, _vp, _vp]
+_lib.ashb_rms_norm_forward.argtypes = [_int, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _f32] + [_vp] * 6
+_lib.ashb_rms_norm_workspace.argtypes = [_i64, _i64]
+_lib.ashb_rms_norm_workspace.restype = _i64
+_lib.ashb_rms_norm_backward.argtypes = [_int] + [_vp] * 5 + [_i64, _i64, _vp, _vp, _vp, _i64, _vp]
+_lib.ashb_linear_forward.argtypes = [_int, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _int, _f32, _int,
+                                     _vp, _vp, _vp]
+_lib.ashb_linear_workspace.argtypes = [_int, _i64, _i64, _i64, _int, _int, _int]
+_lib.ashb_linear_workspace.restype = _i64
+_lib.ashb_linear_backward.argtypes = [_int, _vp, _vp, _int, _vp, _i64, _vp, _i64, _i64, _i64, _i64] + [_vp] * 4 + [_i64, _vp]
+_lib.ashb_layer_timeouts.argtypes = [_vp]
 _lib.ashb_grid_zero_rows.argtypes = [_vp, _int, _vp, _vp, _c.c_double, _vp, _int, _vp, _vp, _i64, _i64, _i64, _vp]
 
 STATUS_CAPACITY, STATUS_PROBE, STATUS_SPIN, STATUS_DUPLICATE = 1, 2, 4, 8
 _DTYPES = {torch.float32: 0, torch.float64: 1}
 _INTERP = {"linear": 0, "smooth_step": 1}
+_VALUE_TYPES = {torch.float32: 0, torch.float16: 2, torch.bfloat16: 3}     # of rows and layers
+_ROW_FORMATS = {torch.float8_e4m3fn: 1, torch.int8: 2}
+_E4M3_ROWS = 8
+_ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "sin": 4}
+
+
+class _RowTable(_c.Structure):
+    _fields_ = [("src", _vp), ("dst", _vp), ("scales", _vp), ("width", _i64), ("format", _c.c_int32), ("dtype", _c.c_int32)]
 
 
 def _check(rc: int):
@@ -354,6 +376,50 @@ class HashMap:
         _check(
             _lib.ashb_map_insert_values(self._h, keys.data_ptr(), keys.shape[0], k, src, dst, row, _stream(self._device))
         )
+
+    def insert_rows(self, keys: torch.Tensor, values: dict, tables: dict) -> None:
+        """``insert`` for tables of which some are kept in 8 bits (not in the reference): ``tables[name]`` is the
+        buffer that takes the rows, or ``(codes, scales)``."""
+        keys = self._keys(keys)
+        n = keys.shape[0]
+        entries, keep = (_RowTable * max(len(tables), 1))(), []
+        for j, (name, table) in enumerate(tables.items()):
+            v = _cuda(values[name].detach(), f"values[{name!r}]")
+            codes, scales = table if isinstance(table, tuple) else (table, None)
+            if codes.device != self._device or not codes.is_contiguous() or v.device != self._device:
+                raise RuntimeError(f"value {name!r}: tables and values must be on {self._device}, tables contiguous")
+            if v.shape[0] != n or codes.shape[0] != self._capacity or v.shape[1:] != codes.shape[1:]:
+                raise RuntimeError(f"value {name!r}: shapes do not match keys / capacity")
+            if scales is None:
+                if v.dtype != codes.dtype:
+                    raise RuntimeError(f"value {name!r} must be {codes.dtype}, got {v.dtype}")
+                entries[j] = _RowTable(v.data_ptr(), codes.data_ptr(), None, codes.nbytes // self._capacity, 0, 0)
+            else:
+                if v.dtype not in _VALUE_TYPES:
+                    raise RuntimeError(f"value {name!r} must be float32, float16 or bfloat16, got {v.dtype}")
+                entries[j] = _RowTable(v.data_ptr(), codes.data_ptr(), scales.data_ptr(), codes.shape[1],
+                                       _ROW_FORMATS[codes.dtype], _VALUE_TYPES[v.dtype])
+            keep.append(v)
+        _check(_lib.ashb_map_insert_rows(self._h, keys.data_ptr(), n, len(tables), entries, _stream(self._device)))
+
+    def find_rows(self, keys: torch.Tensor, tables: dict, dtype: torch.dtype, with_indices: bool):
+        """``(indices or None, masks, {name: rows read back})`` of tables kept in 8 bits, ``(codes, scales)`` each, in one
+        launch; zeros for keys that are absent (not in the reference)."""
+        keys = self._keys(keys)
+        n = keys.shape[0]
+        indices = torch.empty(n, dtype=torch.int64, device=self._device) if with_indices else None
+        masks = torch.empty(n, dtype=torch.bool, device=self._device)
+        entries, out = (_RowTable * max(len(tables), 1))(), {}
+        for j, (name, (codes, scales)) in enumerate(tables.items()):
+            if codes.device != self._device or not codes.is_contiguous() or codes.shape[0] != self._capacity:
+                raise RuntimeError(f"table {name!r}: must be contiguous, of `capacity` rows, on {self._device}")
+            out[name] = torch.empty((n, codes.shape[1]), dtype=dtype, device=self._device)
+            entries[j] = _RowTable(codes.data_ptr(), out[name].data_ptr(), scales.data_ptr(), codes.shape[1],
+                                   _ROW_FORMATS[codes.dtype], _VALUE_TYPES[dtype])
+        if n:
+            _check(_lib.ashb_map_find_rows(self._h, keys.data_ptr(), n, indices.data_ptr() if with_indices else None,
+                                           masks.data_ptr(), len(tables), entries, _stream(self._device)))
+        return indices, masks, out
 
     def erase(self, keys: torch.Tensor) -> None:
         keys = self._keys(keys)
@@ -1535,3 +1601,140 @@ def routed_unpack_grad_x(where, n, D, layout):
     with torch.cuda.device(dev):
         _check(_lib.ashb_routed_unpack_grad_x(where.data_ptr(), n, gx.data_ptr(), D, *layout, _stream(dev)))
     return gx
+
+
+# ---- rows in 8 bits, norms and dense layers (not in the reference's native module) ---------------------------------
+def quantize_rows(x: torch.Tensor, codes_dtype: torch.dtype):
+    """``(codes, scales)`` of the rows of x (..., width)."""
+    x = _cuda(x.detach(), "x")
+    codes = torch.empty(x.shape, dtype=codes_dtype, device=x.device)
+    scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    if scales.numel():
+        table = _RowTable(x.data_ptr(), codes.data_ptr(), scales.data_ptr(), x.shape[-1], _ROW_FORMATS[codes_dtype],
+                          _VALUE_TYPES[x.dtype])
+        with torch.cuda.device(x.device):
+            _check(_lib.ashb_quantize_rows(scales.numel(), _c.byref(table), _stream(x.device)))
+    return codes, scales
+
+
+def read_rows(codes: torch.Tensor, scales: torch.Tensor, indices, dtype: torch.dtype) -> torch.Tensor:
+    """The values of rows kept in 8 bits, all of them or those of ``indices``."""
+    codes, scales = _cuda(codes, "codes"), _cuda(scales, "scales")
+    if indices is not None:
+        indices = _cuda(indices, "indices")
+    shape = codes.shape[:-1] if indices is None else indices.shape
+    out = torch.empty((*shape, codes.shape[-1]), dtype=dtype, device=codes.device)
+    n = shape.numel()
+    if out.numel():
+        table = _RowTable(codes.data_ptr(), out.data_ptr(), scales.data_ptr(), codes.shape[-1], _ROW_FORMATS[codes.dtype],
+                          _VALUE_TYPES[dtype])
+        with torch.cuda.device(codes.device):
+            _check(_lib.ashb_read_rows(n, None if indices is None else indices.data_ptr(), scales.numel(), _c.byref(table),
+                                       _stream(codes.device)))
+    return out
+
+
+def _rows_of(t: torch.Tensor, name: str):
+    """(2-D view or copy whose rows are contiguous, its row stride)."""
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor (there is no CPU implementation), got {t.device}")
+    width = t.shape[-1]
+    if t.dim() != 2:
+        t = t.reshape(-1, width)
+    if t.shape[0] > 1 and t.stride(0) < width or width > 1 and t.stride(1) != 1:
+        t = t.contiguous()
+    return t, t.stride(0) if t.shape[0] > 1 else width
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def rms_norm_forward(x, weight, residual, eps: float, quantize: bool, with_rstd: bool):
+    """``(y or None, codes or None, scales or None, sum or None, rstd or None)``, 2-D."""
+    x, x_stride = _rows_of(x, "x")
+    weight = _cuda(weight, "weight")
+    residual_stride = 0
+    if residual is not None:
+        residual, residual_stride = _rows_of(residual, "residual")
+    rows, width = x.shape
+    empty = lambda *shape, dtype=x.dtype: torch.empty(shape, dtype=dtype, device=x.device)
+    y = None if quantize else empty(rows, width)
+    codes = empty(rows, width, dtype=torch.float8_e4m3fn) if quantize else None
+    scales = empty(rows, dtype=torch.float32) if quantize else None
+    total = empty(rows, width) if residual is not None else None
+    rstd = empty(rows, dtype=torch.float32) if with_rstd else None
+    if rows:
+        with torch.cuda.device(x.device):
+            _check(_lib.ashb_rms_norm_forward(_VALUE_TYPES[x.dtype], x.data_ptr(), x_stride, _ptr(residual), residual_stride,
+                                              weight.data_ptr(), rows, width, eps, _ptr(y), _ptr(codes), _ptr(scales),
+                                              _ptr(total), _ptr(rstd), _stream(x.device)))
+    return y, codes, scales, total, rstd
+
+
+def rms_norm_backward(dy, dsum, s, weight, rstd):
+    """``(dx, dweight)``."""
+    dy, s, weight = _cuda(dy, "grad"), _cuda(s, "s"), _cuda(weight, "weight")
+    dsum = None if dsum is None else _cuda(dsum, "grad")
+    rows, width = s.shape
+    dx, dw = torch.empty_like(s), torch.empty_like(weight)
+    nbytes = _lib.ashb_rms_norm_workspace(rows, width)
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=s.device)
+    with torch.cuda.device(s.device):
+        _check(_lib.ashb_rms_norm_backward(_VALUE_TYPES[s.dtype], dy.data_ptr(), _ptr(dsum), s.data_ptr(), weight.data_ptr(),
+                                           rstd.data_ptr(), rows, width, dx.data_ptr(), dw.data_ptr(), _ptr(workspace), nbytes,
+                                           _stream(s.device)))
+    return dx, dw
+
+
+def linear_forward(x, weight, bias, activation: str, residual, omega: float, with_slope: bool, scales=None, out_dtype=None):
+    """``(y, slope or None)``, 2-D; ``scales``: (of x's rows, of weight's rows) where both are e4m3 codes."""
+    x, x_stride = _rows_of(x, "x")
+    weight, weight_stride = _rows_of(weight, "weight")
+    out_dtype = out_dtype or x.dtype
+    rows, inputs = x.shape
+    outputs = weight.shape[0]
+    bias = None if bias is None else _cuda(bias, "bias")
+    residual_stride = 0
+    if residual is not None:
+        residual, residual_stride = _rows_of(residual, "residual")
+    x_scales, w_scales = (None, None) if scales is None else (_cuda(scales[0], "x.scales"), _cuda(scales[1], "weight.scales"))
+    y = torch.empty((rows, outputs), dtype=out_dtype, device=x.device)
+    slope = torch.empty_like(y) if with_slope else None
+    if rows:
+        with torch.cuda.device(x.device):
+            _check(_lib.ashb_linear_forward(
+                _E4M3_ROWS if scales is not None else _VALUE_TYPES[x.dtype], x.data_ptr(), x_stride, _ptr(x_scales),
+                weight.data_ptr(), weight_stride, _ptr(w_scales), _ptr(bias), _ptr(residual), residual_stride, rows, inputs,
+                outputs, _ACTIVATIONS[activation], omega, _VALUE_TYPES[out_dtype], y.data_ptr(), _ptr(slope),
+                _stream(x.device)))
+    return y, slope
+
+
+def linear_backward(dy, slope, slope_kind: int, x, weight, want_dx: bool, want_dweight: bool, want_dbias: bool):
+    """``(dx, dweight, dbias)``, None where not wanted."""
+    dy = _cuda(dy, "grad")
+    x, x_stride = _rows_of(x, "x")
+    weight, weight_stride = _rows_of(weight, "weight")
+    rows, inputs = x.shape
+    outputs = weight.shape[0]
+    empty = lambda *shape: torch.empty(shape, dtype=dy.dtype, device=dy.device)
+    dx = empty(rows, inputs) if want_dx else None
+    dw = empty(outputs, inputs) if want_dweight else None
+    db = empty(outputs) if want_dbias else None
+    kind = _VALUE_TYPES[dy.dtype]
+    with torch.cuda.device(dy.device):
+        nbytes = _lib.ashb_linear_workspace(kind, rows, inputs, outputs, slope_kind, int(want_dweight), int(want_dbias))
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=dy.device) if nbytes else None
+        _check(_lib.ashb_linear_backward(kind, dy.data_ptr(), _ptr(slope), slope_kind, x.data_ptr(), x_stride,
+                                         weight.data_ptr(), weight_stride, rows, inputs, outputs, _ptr(dx), _ptr(dw), _ptr(db),
+                                         _ptr(workspace), nbytes, _stream(dy.device)))
+    return dx, dw, db
+
+
+def layer_timeouts(device) -> int:
+    """How many waits inside the layer kernels ran out on ``device`` (0 in a healthy run)."""
+    out = _c.c_uint()
+    with torch.cuda.device(device):
+        _check(_lib.ashb_layer_timeouts(_c.byref(out)))
+    return int(out.value)

@@ -197,6 +197,26 @@ class ASHEngine(nn.Module):
         self.backend.insert(k, values, external_values)
         self._after_insert(k.shape[0])
 
+    def insert_rows(self, keys: torch.Tensor, values: Dict[str, torch.Tensor], tables: Dict) -> None:
+        """``insert`` into tables of which some are kept in 8 bits, ``(codes, scales)`` each."""
+        assert values.keys() == tables.keys()
+        k = self._prepare(keys)
+        if k is None:
+            return
+        for v in values.values():
+            assert v.shape[0] == k.shape[0]
+        self.backend.insert_rows(k, values, tables)
+        self._after_insert(k.shape[0])
+
+    def find_rows(self, keys: torch.Tensor, tables: Dict, dtype: torch.dtype, with_indices: bool):
+        """``(indices or None, masks, {name: rows read back})`` of tables kept in 8 bits; zeros for absent keys."""
+        if keys.shape[0] == 0:
+            self._prepare(keys)
+            keys = keys.to(self.device, torch.int32)
+        else:
+            keys = self._prepare(keys)
+        return self.backend.find_rows(keys, tables, dtype, with_indices)
+
     def erase(self, keys: torch.Tensor) -> None:
         self._key_check(keys)
         if keys.shape[0] == 0:

@@ -1,0 +1,484 @@
+// Root-mean-square norm of rows, with the addition of a residual before it and, for layers served in 8 bits, a
+// quantised output after it; and its gradient.
+//
+//   s = x + r                                   (r optional; s is an output then)
+//   y = s rstd w,   rstd = (mean(s^2) + eps)^(-1/2)
+//   8 bits: the row's codes and scale by the rules of rowformat.cuh
+//   gradient, with g = dy w:  dx = dr = ds + rstd (g - s rstd^2 mean(g s)),   dw = sum over rows of dy s rstd
+//
+// Everything is memory traffic: each input is read once and each output written once, the row staying in the
+// registers of the lanes that share it between the sum of squares, the largest magnitude and the stores.  Sums are
+// float32; s enters the statistics before it is rounded to its type, the backward pass reads it rounded.  A row has
+// 8, 32 or 256 threads by its width; rows wider than 8192 are read again for each of their passes.
+// The weight's gradient is summed by a thread over the rows of its CTA, then over the CTAs in their order by a second
+// small kernel: the same bits whenever the same call is made.
+#include <algorithm>
+
+#include "rowformat.cuh"
+
+namespace ashb {
+
+struct NormArgs {
+    const void *x, *residual, *weight;
+    void *y, *sum;
+    uint8_t* codes;
+    float *scales, *rstd;
+    int64_t rows, width, x_stride, residual_stride;
+    float eps;
+};
+
+struct NormGradArgs {
+    const void *dy, *dsum, *s, *weight;
+    const float* rstd;
+    void* dx;
+    float* partial;    // [CTAs][width]
+    int64_t rows, width;
+};
+
+// Reductions over the TPR threads of a row (a CTA of 256 threads where TPR is 256; `shared` has 2 x 8 words, used in turn).
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float* shared) {
+#pragma unroll
+    for (int o = (TPR < 32 ? TPR : 32) >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if constexpr (TPR > 32) {
+        if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
+        __syncthreads();
+        v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < TPR / 32; ++w) v += shared[w];
+    }
+    return v;
+}
+template <int TPR>
+__device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* shared) {
+#pragma unroll
+    for (int o = (TPR < 32 ? TPR : 32) >> 1; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if constexpr (TPR > 32) {
+        if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
+        __syncthreads();
+        v = 0;
+#pragma unroll
+        for (int w = 0; w < TPR / 32; ++w) v = max(v, shared[w]);
+    }
+    return v;
+}
+
+// VEC values an access (one where rows or buffers are not aligned for more), NV accesses a thread.
+template <class T, int VEC, int TPR, int NV, bool QUANT>
+__global__ void __launch_bounds__(256) norm_forward_kernel(const NormArgs a) {
+    __shared__ float shared[16];
+    const int sub = threadIdx.x % TPR;
+    const int64_t row = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+    const bool live = row < a.rows;
+    const T* x = static_cast<const T*>(a.x) + (live ? row * a.x_stride : 0);
+    const T* r = a.residual ? static_cast<const T*>(a.residual) + (live ? row * a.residual_stride : 0) : nullptr;
+    const T* w = static_cast<const T*>(a.weight);
+    float v[NV][VEC];
+    float squares = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int64_t col = ((int64_t)j * TPR + sub) * VEC;
+        const bool in = live && col < a.width;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) v[j][k] = 0.0f;
+        if (in) load_n<T, VEC>(x + col, v[j]);
+    }
+    if (r != nullptr) {
+        T* s = static_cast<T*>(a.sum) + (live ? row * a.width : 0);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int64_t col = ((int64_t)j * TPR + sub) * VEC;
+            if (live && col < a.width) {
+                float u[VEC];
+                load_n<T, VEC>(r + col, u);
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) v[j][k] += u[k];
+                store_n<T, VEC>(s + col, v[j]);
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) squares = fmaf(v[j][k], v[j][k], squares);
+    squares = row_sum<TPR>(squares, shared);
+    const float rstd = 1.0f / sqrtf(squares / (float)a.width + a.eps);
+    if (a.rstd != nullptr && live && sub == 0) a.rstd[row] = rstd;
+    uint32_t amax = 0;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int64_t col = ((int64_t)j * TPR + sub) * VEC;
+        if (live && col < a.width) {
+            float u[VEC];
+            load_n<T, VEC>(w + col, u);
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) v[j][k] = v[j][k] * rstd * u[k];
+            if constexpr (QUANT) {
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) amax = max(amax, magnitude_bits(v[j][k]));
+            } else {
+                store_n<T, VEC>(static_cast<T*>(a.y) + row * a.width + col, v[j]);
+            }
+        }
+    }
+    if constexpr (QUANT) {
+        amax = row_max<TPR>(amax, reinterpret_cast<uint32_t*>(shared) + 8);
+        if (!live) return;
+        const RowScale q(amax, kFormatE4M3);
+        if (sub == 0) a.scales[row] = q.scale;
+        uint8_t* codes = a.codes + row * a.width;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int64_t col = ((int64_t)j * TPR + sub) * VEC;
+            if (col >= a.width) continue;
+            if constexpr (VEC == 1) {
+                const float u[4] = {v[j][0], 0.0f, 0.0f, 0.0f};
+                codes[col] = (uint8_t)encode4(u, q.inverse, kFormatE4M3);
+            } else {
+                uint32_t c[VEC / 4];
+#pragma unroll
+                for (int h = 0; h < VEC / 4; ++h) {
+                    const float u[4] = {v[j][4 * h], v[j][4 * h + 1], v[j][4 * h + 2], v[j][4 * h + 3]};
+                    c[h] = encode4(u, q.inverse, kFormatE4M3);
+                }
+                if constexpr (VEC == 8) *reinterpret_cast<uint2*>(codes + col) = make_uint2(c[0], c[1]);
+                else *reinterpret_cast<uint32_t*>(codes + col) = c[0];
+            }
+        }
+    }
+}
+
+// Rows beyond what registers hold: a CTA a row, x (and the residual) read once a pass.
+template <class T, bool QUANT>
+__global__ void __launch_bounds__(256) norm_forward_long_kernel(const NormArgs a) {
+    __shared__ float shared[16];
+    const int64_t row = blockIdx.x;
+    const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+    const T* r = a.residual ? static_cast<const T*>(a.residual) + row * a.residual_stride : nullptr;
+    const T* w = static_cast<const T*>(a.weight);
+    const auto value = [&](int64_t c) { return to_float(x[c]) + (r ? to_float(r[c]) : 0.0f); };
+    float squares = 0.0f;
+    for (int64_t c = threadIdx.x; c < a.width; c += 256) {
+        const float v = value(c);
+        squares = fmaf(v, v, squares);
+    }
+    squares = row_sum<256>(squares, shared);
+    const float rstd = 1.0f / sqrtf(squares / (float)a.width + a.eps);
+    if (a.rstd != nullptr && threadIdx.x == 0) a.rstd[row] = rstd;
+    uint32_t amax = 0;
+    for (int64_t c = threadIdx.x; c < a.width; c += 256) {
+        const float v = value(c), y = v * rstd * to_float(w[c]);
+        amax = max(amax, magnitude_bits(y));
+        if constexpr (!QUANT) {
+            static_cast<T*>(a.y)[row * a.width + c] = from_float<T>(y);
+            if (r) static_cast<T*>(a.sum)[row * a.width + c] = from_float<T>(v);
+        }
+    }
+    if constexpr (QUANT) {
+        amax = row_max<256>(amax, reinterpret_cast<uint32_t*>(shared) + 8);
+        const RowScale q(amax, kFormatE4M3);
+        if (threadIdx.x == 0) a.scales[row] = q.scale;
+        for (int64_t c = threadIdx.x; c < a.width; c += 256) {
+            const float v = value(c);
+            const float u[4] = {v * rstd * to_float(w[c]), 0.0f, 0.0f, 0.0f};
+            a.codes[row * a.width + c] = (uint8_t)encode4(u, q.inverse, kFormatE4M3);
+            if (r) static_cast<T*>(a.sum)[row * a.width + c] = from_float<T>(v);
+        }
+    }
+}
+
+// Rows in turn, so that a thread keeps the weight's gradient of its columns in registers.
+template <class T, int VEC, int TPR, int NV>
+__global__ void __launch_bounds__(256) norm_backward_kernel(const NormGradArgs a) {
+    __shared__ float shared[16];
+    extern __shared__ float columns[];     // width: the CTA's sums
+    constexpr int kGroups = 256 / TPR;
+    const int sub = threadIdx.x % TPR, group = threadIdx.x / TPR;
+    const T* w = static_cast<const T*>(a.weight);
+    float dw[NV][VEC];
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) dw[j][k] = 0.0f;
+    int turn = 0;
+    for (int64_t first = (int64_t)blockIdx.x * kGroups; first < a.rows; first += (int64_t)gridDim.x * kGroups) {
+        const int64_t row = first + group;
+        const bool live = row < a.rows;
+        const int64_t at = live ? row * a.width : 0;
+        const float rstd = live ? a.rstd[row] : 0.0f;
+        float s[NV][VEC], g[NV][VEC];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int64_t col = ((int64_t)j * TPR + sub) * VEC;
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) s[j][k] = g[j][k] = 0.0f;
+            if (live && col < a.width) {
+                load_n<T, VEC>(static_cast<const T*>(a.s) + at + col, s[j]);
+                load_n<T, VEC>(static_cast<const T*>(a.dy) + at + col, g[j]);
+            }
+        }
+        float dot = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int64_t col = ((int64_t)j * TPR + sub) * VEC;
+            if (col < a.width) {
+                float u[VEC];
+                load_n<T, VEC>(w + col, u);
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) {
+                    dw[j][k] = fmaf(g[j][k] * s[j][k], rstd, dw[j][k]);
+                    g[j][k] *= u[k];
+                    dot = fmaf(g[j][k], s[j][k], dot);
+                }
+            }
+        }
+        // the sums of two rows in turn go through different words: no second barrier
+        dot = row_sum<TPR>(dot, shared + 8 * turn);
+        turn ^= 1;
+        const float c = rstd * rstd * (dot / (float)a.width);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int64_t col = ((int64_t)j * TPR + sub) * VEC;
+            if (live && col < a.width) {
+                float u[VEC];
+                if (a.dsum != nullptr) load_n<T, VEC>(static_cast<const T*>(a.dsum) + at + col, u);
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) {
+                    const float d = rstd * fmaf(-s[j][k], c, g[j][k]);
+                    u[k] = a.dsum != nullptr ? u[k] + d : d;
+                }
+                store_n<T, VEC>(static_cast<T*>(a.dx) + at + col, u);
+            }
+        }
+    }
+    // the groups of the CTA add to its sums one after another
+    for (int owner = 0; owner < kGroups; ++owner) {
+        if (group == owner) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) {
+                    const int64_t col = ((int64_t)j * TPR + sub) * VEC + k;
+                    if (col < a.width) columns[col] = owner == 0 ? dw[j][k] : columns[col] + dw[j][k];
+                }
+        }
+        __syncthreads();
+    }
+    for (int64_t col = threadIdx.x; col < a.width; col += 256) a.partial[blockIdx.x * a.width + col] = columns[col];
+}
+
+// Rows beyond registers: a CTA a row in turn, the CTA's sums in its row of `partial` from the start.
+template <class T>
+__global__ void __launch_bounds__(256) norm_backward_long_kernel(const NormGradArgs a) {
+    __shared__ float shared[16];
+    const T* w = static_cast<const T*>(a.weight);
+    float* sums = a.partial + blockIdx.x * a.width;
+    for (int64_t c = threadIdx.x; c < a.width; c += 256) sums[c] = 0.0f;
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T* s = static_cast<const T*>(a.s) + row * a.width;
+        const T* dy = static_cast<const T*>(a.dy) + row * a.width;
+        const T* ds = a.dsum ? static_cast<const T*>(a.dsum) + row * a.width : nullptr;
+        const float rstd = a.rstd[row];
+        float dot = 0.0f;
+        for (int64_t c = threadIdx.x; c < a.width; c += 256) {
+            const float sv = to_float(s[c]), dv = to_float(dy[c]);
+            sums[c] = fmaf(dv * sv, rstd, sums[c]);
+            dot = fmaf(dv * to_float(w[c]), sv, dot);
+        }
+        dot = row_sum<256>(dot, shared + 8 * turn);
+        turn ^= 1;
+        const float q = rstd * rstd * (dot / (float)a.width);
+        for (int64_t c = threadIdx.x; c < a.width; c += 256) {
+            const float d = rstd * fmaf(-to_float(s[c]), q, to_float(dy[c]) * to_float(w[c]));
+            static_cast<T*>(a.dx)[row * a.width + c] = from_float<T>(ds ? to_float(ds[c]) + d : d);
+        }
+    }
+}
+
+// Columns summed over the CTAs' rows: 8 warps share the CTAs of 32 columns, joined in order.
+template <class T>
+__global__ void __launch_bounds__(256) column_sums_kernel(const float* __restrict__ partial, int64_t n, int64_t width,
+                                                          T* __restrict__ out) {
+    __shared__ float mine[8][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t col = (int64_t)blockIdx.x * 32 + lane;
+    float v = 0.0f;
+    if (col < width)
+        for (int64_t i = warp; i < n; i += 8) v += partial[i * width + col];
+    mine[warp][lane] = v;
+    __syncthreads();
+    if (warp == 0 && col < width) {
+        float t = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) t += mine[w][lane];
+        out[col] = from_float<T>(t);
+    }
+}
+
+// ---- launches ----------------------------------------------------------------------------------------------------
+constexpr int64_t kLongRow = 8192;
+
+// Threads a row and accesses a thread for a width: as few threads as keep 32 values or less each, so that narrow rows
+// leave no lane idle; the largest NV of a vector width is 32 / VEC.
+template <class F>
+static void by_width(int64_t width, int vec, F&& f) {
+    const int tpr = width <= 64 ? 8 : width <= 1024 ? 32 : 256;
+    int nv = 1;
+    while ((int64_t)nv * vec * tpr < width) nv <<= 1;
+    f(tpr, nv);
+}
+
+template <class T, int VEC, int TPR, bool QUANT>
+static void launch_forward(const NormArgs& a, int nv, cudaStream_t st) {
+    const unsigned grid = (unsigned)((a.rows + 256 / TPR - 1) / (256 / TPR));
+    switch (nv) {
+        case 1: norm_forward_kernel<T, VEC, TPR, 1, QUANT><<<grid, 256, 0, st>>>(a); break;
+        case 2: norm_forward_kernel<T, VEC, TPR, 2, QUANT><<<grid, 256, 0, st>>>(a); break;
+        case 4: norm_forward_kernel<T, VEC, TPR, 4, QUANT><<<grid, 256, 0, st>>>(a); break;
+        default:
+            if constexpr (VEC <= 4) {
+                if (nv == 8) { norm_forward_kernel<T, VEC, TPR, 8, QUANT><<<grid, 256, 0, st>>>(a); break; }
+            }
+            if constexpr (VEC == 1 && TPR >= 32) {
+                if (nv == 16) { norm_forward_kernel<T, VEC, TPR, 16, QUANT><<<grid, 256, 0, st>>>(a); break; }
+                norm_forward_kernel<T, VEC, TPR, 32, QUANT><<<grid, 256, 0, st>>>(a);
+            }
+    }
+}
+
+template <class T, int VEC, bool QUANT>
+static void forward_by_width(const NormArgs& a, cudaStream_t st) {
+    by_width(a.width, VEC, [&](int tpr, int nv) {
+        if (tpr == 8) launch_forward<T, VEC, 8, QUANT>(a, nv, st);
+        else if (tpr == 32) launch_forward<T, VEC, 32, QUANT>(a, nv, st);
+        else launch_forward<T, VEC, 256, QUANT>(a, nv, st);
+    });
+}
+
+// Whether every pointer is a multiple of `bytes` (null is).
+static bool aligned(uintptr_t bytes, std::initializer_list<const void*> pointers) {
+    uintptr_t bits = 0;
+    for (const void* p : pointers) bits |= (uintptr_t)p;
+    return bits % bytes == 0;
+}
+
+template <class T>
+static void forward_typed(const NormArgs& a, cudaStream_t st) {
+    constexpr int kVec = 16 / sizeof(T);
+    const bool wide = a.width % kVec == 0 && a.x_stride % kVec == 0 && a.residual_stride % kVec == 0 &&
+                      aligned(16, {a.x, a.residual, a.weight, a.y, a.sum}) && aligned(kVec, {a.codes});
+    if (a.width > kLongRow) {
+        if (a.codes) norm_forward_long_kernel<T, true><<<(unsigned)a.rows, 256, 0, st>>>(a);
+        else norm_forward_long_kernel<T, false><<<(unsigned)a.rows, 256, 0, st>>>(a);
+    } else if (wide) {
+        if (a.codes) forward_by_width<T, kVec, true>(a, st);
+        else forward_by_width<T, kVec, false>(a, st);
+    } else {
+        if (a.codes) forward_by_width<T, 1, true>(a, st);
+        else forward_by_width<T, 1, false>(a, st);
+    }
+}
+
+// CTAs of the backward pass: what is resident at once, and no more than there are rows for.
+static unsigned backward_ctas(int64_t rows, int64_t width) {
+    const int groups = width <= 64 ? 32 : width <= 1024 ? 8 : 1;
+    return (unsigned)std::max<int64_t>(1, std::min<int64_t>((rows + groups - 1) / groups, (int64_t)sm_count() * 4));
+}
+
+template <class T, int VEC, int TPR>
+static void launch_backward(const NormGradArgs& a, int nv, unsigned grid, cudaStream_t st) {
+    const size_t smem = (size_t)a.width * 4;
+    switch (nv) {
+        case 1: norm_backward_kernel<T, VEC, TPR, 1><<<grid, 256, smem, st>>>(a); break;
+        case 2: norm_backward_kernel<T, VEC, TPR, 2><<<grid, 256, smem, st>>>(a); break;
+        case 4: norm_backward_kernel<T, VEC, TPR, 4><<<grid, 256, smem, st>>>(a); break;
+        default:
+            if constexpr (VEC <= 4) {
+                if (nv == 8) { norm_backward_kernel<T, VEC, TPR, 8><<<grid, 256, smem, st>>>(a); break; }
+            }
+            if constexpr (VEC == 1 && TPR >= 32) {
+                if (nv == 16) { norm_backward_kernel<T, VEC, TPR, 16><<<grid, 256, smem, st>>>(a); break; }
+                norm_backward_kernel<T, VEC, TPR, 32><<<grid, 256, smem, st>>>(a);
+            }
+    }
+}
+
+template <class T>
+static void backward_typed(const NormGradArgs& a, unsigned grid, void* dw, cudaStream_t st) {
+    constexpr int kVec = 16 / sizeof(T);
+    if (a.width > kLongRow) {
+        norm_backward_long_kernel<T><<<grid, 256, 0, st>>>(a);
+    } else {
+        const bool wide = a.width % kVec == 0 && aligned(16, {a.dy, a.dsum, a.s, a.weight, a.dx});
+        const auto go = [&](auto vec) {
+            constexpr int VEC = decltype(vec)::value;
+            by_width(a.width, VEC, [&](int tpr, int nv) {
+                if (tpr == 8) launch_backward<T, VEC, 8>(a, nv, grid, st);
+                else if (tpr == 32) launch_backward<T, VEC, 32>(a, nv, grid, st);
+                else launch_backward<T, VEC, 256>(a, nv, grid, st);
+            });
+        };
+        if (wide) go(std::integral_constant<int, kVec>{});
+        else go(std::integral_constant<int, 1>{});
+    }
+    column_sums_kernel<T><<<(unsigned)((a.width + 31) / 32), 256, 0, st>>>(a.partial, grid, a.width, static_cast<T*>(dw));
+}
+
+}  // namespace ashb
+
+using namespace ashb;
+
+extern "C" {
+
+int ashb_rms_norm_forward(int dtype, const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                          const void* weight, int64_t rows, int64_t width, float eps, void* y, uint8_t* codes,
+                          float* scales, void* sum, float* rstd, void* stream) {
+    ASHB_REQUIRE(is_value_type(dtype), "value type %d", dtype);
+    ASHB_REQUIRE(rows >= 0 && rows <= 0x7FFFFFFF && width >= 1 && width <= 1 << 30, "%lld rows of %lld", (long long)rows,
+                 (long long)width);
+    if (rows == 0) return ASHB_OK;
+    ASHB_REQUIRE(x && weight && (y != nullptr) != (codes != nullptr) && (codes == nullptr) == (scales == nullptr) &&
+                         (residual == nullptr) == (sum == nullptr),
+                 "null buffer, or neither or both kinds of output");
+    ASHB_REQUIRE(x_stride >= width || rows == 1, "rows overlap");
+    ASHB_REQUIRE(aligned(value_bytes(dtype), {x, residual, weight, y, sum}), "buffers not aligned to their type");
+    const NormArgs a{x, residual, weight, y, sum, codes, scales, rstd, rows, width, x_stride, residual ? residual_stride : 0, eps};
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == ASHB_F32) forward_typed<float>(a, st);
+    else if (dtype == ASHB_F16) forward_typed<__half>(a, st);
+    else forward_typed<__nv_bfloat16>(a, st);
+    ASHB_LAUNCH_CHECK();
+    return ASHB_OK;
+}
+
+int64_t ashb_rms_norm_workspace(int64_t rows, int64_t width) {
+    if (rows <= 0 || width <= 0) return 0;
+    return (int64_t)backward_ctas(rows, width) * width * (int64_t)sizeof(float);
+}
+
+int ashb_rms_norm_backward(int dtype, const void* dy, const void* dsum, const void* s, const void* weight, const float* rstd,
+                           int64_t rows, int64_t width, void* dx, void* dweight, void* workspace, int64_t workspace_bytes,
+                           void* stream) {
+    ASHB_REQUIRE(is_value_type(dtype), "value type %d", dtype);
+    ASHB_REQUIRE(rows >= 0 && rows <= 0x7FFFFFFF && width >= 1 && width <= 1 << 30, "%lld rows of %lld", (long long)rows,
+                 (long long)width);
+    ASHB_REQUIRE(dweight != nullptr, "null buffer");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (rows == 0) {
+        ASHB_CUDA_TRY(cudaMemsetAsync(dweight, 0, (size_t)(width * value_bytes(dtype)), st));
+        return ASHB_OK;
+    }
+    ASHB_REQUIRE(dy && s && weight && rstd && dx && workspace, "null buffer");
+    ASHB_REQUIRE(workspace_bytes >= ashb_rms_norm_workspace(rows, width) && aligned(4, {workspace}), "small workspace");
+    ASHB_REQUIRE(aligned(value_bytes(dtype), {dy, dsum, s, weight, dx, dweight}), "buffers not aligned to their type");
+    const NormGradArgs a{dy, dsum, s, weight, rstd, dx, static_cast<float*>(workspace), rows, width};
+    const unsigned grid = backward_ctas(rows, width);
+    if (dtype == ASHB_F32) backward_typed<float>(a, grid, dweight, st);
+    else if (dtype == ASHB_F16) backward_typed<__half>(a, grid, dweight, st);
+    else backward_typed<__nv_bfloat16>(a, grid, dweight, st);
+    ASHB_LAUNCH_CHECK();
+    return ASHB_OK;
+}
+
+}  // extern "C"
