@@ -18,7 +18,7 @@
 // becomes NaN: its mid part is infinity less infinity.)
 //
 // Shape of a CTA, one per SM and looping over tiles of 128 x bn: loaders fill a ring of shared-memory stages, one thread
-// issues the products, and eight warps finish the tile before in the other half of tensor memory.  Loaders are one thread
+// issues the products, and eight warps finish the tiles before, whose sums are in tensor memory.  Loaders are one thread
 // with tiled bulk copies where types are 8 or 16 bits and rows are multiples of 16 bytes, else seven warps with loads of
 // their own, which take any size and alignment and split float32 on the way.
 // A layer's rows are long and few values wide as often as not: then the kernel is bound by memory, and a weight tile that
@@ -35,46 +35,114 @@ namespace ashb {
 
 constexpr int kRowBytes = 128;            // of a tile row: 64 values of 16 bits, 128 of 8
 constexpr int kTileM = 128;
-constexpr int kLoaders = 7, kFinishers = 8;             // warps; the one between them issues the products: 16 in all, 128 registers
-constexpr int kGemmThreads = (kLoaders + kFinishers + 1) * 32;
+// Warps, 16 in all (128 registers): with loads of their own seven loaders, one that issues the products and eight that finish
+// tiles; with bulk copies one loader, one for the products, two that idle, and eight or twelve that finish.
+constexpr int kGemmThreads = 512, kLoaders = 7;
+template <bool BULK>
+constexpr int kProductWarp = BULK ? 1 : kLoaders;
+template <bool BULK>
+constexpr int kFirstFinisher = BULK ? 4 : 8;
 constexpr int kPhaseBlocks = 8;           // blocks of 64 between the float32 sums of split products
 constexpr int kMaxStages = 8;
+constexpr int kMaxSlots = 8;              // tiles whose sums are in tensor memory
 constexpr size_t kSharedLimit = 232448;
-constexpr size_t kFinishBytes = kFinishers * 32 * 32 * sizeof(float);
+constexpr size_t kFinishBytes = 4 * 32 * 32 * sizeof(float);      // of a group of four finishers
 
 enum Activation { kNone = ASHB_ACT_NONE, kRelu = ASHB_ACT_RELU, kSilu = ASHB_ACT_SILU, kGelu = ASHB_ACT_GELU, kSin = ASHB_ACT_SIN };
 
 __device__ unsigned int g_layer_timeouts = 0;
 
 // ---- activations -----------------------------------------------------------------------------------------------------
-// act(z) and, where SLOPE, act'(z).  ROUNDED: the results are rounded to 16 bits, for which the hardware's exponential
-// (2^-21 of the value) is exact enough; float32 results take the library's.
+// Short and without branches, so that a block's 32 values a lane are straight code.  ROUNDED: the results are rounded to 16
+// bits, for which the hardware's exponential and reciprocal (2^-21 of the value) are exact enough.
+
+// sin(x + turn pi / 2), turn 0 or 1.  Reduction by a multiple k of pi in two parts (W. J. Cody, W. Waite, Software Manual for
+// the Elementary Functions, 1980): k times the first part is a multiple of x's last place, so the first step is exact.
+// Then the Taylor series to the 13th power, whose remainder within pi / 2 is below 2^-29.  Phases beyond 2^17, where a
+// float32 phase is good to 2^-7 at best, take the library's reduction.
+constexpr float kLongPhase = 131072.0f;
+__device__ __noinline__ float long_phase(float x, int turn) { return turn ? cosf(x) : sinf(x); }
+
+template <int TURN>
+__device__ __forceinline__ float short_phase(float x) {
+    constexpr float kRound = 12582912.0f;             // 1.5 * 2^23: what is added to it is rounded to a whole number
+    // cos x = (-1)^(m+1) sin(x - (m + 1/2) pi)
+    const float m = TURN ? __fadd_rn(fmaf(x, 0.318309886f, -0.5f), kRound) : fmaf(x, 0.318309886f, kRound);
+    const uint32_t sign = (__float_as_uint(m) << 31) ^ (TURN ? 0x80000000u : 0u);
+    const float k = __fadd_rn(m, -kRound) + (TURN ? 0.5f : 0.0f);
+    float r = fmaf(-k, 3.14159274f, x);               // pi rounded to float32
+    r = fmaf(-k, -8.74227766e-8f, r);                 // and what that leaves
+    const float u = r * r;
+    float p = fmaf(u, 1.6059044e-10f, -2.5052108e-8f);      // 1/13!, -1/11!
+    p = fmaf(u, p, 2.7557319e-6f);
+    p = fmaf(u, p, -1.9841270e-4f);
+    p = fmaf(u, p, 8.3333333e-3f);
+    p = fmaf(u, p, -1.6666667e-1f);
+    return __uint_as_float(__float_as_uint(fmaf(u * r, p, r)) ^ sign);
+}
+
+// act(z) and, where SLOPE, act'(z); not of a sine's long phases.
 template <int ACT, bool SLOPE, bool ROUNDED>
-__device__ __forceinline__ float activate(float omega, float z, float& slope) {
+__device__ __forceinline__ float activate_one(float omega, float z, float& slope) {
     if constexpr (ACT == kRelu) {
         if (SLOPE) slope = z > 0.0f ? 1.0f : 0.0f;
         return z < 0.0f ? 0.0f : z;      // a NaN stays
     } else if constexpr (ACT == kSilu) {
-        const float e = ROUNDED ? __expf(-z) : expf(-z);
-        const float p = ROUNDED ? __fdividef(1.0f, 1.0f + e) : 1.0f / (1.0f + e);
+        const float p = __fdividef(1.0f, 1.0f + (ROUNDED ? __expf(-z) : expf(-z)));
         if (SLOPE) slope = p * fmaf(z, 1.0f - p, 1.0f);
         return z * p;
     } else if constexpr (ACT == kGelu) {
-        const float c = 0.5f * (1.0f + erff(z * 0.70710678f));
-        if (SLOPE) slope = fmaf(z * 0.39894228f, ROUNDED ? __expf(-0.5f * z * z) : expf(-0.5f * z * z), c);
-        return z * c;
-    } else if constexpr (ACT == kSin) {
-        if (SLOPE) {
-            float s, co;
-            sincosf(omega * z, &s, &co);
-            slope = omega * co;
-            return s;
+        if constexpr (ROUNDED) {
+            // erf by formula 7.1.26 of M. Abramowitz and I. Stegun, Handbook of Mathematical Functions: good to 1.5e-7; its
+            // exponential is the density that the slope wants
+            const float x = fabsf(z) * 0.70710678f, t = __fdividef(1.0f, fmaf(0.3275911f, x, 1.0f));
+            float p = fmaf(t, 1.061405429f, -1.453152027f);
+            p = fmaf(t, p, 1.421413741f);
+            p = fmaf(t, p, -0.284496736f);
+            p = fmaf(t, p, 0.254829592f);
+            const float e = __expf(-x * x), tail = 0.5f * p * t * e, c = z < 0.0f ? tail : 1.0f - tail;
+            if (SLOPE) slope = fmaf(z * 0.39894228f, e, c);
+            return z * c;
+        } else {
+            const float c = 0.5f * (1.0f + erff(z * 0.70710678f));
+            if (SLOPE) slope = fmaf(z * 0.39894228f, expf(-0.5f * z * z), c);
+            return z * c;
         }
-        return sinf(omega * z);
+    } else if constexpr (ACT == kSin) {
+        if (SLOPE) slope = omega * short_phase<1>(omega * z);
+        return short_phase<0>(omega * z);
     } else {
         if (SLOPE) slope = 1.0f;
         return z;
     }
+}
+
+// N values in place and their slopes.  Long phases are looked for once for all of them: a branch per value would keep the
+// values from being worked on side by side.
+template <int ACT, bool SLOPE, bool ROUNDED, int N>
+__device__ __forceinline__ void activate(float omega, float (&z)[N], float (&slope)[N]) {
+    if constexpr (ACT == kSin) {
+        float most = 0.0f;
+#pragma unroll
+        for (int k = 0; k < N; ++k) most = fmaxf(most, fabsf(omega * z[k]));     // a NaN takes either way
+        if (most > kLongPhase) {
+#pragma unroll 1
+            for (int k = 0; k < N; ++k) {
+                float x = 0.0f;
+#pragma unroll
+                for (int j = 0; j < N; ++j) x = j == k ? omega * z[j] : x;
+                const float s = long_phase(x, 0), c = SLOPE ? omega * long_phase(x, 1) : 0.0f;
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    z[j] = j == k ? s : z[j];
+                    if (SLOPE) slope[j] = j == k ? c : slope[j];
+                }
+            }
+            return;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) z[k] = activate_one<ACT, SLOPE, ROUNDED>(omega, z[k], slope[k]);
 }
 
 // f(std::integral_constant<int, activation>), so that a launch runs the code of one activation: with the choice made
@@ -96,7 +164,7 @@ enum Kind { kHalf, kSplit, kEight };     // operands: 16 bits, float32 in three 
 struct Operand {
     const void* at;
     int64_t stride;      // values between rows
-    int wide;            // rows start at multiples of 16 bytes
+    int wide;            // rows start and end at multiples of 16 bytes
 };
 
 struct Finish {          // what becomes of the sums
@@ -112,52 +180,54 @@ struct Finish {          // what becomes of the sums
 struct GemmArgs {
     Operand a, b;
     Finish f;
-    int64_t m, n, k, k_split;              // k_split: of a split, a multiple of a stage's
-    int64_t tiles_m, tiles_n, items;
+    int64_t m, n, k;
+    uint32_t tiles_m, tiles_n, tiles, items;             // tiles = tiles_m * tiles_n, items = tiles * splits
+    uint32_t splits, blocks_k, split_blocks, block_k;    // stages along k: all, of a split; values of a stage
     uint32_t desc;
-    int bn, stages, b_stays, columns;      // columns: tensor memory to allocate
+    int bn, stages, slots, groups, b_stays, columns;      // groups: of four finishers; columns: tensor memory to allocate
 };
 
-// Eight consecutive values of an operand as one 16-byte word per part.
+// Consecutive values of an operand that make one 16-byte word of each of its parts, at p; `left` of them exist, none if it is
+// not positive.  WIDE: all or none do, on 16-byte boundaries; the loads are predicated, so that nothing waits for them here.
 struct Eight32 { float v[8]; };
 struct Eight16 { uint4 w; };
+struct Sixteen8 { uint4 w; };
 
 template <bool WIDE>
-__device__ __forceinline__ void fetch8(Eight32& e, const Operand& o, int64_t row, int64_t col, int64_t rows, int64_t cols) {
-    const float* p = static_cast<const float*>(o.at) + row * o.stride + col;
-    if (WIDE && row < rows && col + 8 <= cols) {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+__device__ __forceinline__ void fetch_word(Eight32& e, const float* p, int left) {
+    if (WIDE) {
+        float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f), b = a;
+        if (left >= 4) a = __ldg(reinterpret_cast<const float4*>(p));
+        if (left >= 8) b = __ldg(reinterpret_cast<const float4*>(p) + 1);
         e.v[0] = a.x; e.v[1] = a.y; e.v[2] = a.z; e.v[3] = a.w;
         e.v[4] = b.x; e.v[5] = b.y; e.v[6] = b.z; e.v[7] = b.w;
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) e.v[j] = row < rows && col + j < cols ? __ldg(p + j) : 0.0f;
+        for (int j = 0; j < 8; ++j) e.v[j] = j < left ? __ldg(p + j) : 0.0f;
     }
 }
 template <bool WIDE>
-__device__ __forceinline__ void fetch8(Eight16& e, const Operand& o, int64_t row, int64_t col, int64_t rows, int64_t cols) {
-    const uint16_t* p = static_cast<const uint16_t*>(o.at) + row * o.stride + col;
-    if (WIDE && row < rows && col + 8 <= cols) {
-        e.w = __ldg(reinterpret_cast<const uint4*>(p));
+__device__ __forceinline__ void fetch_word(Eight16& e, const uint16_t* p, int left) {
+    e.w = make_uint4(0, 0, 0, 0);
+    if (WIDE) {
+        if (left >= 8) e.w = __ldg(reinterpret_cast<const uint4*>(p));
     } else {
         uint32_t h[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) h[j] = row < rows && col + j < cols ? (uint32_t)__ldg(p + j) : 0u;
+        for (int j = 0; j < 8; ++j) h[j] = j < left ? (uint32_t)__ldg(p + j) : 0u;
         e.w = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
     }
 }
-// e4m3: sixteen values.
-struct Sixteen8 { uint4 w; };
 template <bool WIDE>
-__device__ __forceinline__ void fetch8(Sixteen8& e, const Operand& o, int64_t row, int64_t col, int64_t rows, int64_t cols) {
-    const uint8_t* p = static_cast<const uint8_t*>(o.at) + row * o.stride + col;
-    if (WIDE && row < rows && col + 16 <= cols) {
-        e.w = __ldg(reinterpret_cast<const uint4*>(p));
+__device__ __forceinline__ void fetch_word(Sixteen8& e, const uint8_t* p, int left) {
+    e.w = make_uint4(0, 0, 0, 0);
+    if (WIDE) {
+        if (left >= 16) e.w = __ldg(reinterpret_cast<const uint4*>(p));
     } else {
         uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int j = 0; j < 16; ++j)
-            if (row < rows && col + j < cols) w[j / 4] |= (uint32_t)__ldg(p + j) << (8 * (j % 4));
+            if (j < left) w[j / 4] |= (uint32_t)__ldg(p + j) << (8 * (j % 4));
         e.w = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
@@ -202,11 +272,12 @@ __host__ __device__ constexpr uint32_t part_bytes(int extent) {
     return DOWN ? (uint32_t)((extent + 63) / 64) * 64u * kRowBytes : (uint32_t)extent * kRowBytes;
 }
 
-// A stage's tile of an operand by loads of the loader warps' own: CHUNKS chunks a thread.
-// Chunk `i` of a tile: along rows, row i / 8 and word i % 8; down rows, word i % 8 of row (i / 8) % 64 of box i / 512.
+// A stage's tile of an operand by loads of the loader warps' own: CHUNKS words a thread.
+// Word `i` of a tile: along rows, row i / 8 and word i % 8; down rows, word i % 8 of row (i / 8) % 64 of box i / 512.
 template <int KIND, bool DOWN, int CHUNKS>
 struct TileFetch {
     using Chunk = typename KindOf<KIND>::Chunk;
+    using Value = std::conditional_t<KIND == kSplit, float, std::conditional_t<KIND == kEight, uint8_t, uint16_t>>;
     static constexpr int kValues = KIND == kEight ? 16 : 8;
     Chunk c[CHUNKS];
 
@@ -219,15 +290,18 @@ struct TileFetch {
     template <bool WIDE>
     __device__ __forceinline__ void fetch_as(const Operand& o, int thread, int total, int64_t across0, int64_t across,
                                              int64_t k0, int64_t k, int words) {
+        const Value* tile = static_cast<const Value*>(o.at) + (DOWN ? k0 * o.stride + across0 : across0 * o.stride + k0);
+        const int across_left = (int)min(across - across0, (int64_t)1024), k_left = (int)min(k - k0, (int64_t)1024);
 #pragma unroll
         for (int j = 0; j < CHUNKS; ++j) {
             const int i = thread + j * kLoaders * 32;
-            if (i >= total) break;
             if (DOWN) {
-                const int r = (i >> 3) & 63;
-                if (r < words * 8) fetch8<WIDE>(c[j], o, k0 + r, across0 + (int64_t)(i >> 9) * 64 + (i & 7) * 8, k, across);
-            } else if ((i & 7) < words) {
-                fetch8<WIDE>(c[j], o, across0 + (i >> 3), k0 + (int64_t)(i & 7) * kValues, across, k);
+                const int r = (i >> 3) & 63, col = (i >> 9) * 64 + (i & 7) * 8;
+                fetch_word<WIDE>(c[j], tile + r * o.stride + col, i < total && r < k_left ? across_left - col : 0);
+            } else {
+                const int r = i >> 3, col = (i & 7) * kValues;
+                fetch_word<WIDE>(c[j], tile + r * o.stride + col,
+                                 i < total && (i & 7) < words && r < across_left ? k_left - col : 0);
             }
         }
     }
@@ -244,15 +318,41 @@ struct TileFetch {
 };
 
 // Order of the tiles: bands of 8 rows of tiles, down the band first, so that the tiles in flight share operands in L2.
-__device__ __forceinline__ void tile_of(const GemmArgs& g, int64_t item, int64_t& tm, int64_t& tn, int64_t& split) {
-    const int64_t tiles = g.tiles_m * g.tiles_n;
-    split = item / tiles;
-    const int64_t t = item - split * tiles;
-    const int64_t band = t / (8 * g.tiles_n), in = t - band * 8 * g.tiles_n;
-    const int64_t high = min((int64_t)8, g.tiles_m - band * 8);
-    tn = in / high;
-    tm = band * 8 + in - tn * high;
+// In 32 bits throughout: with 64-bit quotients per stage and tile the threads that issue copies and products spent more time
+// dividing than anything else.
+struct Tile {
+    int m, n, split, blocks;      // blocks: stages along k
+    int64_t k0;
+};
+__device__ __forceinline__ Tile tile_of(const GemmArgs& g, uint32_t item) {
+    Tile t{(int)item, 0, 0, 0, 0};
+    if (g.splits > 1) {
+        t.split = (int)(item / g.tiles);
+        item -= (uint32_t)t.split * g.tiles;
+        t.m = (int)item;
+    }
+    if (g.tiles_n > 1) {
+        const uint32_t band = item / (8u * g.tiles_n), in = item - band * 8u * g.tiles_n;
+        const uint32_t high = min(8u, g.tiles_m - band * 8u);
+        t.n = (int)(in / high);
+        t.m = (int)(band * 8u + in - (uint32_t)t.n * high);
+    }
+    t.k0 = (int64_t)t.split * g.split_blocks * g.block_k;
+    t.blocks = (int)min(g.split_blocks, g.blocks_k - (uint32_t)t.split * g.split_blocks);
+    return t;
 }
+
+// A place in the ring of stages, or of the tiles in tensor memory, and the parity of its next phase.
+struct Turn {
+    int at = 0;
+    uint32_t parity = 0;
+    __device__ __forceinline__ void next(int size) {
+        if (++at == size) {
+            at = 0;
+            parity ^= 1u;
+        }
+    }
+};
 
 // The sums of a warp's 32 x 32 block, from registers (a row a thread) through shared memory to memory (rows whole).
 __device__ __forceinline__ void put_block(float* block, int lane, const float (&r)[32]) {
@@ -262,54 +362,103 @@ __device__ __forceinline__ void put_block(float* block, int lane, const float (&
                 make_float4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
 }
 
-// Four values a lane, four rows a pass.  The residuals of four passes are fetched together.
+// What a lane of finish_wide wants besides the sums, fetched before they are waited for: its columns' bias and scales, and the
+// residuals of the first four of its eight passes.
+template <class T>
+struct Ahead {
+    using Four = typename Word<4 * sizeof(T)>::type;
+    Four bias, residual[4];
+    float4 scales;
+    __device__ __forceinline__ void fetch(const Finish& f, int lane, int64_t row0, int64_t col0, int64_t m, int64_t n) {
+        if (!f.wide) return;
+        const int64_t col = col0 + 4 * (lane & 7);
+        if (col >= n) return;
+        if (f.bias) bias = __ldg(reinterpret_cast<const Four*>(static_cast<const T*>(f.bias) + col));
+        if (f.b_scales) scales = __ldg(reinterpret_cast<const float4*>(f.b_scales + col));
+        if (f.residual) {
+            const int64_t row = row0 + (lane >> 3);
+            const T* p = static_cast<const T*>(f.residual) + row * f.residual_stride + col;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (row + 4 * i < m) residual[i] = __ldg(reinterpret_cast<const Four*>(p + 4 * i * f.residual_stride));
+        }
+    }
+};
+
+// Four values a lane, four rows a pass, two passes a round.  A loop, so that its code stays where instructions are fetched
+// from (in one piece of eight passes half of the cycles went by waiting for code), with the next round's sums and the round
+// after that's residuals under way: what a round stores may be the same memory for all that the compiler knows, so a read
+// written after it would wait for it.
 template <class T, int ACT, bool SLOPE>
-__device__ __forceinline__ void finish_wide(const Finish& f, const float* block, int lane, int64_t row0, int64_t col0, int64_t m,
-                                            int64_t n) {
+__device__ __forceinline__ void finish_wide(const Finish& f, const float* block, Ahead<T>& ahead, int lane, int64_t row0,
+                                            int64_t col0, int64_t m, int64_t n) {
     constexpr bool kRounded = sizeof(T) == 2;
     const int q = lane & 7, sub = lane >> 3;
     const int64_t col = col0 + 4 * q;
     if (col >= n) return;
-    float b[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sb[4] = {1.0f, 1.0f, 1.0f, 1.0f};
-    if (f.bias) load_n<T, 4>(static_cast<const T*>(f.bias) + col, b);
-    if (f.b_scales) load_n<float, 4>(f.b_scales + col, sb);
-    const int64_t row = row0 + sub;
-    const int left = (int)min((int64_t)32, m - row0);
-    T* out = static_cast<T*>(f.out) + row * n + col;
-    T* slopes = SLOPE ? static_cast<T*>(f.slope) + row * n + col : nullptr;
-    const T* residual = f.residual ? static_cast<const T*>(f.residual) + row * f.residual_stride + col : nullptr;
+    float b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (f.bias) {
+        const T* t = reinterpret_cast<const T*>(&ahead.bias);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) b[k] = to_float(t[k]);
+    }
+    const int left = (int)min((int64_t)32, m - row0) - sub;      // of this lane's rows, four apart
+    T* out = static_cast<T*>(f.out) + (row0 + sub) * n + col;
+    T* slopes = SLOPE ? static_cast<T*>(f.slope) + (row0 + sub) * n + col : nullptr;
+    const T* residual = f.residual ? static_cast<const T*>(f.residual) + (row0 + sub + 16) * f.residual_stride + col : nullptr;
+    const float* scale = f.b_scales ? f.a_scales + row0 + sub : nullptr;
+    // rows sub and sub + 4 of every eight: two places in the block, a round 8 rows on
+    const float4* at0 = reinterpret_cast<const float4*>(block + sub * 32 + ((q ^ sub) << 2));
+    const float4* at1 = reinterpret_cast<const float4*>(block + (sub + 4) * 32 + ((q ^ (sub + 4)) << 2));
+    float4 next[2] = {at0[0], at1[0]};
 #pragma unroll 1
-    for (int first = sub; first < left; first += 16) {
-        float r[4][4];
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) r[p][k] = 0.0f;
-            if (residual && first + 4 * p < left) load_n<T, 4>(residual + 4 * p * f.residual_stride, r[p]);
+    for (int in = 0; in < 32; in += 8) {      // rows beyond the last are worked on and not stored
+        float z[2][4] = {{next[0].x, next[0].y, next[0].z, next[0].w}, {next[1].x, next[1].y, next[1].z, next[1].w}}, d[2][4];
+        if (in < 24) {
+            next[0] = at0[(in + 8) * 8];
+            next[1] = at1[(in + 8) * 8];
         }
+        if (scale) {
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
-            const int in = first + 4 * p;
-            if (in >= left) break;
-            const float4 z4 = *reinterpret_cast<const float4*>(block + in * 32 + ((q ^ (in & 7)) << 2));
-            float z[4] = {z4.x, z4.y, z4.z, z4.w}, d[4];
-            if (f.b_scales) {
-                const float sa = __ldg(f.a_scales + row0 + in);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) z[k] *= sa * sb[k];
+            for (int p = 0; p < 2; ++p) {
+                const float sa = in + 4 * p < left ? __ldg(scale + in + 4 * p) : 0.0f;
+                z[p][0] *= sa * ahead.scales.x;
+                z[p][1] *= sa * ahead.scales.y;
+                z[p][2] *= sa * ahead.scales.z;
+                z[p][3] *= sa * ahead.scales.w;
             }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) z[k] = activate<ACT, SLOPE, kRounded>(f.omega, z[k] + b[k], d[k]) + r[p][k];
-            if (SLOPE) store_n<T, 4>(slopes + 4 * p * n, d);
-            store_n<T, 4>(out + 4 * p * n, z);
         }
-        out += 16 * n;
-        if (SLOPE) slopes += 16 * n;
-        if (residual) residual += 16 * f.residual_stride;
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) z[p][k] += b[k];
+        activate<ACT, SLOPE, kRounded>(f.omega, z[0], d[0]);
+        activate<ACT, SLOPE, kRounded>(f.omega, z[1], d[1]);
+        if (f.residual) {
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                const T* r = reinterpret_cast<const T*>(&ahead.residual[p]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) z[p][k] += to_float(r[k]);
+                ahead.residual[p] = ahead.residual[p + 2];
+                if (in < 16 && in + 16 + 4 * p < left)
+                    ahead.residual[p + 2] = __ldg(reinterpret_cast<const typename Ahead<T>::Four*>(residual + 4 * p * f.residual_stride));
+            }
+            residual += 8 * f.residual_stride;
+        }
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            if (in + 4 * p < left) {
+                if (SLOPE) store_n<T, 4>(slopes + 4 * p * n, d[p]);
+                store_n<T, 4>(out + 4 * p * n, z[p]);
+            }
+        }
+        out += 8 * n;
+        if (SLOPE) slopes += 8 * n;
     }
 }
 
-// A value a lane, a row a pass.
+// A value a lane, a row a pass; eight rows' values are read before any is stored.
 template <class T, int ACT, bool SLOPE>
 __device__ __forceinline__ void finish_narrow(const Finish& f, const float* block, int lane, int64_t row0, int64_t col0, int64_t m,
                                               int64_t n) {
@@ -321,14 +470,24 @@ __device__ __forceinline__ void finish_narrow(const Finish& f, const float* bloc
     T* out = static_cast<T*>(f.out) + row0 * n + col;
     T* slopes = SLOPE ? static_cast<T*>(f.slope) + row0 * n + col : nullptr;
     const T* residual = f.residual ? static_cast<const T*>(f.residual) + row0 * f.residual_stride + col : nullptr;
-#pragma unroll 4
-    for (int in = 0; in < left; ++in) {
-        const float r = residual ? to_float(residual[in * f.residual_stride]) : 0.0f;
-        float z = block[in * 32 + (((lane >> 2) ^ (in & 7)) << 2) + (lane & 3)], d;
-        if (f.b_scales) z *= f.a_scales[row0 + in] * sb;
-        z = activate<ACT, SLOPE, kRounded>(f.omega, z + b, d) + r;
-        if (SLOPE) slopes[in * n] = from_float<T>(d);
-        out[in * n] = from_float<T>(z);
+#pragma unroll 1
+    for (int first = 0; first < left; first += 8) {
+        float z[8], d[8], r[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int in = first + i, row = min(in, left - 1);
+            z[i] = block[in * 32 + (((lane >> 2) ^ (in & 7)) << 2) + (lane & 3)];
+            if (f.b_scales) z[i] *= f.a_scales[row0 + row] * sb;
+            z[i] += b;
+            r[i] = residual ? to_float(residual[row * f.residual_stride]) : 0.0f;
+        }
+        activate<ACT, SLOPE, kRounded>(f.omega, z, d);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (first + i >= left) break;
+            if (SLOPE) slopes[(first + i) * n] = from_float<T>(d[i]);
+            out[(first + i) * n] = from_float<T>(z[i] + r[i]);
+        }
     }
 }
 
@@ -336,197 +495,288 @@ __device__ __forceinline__ void finish_partial(float* partial, const float* bloc
                                                int64_t n) {
     const int64_t col = col0 + lane;
     if (col >= n) return;
-#pragma unroll 8
-    for (int in = 0; in < 32; ++in)
-        if (row0 + in < m) partial[(row0 + in) * n + col] = block[in * 32 + (((lane >> 2) ^ (in & 7)) << 2) + (lane & 3)];
+    partial += row0 * n + col;
+    const int left = (int)min((int64_t)32, m - row0);
+#pragma unroll
+    for (int first = 0; first < 32; first += 8) {
+        float z[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int in = first + i;
+            z[i] = block[in * 32 + (((lane >> 2) ^ (in & 7)) << 2) + (lane & 3)];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (first + i < left) partial[(first + i) * n] = z[i];
+    }
 }
 
 template <class T, int ACT, bool SLOPE>
-__device__ __forceinline__ void finish_as(const GemmArgs& g, const float* block, int lane, int64_t row0, int64_t col0) {
-    if (g.f.wide) finish_wide<T, ACT, SLOPE>(g.f, block, lane, row0, col0, g.m, g.n);
+__device__ __forceinline__ void finish_as(const GemmArgs& g, const float* block, Ahead<T>& r, int lane, int64_t row0,
+                                          int64_t col0) {
+    if (g.f.wide) finish_wide<T, ACT, SLOPE>(g.f, block, r, lane, row0, col0, g.m, g.n);
     else finish_narrow<T, ACT, SLOPE>(g.f, block, lane, row0, col0, g.m, g.n);
 }
 
 // FORWARD: the layer's own product; the gradients' have no activation.
 template <int KIND, bool FORWARD, class T>
-__device__ __forceinline__ void finish_typed(const GemmArgs& g, const float* block, int lane, int64_t row0, int64_t col0) {
+__device__ __forceinline__ void finish_typed(const GemmArgs& g, const float* block, Ahead<T>& r, int lane,
+                                             int64_t row0, int64_t col0) {
     if constexpr (!FORWARD) {
-        finish_as<T, kNone, false>(g, block, lane, row0, col0);
+        finish_as<T, kNone, false>(g, block, r, lane, row0, col0);
     } else {
         by_activation(g.f.activation, [&](auto act) {
             constexpr int ACT = decltype(act)::value;
             if constexpr (KIND != kEight && ACT != kNone) {
                 if (g.f.slope) {
-                    finish_as<T, ACT, true>(g, block, lane, row0, col0);
+                    finish_as<T, ACT, true>(g, block, r, lane, row0, col0);
                     return;
                 }
             }
-            finish_as<T, ACT, false>(g, block, lane, row0, col0);
+            finish_as<T, ACT, false>(g, block, r, lane, row0, col0);
         });
     }
 }
 
+// What is fetched ahead is in words: of 16-bit values held as bf16 whichever of the two they are.
+template <int KIND>
+struct AheadOf { using type = Ahead<__nv_bfloat16>; };
+template <>
+struct AheadOf<kSplit> { using type = Ahead<float>; };
+
+template <class T>
+__device__ __forceinline__ Ahead<T> as_type(const Ahead<__nv_bfloat16>& a) {
+    Ahead<T> t;
+    t.bias = a.bias;
+    t.scales = a.scales;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t.residual[i] = a.residual[i];
+    return t;
+}
+
 template <int KIND, bool FORWARD>
-__device__ __forceinline__ void finish(const GemmArgs& g, const float* block, int lane, int64_t row0, int64_t col0, int64_t split) {
+__device__ __forceinline__ void finish(const GemmArgs& g, const float* block, typename AheadOf<KIND>::type& r, int lane,
+                                       int64_t row0, int64_t col0, int split) {
     if (!FORWARD && g.f.partial) {
         finish_partial(g.f.partial + split * g.m * g.n, block, lane, row0, col0, g.m, g.n);
         return;
     }
-    if constexpr (KIND != kHalf) {
-        if (KIND == kSplit || g.f.type == ASHB_F32) {
-            finish_typed<KIND, FORWARD, float>(g, block, lane, row0, col0);
-            return;
+    if constexpr (KIND == kSplit) {
+        finish_typed<KIND, FORWARD, float>(g, block, r, lane, row0, col0);
+    } else {
+        if constexpr (KIND == kEight) {
+            if (g.f.type == ASHB_F32) {
+                Ahead<float> wide;
+                wide.fetch(g.f, lane, row0, col0, g.m, g.n);
+                finish_typed<KIND, FORWARD, float>(g, block, wide, lane, row0, col0);
+                return;
+            }
         }
-    }
-    if constexpr (KIND != kSplit) {
-        if (g.f.type == ASHB_F16) finish_typed<KIND, FORWARD, __half>(g, block, lane, row0, col0);
-        else finish_typed<KIND, FORWARD, __nv_bfloat16>(g, block, lane, row0, col0);
+        if (g.f.type == ASHB_F16) {
+            Ahead<__half> h = as_type<__half>(r);
+            finish_typed<KIND, FORWARD, __half>(g, block, h, lane, row0, col0);
+        } else finish_typed<KIND, FORWARD, __nv_bfloat16>(g, block, r, lane, row0, col0);
     }
 }
 
 struct GemmShared {
-    uint64_t full[kMaxStages], empty[kMaxStages], sums_full[2], sums_empty[2], drained;
+    uint64_t full[kMaxStages], empty[kMaxStages], sums_full[kMaxSlots], sums_empty[kMaxSlots], drained;
     uint32_t tmem;
     int gave_up;
 };
 
 // Barriers: full[s] by the loaders (the copies' bytes, or a count of their threads), empty[s] by the products that read
-// stage s, sums_full / sums_empty of the two halves of tensor memory.  Every role walks the same items, blocks and phases.
-template <int KIND, bool BULK, bool A_DOWN, bool B_DOWN>
+// stage s, sums_full / sums_empty of the tiles in tensor memory.  Every role walks the same items, blocks and phases.
+// STAYS (loaders with loads of their own): B is loaded once; the registers that held it hold a second tile of A under way.
+template <int KIND, bool BULK, bool A_DOWN, bool B_DOWN, bool STAYS>
 __global__ void __launch_bounds__(kGemmThreads, 1) layer_gemm_kernel(const GemmArgs g, const __grid_constant__ CUtensorMap map_a,
                                                                      const __grid_constant__ CUtensorMap map_b) {
     extern __shared__ __align__(1024) uint8_t dynamic[];
     __shared__ GemmShared sh;
-    constexpr int kBlock = kBlockK<KIND>, kPartsOf = kParts<KIND>;
+    constexpr int kBlock = kBlockK<KIND>, kPartsOf = kParts<KIND>, kStep = KIND == kEight ? 32 : 16;
+    constexpr bool kForward = !A_DOWN && !B_DOWN;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t base = (smem_of(dynamic) + 1023u) & ~1023u;
     const uint32_t a_part = part_bytes<A_DOWN>(kTileM), b_part = part_bytes<B_DOWN>(g.bn);
     const uint32_t a_bytes = a_part * kPartsOf, stage_bytes = a_bytes + b_part * kPartsOf;
     float* blocks = reinterpret_cast<float*>(dynamic + (base - smem_of(dynamic)) + (size_t)stage_bytes * g.stages);
     volatile int* gave_up = &sh.gave_up;
+    const uint32_t full = smem_of(sh.full), empty = smem_of(sh.empty);
+    const uint32_t sums_full = smem_of(sh.sums_full), sums_empty = smem_of(sh.sums_empty);
 
     if (threadIdx.x == 0) {
         sh.gave_up = 0;
         for (int s = 0; s < g.stages; ++s) {
-            bar_init(smem_of(&sh.full[s]), BULK ? 1 : kLoaders * 32);
-            bar_init(smem_of(&sh.empty[s]), 1);
+            bar_init(full + 8 * s, BULK ? 1 : kLoaders * 32);
+            bar_init(empty + 8 * s, 1);
         }
-        for (int h = 0; h < 2; ++h) {
-            bar_init(smem_of(&sh.sums_full[h]), 1);
-            bar_init(smem_of(&sh.sums_empty[h]), kFinishers);
+        for (int h = 0; h < g.slots; ++h) {
+            bar_init(sums_full + 8 * h, 1);
+            bar_init(sums_empty + 8 * h, KIND == kSplit ? 8 : 4 * ((g.bn + 31) >> 5));
         }
         bar_init(smem_of(&sh.drained), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == kLoaders) tmem_alloc(smem_of(&sh.tmem), (uint32_t)g.columns);
+    if (warp == kProductWarp<BULK>) tmem_alloc(smem_of(&sh.tmem), (uint32_t)g.columns);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
-    const uint32_t half_columns = (uint32_t)g.bn * (KIND == kSplit ? 2u : 1u);
+    const uint32_t slot_columns = (uint32_t)g.bn * (KIND == kSplit ? 2u : 1u);
 
-    if (warp < kLoaders) {
-        if (!BULK || threadIdx.x == 0) {
-            int64_t fill = 0;      // stages filled so far
-            bool ok = true;
-            for (int64_t item = blockIdx.x; item < g.items && ok; item += gridDim.x) {
-                int64_t tm, tn, split;
-                tile_of(g, item, tm, tn, split);
-                const int64_t k0 = split * g.k_split, k1 = min(g.k, k0 + g.k_split);
-                for (int64_t k = k0; k < k1 && ok; k += kBlock, ++fill) {
-                    const int s = (int)(fill % g.stages);
-                    const uint32_t parity = (uint32_t)(fill / g.stages) & 1u;
-                    const bool with_b = !g.b_stays || fill < g.stages;
-                    const uint32_t tile_a = base + (uint32_t)s * stage_bytes, tile_b = tile_a + a_bytes;
-                    const uint32_t full = smem_of(&sh.full[s]), empty = smem_of(&sh.empty[s]);
-                    if constexpr (BULK) {
-                        if (!(ok = bar_wait(empty, parity ^ 1u, gave_up))) break;
-                        bar_expect(full, a_part + (with_b ? b_part : 0u));
+    if (warp < (BULK ? 1 : kLoaders)) {
+        if constexpr (BULK) {
+            if (threadIdx.x == 0) {
+                Turn turn;
+                int fills = 0;      // up to the number of stages
+                bool ok = true;
+                for (uint32_t item = blockIdx.x; item < g.items && ok; item += gridDim.x) {
+                    const Tile t = tile_of(g, item);
+                    int k = (int)t.k0;
+                    for (int b = 0; b < t.blocks; ++b, k += kBlock, turn.next(g.stages)) {
+                        if (!(ok = bar_wait(empty + 8 * turn.at, turn.parity ^ 1u, gave_up))) break;
+                        const bool with_b = !g.b_stays || fills < g.stages;
+                        if (fills < g.stages) ++fills;
+                        const uint32_t tile_a = base + (uint32_t)turn.at * stage_bytes, tile_b = tile_a + a_bytes;
+                        const uint32_t bar = full + 8 * turn.at;
+                        bar_expect(bar, a_part + (with_b ? b_part : 0u));
                         if constexpr (A_DOWN) {
                             for (int box = 0; box < kTileM / 64; ++box)
-                                tma_load_2d(tile_a + box * 64 * kRowBytes, &map_a, (int)(tm * kTileM + box * 64), (int)k, full);
+                                tma_load_2d(tile_a + box * 64 * kRowBytes, &map_a, t.m * kTileM + box * 64, k, bar);
                         } else {
-                            tma_load_2d(tile_a, &map_a, (int)k, (int)(tm * kTileM), full);
+                            tma_load_2d(tile_a, &map_a, k, t.m * kTileM, bar);
                         }
                         if (with_b) {
                             if constexpr (B_DOWN) {
                                 for (int box = 0; box * 64 < g.bn; ++box)
-                                    tma_load_2d(tile_b + box * 64 * kRowBytes, &map_b, (int)(tn * g.bn + box * 64), (int)k, full);
+                                    tma_load_2d(tile_b + box * 64 * kRowBytes, &map_b, t.n * g.bn + box * 64, k, bar);
                             } else {
-                                tma_load_2d(tile_b, &map_b, (int)k, (int)(tn * g.bn), full);
+                                tma_load_2d(tile_b, &map_b, k, t.n * g.bn, bar);
                             }
                         }
-                    } else {
-                        constexpr int kValues = KIND == kEight ? 16 : 8, kStep = KIND == kEight ? 32 : 16;
-                        const int left = (int)min((int64_t)kBlock, k1 - k);
-                        const int words = (left + kStep - 1) / kStep * (kStep / kValues);
-                        // 224 threads, 1024 words of A and as many of B (twice as many of 16 and 8 bits)
-                        constexpr int kB = KIND == kSplit ? 5 : 10;
-                        TileFetch<KIND, A_DOWN, 5> fa;
-                        TileFetch<KIND, B_DOWN, kB> fb;
-                        const int b_chunks = (int)(b_part / 16);
-                        fa.fetch(g.a, threadIdx.x, 1024, tm * kTileM, g.m, k, k1, words);
-                        if (with_b) fb.fetch(g.b, threadIdx.x, b_chunks, tn * g.bn, g.n, k, k1, words);
-                        if (!(ok = bar_wait(empty, parity ^ 1u, gave_up))) break;
-                        fa.put(tile_a, a_part, threadIdx.x, 1024, words);
-                        if (with_b) fb.put(tile_b, b_part, threadIdx.x, b_chunks, words);
-                        fence_async_shared();
-                        bar_arrive(full);
+                    }
+                }
+                if (!ok) {      // the copies still under way end before the CTA does
+                    for (int i = 0; i < fills; ++i) {
+                        if (turn.at == 0) turn.parity ^= 1u;
+                        turn.at = (turn.at == 0 ? g.stages : turn.at) - 1;
+                        bar_drain(full + 8 * turn.at, turn.parity);
                     }
                 }
             }
-            if (BULK && !ok)      // the copies still under way end before the CTA does
-                for (int64_t f = max((int64_t)0, fill - g.stages); f < fill; ++f)
-                    bar_drain(smem_of(&sh.full[f % g.stages]), (uint32_t)(f / g.stages) & 1u);
-        }
-    } else if (warp == kLoaders) {
-        if (lane == 0) {
-            int64_t fill = 0, phase = 0;
+        } else {
+            // words along k that the products of a stage read, of 8
+            constexpr int kStepWords = 2;
+            const auto words_of = [&](int64_t k) {
+                return (int)((min((int64_t)kBlock, g.k - k) + kStep - 1) / kStep) * kStepWords;
+            };
+            constexpr int kB = KIND == kSplit ? 5 : 10;      // 224 threads, 1024 words of A and of B (16 and 8 bits: 2048)
+            const int b_words = (int)(b_part / 16);
+            Turn turn;
             bool ok = true;
-            for (int64_t item = blockIdx.x; item < g.items && ok; item += gridDim.x) {
-                int64_t tm, tn, split;
-                tile_of(g, item, tm, tn, split);
-                const int64_t k0 = split * g.k_split, k1 = min(g.k, k0 + g.k_split);
-                const int64_t phase_k = KIND == kSplit ? (int64_t)kPhaseBlocks * kBlock : g.k_split;
-                for (int64_t p0 = k0; p0 < k1 && ok; p0 += phase_k, ++phase) {
-                    const int h = (int)(phase & 1);
-                    const uint32_t sums = tmem + (uint32_t)h * half_columns;
-                    if (!(ok = bar_wait(smem_of(&sh.sums_empty[h]), ((uint32_t)(phase >> 1) & 1u) ^ 1u, gave_up))) break;
+            if constexpr (STAYS) {
+                TileFetch<KIND, A_DOWN, 5> fa[2];
+                {
+                    TileFetch<KIND, B_DOWN, kB> fb;      // a stage's block of k is the same in every round
+                    for (int s = 0; s < g.stages; ++s) {
+                        const int64_t k = (int64_t)(s % (int)g.blocks_k) * kBlock;
+                        fb.fetch(g.b, threadIdx.x, b_words, 0, g.n, k, g.k, words_of(k));
+                        fb.put(base + (uint32_t)s * stage_bytes + a_bytes, b_part, threadIdx.x, b_words, words_of(k));
+                    }
+                }
+                // tiles and blocks in one sequence: `next` is fetched one ahead
+                uint32_t item = blockIdx.x, next_item = blockIdx.x;
+                int b = 0, next_b = 0;
+                const auto fetch = [&](TileFetch<KIND, A_DOWN, 5>& f) {
+                    if (next_item >= g.items) return;
+                    const int64_t k = (int64_t)next_b * kBlock;
+                    f.fetch(g.a, threadIdx.x, 1024, (int64_t)next_item * kTileM, g.m, k, g.k, words_of(k));
+                    if (++next_b == (int)g.blocks_k) {
+                        next_b = 0;
+                        next_item += gridDim.x;
+                    }
+                };
+                const auto put = [&](TileFetch<KIND, A_DOWN, 5>& f) {
+                    if (!(ok = bar_wait(empty + 8 * turn.at, turn.parity ^ 1u, gave_up))) return;
+                    f.put(base + (uint32_t)turn.at * stage_bytes, a_part, threadIdx.x, 1024, words_of((int64_t)b * kBlock));
+                    fence_async_shared();
+                    bar_arrive(full + 8 * turn.at);
+                    turn.next(g.stages);
+                    if (++b == (int)g.blocks_k) {
+                        b = 0;
+                        item += gridDim.x;
+                    }
+                };
+                fetch(fa[0]);
+                while (item < g.items && ok) {
+                    fetch(fa[1]);
+                    put(fa[0]);
+                    if (item >= g.items || !ok) break;
+                    fetch(fa[0]);
+                    put(fa[1]);
+                }
+            } else {
+                for (uint32_t item = blockIdx.x; item < g.items && ok; item += gridDim.x) {
+                    const Tile t = tile_of(g, item);
+                    int64_t k = t.k0;
+                    for (int b = 0; b < t.blocks; ++b, k += kBlock, turn.next(g.stages)) {
+                        const uint32_t tile_a = base + (uint32_t)turn.at * stage_bytes, tile_b = tile_a + a_bytes;
+                        const int words = words_of(k);
+                        TileFetch<KIND, A_DOWN, 5> fa;
+                        TileFetch<KIND, B_DOWN, kB> fb;
+                        fa.fetch(g.a, threadIdx.x, 1024, (int64_t)t.m * kTileM, g.m, k, g.k, words);
+                        fb.fetch(g.b, threadIdx.x, b_words, (int64_t)t.n * g.bn, g.n, k, g.k, words);
+                        if (!(ok = bar_wait(empty + 8 * turn.at, turn.parity ^ 1u, gave_up))) break;
+                        fa.put(tile_a, a_part, threadIdx.x, 1024, words);
+                        fb.put(tile_b, b_part, threadIdx.x, b_words, words);
+                        fence_async_shared();
+                        bar_arrive(full + 8 * turn.at);
+                    }
+                }
+            }
+        }
+    } else if (warp == kProductWarp<BULK>) {
+        if (lane == 0) {
+            Turn turn, slot;
+            bool ok = true;
+            for (uint32_t item = blockIdx.x; item < g.items && ok; item += gridDim.x) {
+                const Tile t = tile_of(g, item);
+                int left = (int)min((int64_t)t.blocks * kBlock, g.k - t.k0);      // values along k
+                for (int b0 = 0; b0 < t.blocks && ok; slot.next(g.slots)) {
+                    const int b1 = KIND == kSplit ? min(t.blocks, b0 + kPhaseBlocks) : t.blocks;
+                    const uint32_t sums = tmem + (uint32_t)slot.at * slot_columns;
+                    if (!(ok = bar_wait(sums_empty + 8 * slot.at, slot.parity ^ 1u, gave_up))) break;
                     tc_fence_after();
-                    const int64_t p1 = min(k1, p0 + phase_k);
                     bool add = false;
-                    for (int64_t k = p0; k < p1; k += kBlock, ++fill) {
-                        const int s = (int)(fill % g.stages);
-                        if (!(ok = bar_wait(smem_of(&sh.full[s]), (uint32_t)(fill / g.stages) & 1u, gave_up))) break;
+                    for (; b0 < b1; ++b0, left -= kBlock, turn.next(g.stages)) {
+                        if (!(ok = bar_wait(full + 8 * turn.at, turn.parity, gave_up))) break;
                         tc_fence_after();
-                        constexpr int kStep = KIND == kEight ? 32 : 16;
-                        const int steps = (int)((min((int64_t)kBlock, k1 - k) + kStep - 1) / kStep);
-                        const uint32_t tile_a = base + (uint32_t)s * stage_bytes, tile_b = tile_a + a_bytes;
+                        const int steps = (min(kBlock, left) + kStep - 1) / kStep;
+                        const uint32_t tile_a = base + (uint32_t)turn.at * stage_bytes;
                         // a step along k: 32 bytes along rows, 16 rows down them
                         constexpr uint64_t a_step = (A_DOWN ? 16 * kRowBytes : 32) >> 4, b_step = (B_DOWN ? 16 * kRowBytes : 32) >> 4;
-                        const uint64_t a = tile_desc(tile_a, 64 * kRowBytes), b = tile_desc(tile_b, 64 * kRowBytes);
+                        uint64_t a = tile_desc(tile_a, 64 * kRowBytes), b = tile_desc(tile_a + a_bytes, 64 * kRowBytes);
                         if constexpr (KIND == kSplit) {
                             const uint64_t ap = a_part >> 4, bp = b_part >> 4;
-                            for (int i = 0; i < steps; ++i) {
-                                const uint64_t ai = a + i * a_step, bi = b + i * b_step;
-                                product<false>(sums, ai, bi, g.desc, add);
-                                const uint32_t small = sums + (uint32_t)g.bn;
-                                product<false>(small, ai + 2 * ap, bi, g.desc, add);
-                                product<false>(small, ai, bi + 2 * bp, g.desc, true);
-                                product<false>(small, ai + ap, bi + bp, g.desc, true);
-                                product<false>(small, ai + ap, bi, g.desc, true);
-                                product<false>(small, ai, bi + bp, g.desc, true);
+                            const uint32_t small = sums + (uint32_t)g.bn;
+                            for (int i = 0; i < steps; ++i, a += a_step, b += b_step) {
+                                product<false>(sums, a, b, g.desc, add);
+                                product<false>(small, a + 2 * ap, b, g.desc, add);
+                                product<false>(small, a, b + 2 * bp, g.desc, true);
+                                product<false>(small, a + ap, b + bp, g.desc, true);
+                                product<false>(small, a + ap, b, g.desc, true);
+                                product<false>(small, a, b + bp, g.desc, true);
                                 add = true;
                             }
                         } else {
-                            for (int i = 0; i < steps; ++i) {
-                                product<KIND == kEight>(sums, a + i * a_step, b + i * b_step, g.desc, add);
+                            for (int i = 0; i < steps; ++i, a += a_step, b += b_step) {
+                                product<KIND == kEight>(sums, a, b, g.desc, add);
                                 add = true;
                             }
                         }
-                        products_done(smem_of(&sh.empty[s]));
+                        products_done(empty + 8 * turn.at);
                     }
-                    if (ok) products_done(smem_of(&sh.sums_full[h]));
+                    if (ok) products_done(sums_full + 8 * slot.at);
                 }
             }
             if (!ok) {      // tensor memory is not given back under products still running
@@ -535,76 +785,75 @@ __global__ void __launch_bounds__(kGemmThreads, 1) layer_gemm_kernel(const GemmA
                 atomicAdd(&g_layer_timeouts, 1u);
             }
         }
-    } else {
-        const int quarter = warp & 3, which = (warp - kLoaders - 1) >> 2;      // lanes of tensor memory; which of the blocks of 32 columns
-        float* block = blocks + (size_t)(warp - kLoaders - 1) * 32 * 32;
+    } else if (warp >= kFirstFinisher<BULK> && warp < kFirstFinisher<BULK> + 4 * g.groups) {
+        // lanes of tensor memory that the warp may read, and its group: the blocks of 32 columns go to the groups in turn
+        const int quarter = warp & 3, which = (warp - kFirstFinisher<BULK>) >> 2;
+        float* block = blocks + (size_t)(warp - kFirstFinisher<BULK>) * 32 * 32;
         const int n_blocks = (g.bn + 31) >> 5;
-        int64_t phase = 0;
-        bool ok = true;
-        for (int64_t item = blockIdx.x; item < g.items && ok; item += gridDim.x) {
-            int64_t tm, tn, split;
-            tile_of(g, item, tm, tn, split);
-            const int64_t row0 = tm * kTileM + quarter * 32, col0 = tn * g.bn;
+        Turn slot;
+        typename AheadOf<KIND>::type ahead;
+        int blk = which;
+        for (uint32_t item = blockIdx.x; item < g.items; item += gridDim.x) {
+            const Tile t = tile_of(g, item);
+            const int64_t row0 = (int64_t)t.m * kTileM + quarter * 32, col0 = (int64_t)t.n * g.bn;
+            bool ok = true;
             if constexpr (KIND == kSplit) {
                 float sums[2][32];
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
 #pragma unroll
                     for (int j = 0; j < 32; ++j) sums[c][j] = 0.0f;
-                const int64_t k0 = split * g.k_split, k1 = min(g.k, k0 + g.k_split);
-                for (int64_t p0 = k0; p0 < k1 && ok; p0 += (int64_t)kPhaseBlocks * kBlock, ++phase) {
-                    const int h = (int)(phase & 1);
-                    ok = __all_sync(0xffffffffu, bar_wait(smem_of(&sh.sums_full[h]), (uint32_t)(phase >> 1) & 1u, gave_up));
+                for (int b0 = 0; b0 < t.blocks; b0 += kPhaseBlocks, slot.next(g.slots)) {
+                    ok = __all_sync(0xffffffffu, bar_wait(sums_full + 8 * slot.at, slot.parity, gave_up));
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t at = tmem + (uint32_t)h * half_columns + ((uint32_t)(quarter * 32) << 16);
+                    const uint32_t at = tmem + (uint32_t)slot.at * slot_columns + ((uint32_t)(quarter * 32) << 16);
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
-                        const int blk = which + 2 * c;
-                        if (blk >= n_blocks) continue;
+                        const int mine = which + 2 * c;
+                        if (mine >= n_blocks) continue;
                         float r[32];
-                        tmem_load32(at + (uint32_t)(g.bn + blk * 32), r);
+                        tmem_load32(at + (uint32_t)(g.bn + mine * 32), r);
 #pragma unroll
                         for (int j = 0; j < 32; ++j) sums[c][j] += r[j];
-                        tmem_load32(at + (uint32_t)(blk * 32), r);
+                        tmem_load32(at + (uint32_t)(mine * 32), r);
 #pragma unroll
                         for (int j = 0; j < 32; ++j) sums[c][j] += r[j];
                     }
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) bar_arrive(smem_of(&sh.sums_empty[h]));
+                    if (lane == 0) bar_arrive(sums_empty + 8 * slot.at);
                 }
                 if (!ok) break;
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    const int blk = which + 2 * c;
-                    if (blk >= n_blocks) continue;
+                    const int mine = which + 2 * c;
+                    if (mine >= n_blocks) continue;
+                    // not ahead of the sums: the registers are theirs until now
+                    if (kForward) ahead.fetch(g.f, lane, row0, col0 + mine * 32, g.m, g.n);
                     put_block(block, lane, sums[c]);
                     __syncwarp();
-                    finish<KIND, !A_DOWN && !B_DOWN>(g, block, lane, row0, col0 + blk * 32, split);
+                    finish<KIND, kForward>(g, block, ahead, lane, row0, col0 + mine * 32, t.split);
                     __syncwarp();
                 }
             } else {
-                const int h = (int)(phase & 1);
-                ok = __all_sync(0xffffffffu, bar_wait(smem_of(&sh.sums_full[h]), (uint32_t)(phase >> 1) & 1u, gave_up));
-                if (!ok) break;
-                ++phase;
-                tc_fence_after();
-                const uint32_t at = tmem + (uint32_t)h * half_columns + ((uint32_t)(quarter * 32) << 16);
-                for (int blk = which; blk < n_blocks; blk += 2) {
+                for (; blk < n_blocks && ok; blk += g.groups) {
+                    if (kForward) ahead.fetch(g.f, lane, row0, col0 + blk * 32, g.m, g.n);
+                    ok = __all_sync(0xffffffffu, bar_wait(sums_full + 8 * slot.at, slot.parity, gave_up));
+                    if (!ok) break;
+                    tc_fence_after();
                     float r[32];
-                    tmem_load32(at + (uint32_t)(blk * 32), r);
+                    tmem_load32(tmem + (uint32_t)slot.at * slot_columns + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(blk * 32), r);
                     put_block(block, lane, r);
-                    if (blk + 2 >= n_blocks) {      // the sums are out: the next tile but one may have their place
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) bar_arrive(smem_of(&sh.sums_empty[h]));
-                    }
+                    tc_fence_before();
                     __syncwarp();
-                    finish<KIND, !A_DOWN && !B_DOWN>(g, block, lane, row0, col0 + blk * 32, split);
+                    if (lane == 0) bar_arrive(sums_empty + 8 * slot.at);
+                    finish<KIND, kForward>(g, block, ahead, lane, row0, col0 + blk * 32, t.split);
                     __syncwarp();
                 }
-                if (which >= n_blocks && lane == 0) bar_arrive(smem_of(&sh.sums_empty[h]));   // had none of them
+                if (!ok) break;
+                blk -= n_blocks;
+                slot.next(g.slots);
             }
         }
     }
@@ -612,7 +861,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) layer_gemm_kernel(const GemmA
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == kLoaders) tmem_free(tmem, (uint32_t)g.columns);
+    if (warp == kProductWarp<BULK>) tmem_free(tmem, (uint32_t)g.columns);
 }
 
 // ---- few rows ------------------------------------------------------------------------------------------------------
@@ -672,17 +921,18 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const GemmArgs g) {
         }
         if (lane < rows) {
             const Finish& f = g.f;
-            float z = mine, d = 1.0f;
-            if (f.b_scales) z *= f.a_scales[lane] * f.b_scales[n];
-            if (f.bias) z += to_float(static_cast<const OUT*>(f.bias)[n]);
+            float z[1] = {mine}, d[1] = {1.0f};
+            if (f.b_scales) z[0] *= f.a_scales[lane] * f.b_scales[n];
+            if (f.bias) z[0] += to_float(static_cast<const OUT*>(f.bias)[n]);
             const float r = f.residual ? to_float(static_cast<const OUT*>(f.residual)[lane * f.residual_stride + n]) : 0.0f;
             const int64_t at = lane * g.n + n;
             by_activation(f.activation, [&](auto act) {
                 constexpr int ACT = decltype(act)::value;
-                z = f.slope ? activate<ACT, true, ROUNDED>(f.omega, z, d) : activate<ACT, false, ROUNDED>(f.omega, z, d);
+                if (f.slope) activate<ACT, true, ROUNDED>(f.omega, z, d);
+                else activate<ACT, false, ROUNDED>(f.omega, z, d);
             });
-            if (f.slope) static_cast<OUT*>(f.slope)[at] = from_float<OUT>(d);
-            static_cast<OUT*>(f.out)[at] = from_float<OUT>(z + r);
+            if (f.slope) static_cast<OUT*>(f.slope)[at] = from_float<OUT>(d[0]);
+            static_cast<OUT*>(f.out)[at] = from_float<OUT>(z[0] + r);
         }
     }
 }
@@ -771,8 +1021,9 @@ __global__ void __launch_bounds__(256) join_kernel(const Join<T> first, const Jo
 static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 struct Plan {
-    int bn, stages, b_stays, columns;
-    int64_t tiles_m, tiles_n, splits, k_split;
+    int bn, stages, slots, groups, b_stays, columns;
+    size_t stage;
+    int64_t tiles_m, tiles_n, splits, split_blocks;
     size_t shared;
 };
 
@@ -809,26 +1060,33 @@ static Plan plan_product(int kind, bool a_down, bool b_down, int64_t m, int64_t 
             if (least == 0.0 || c < least) {
                 least = c;
                 p.splits = splits;
-                p.k_split = per * block;
+                p.split_blocks = per;
                 best = p;
             }
         }
     }
-    const size_t stage = (size_t)parts * ((a_down ? part_bytes<true>(kTileM) : part_bytes<false>(kTileM)) +
-                                          (b_down ? part_bytes<true>(best.bn) : part_bytes<false>(best.bn)));
-    const size_t room = kSharedLimit - 2048 - kFinishBytes;
-    best.stages = (int)std::min<size_t>(kMaxStages, room / stage);
-    const int64_t blocks = ceil_div(k, block);
-    if (best.tiles_n == 1 && best.splits == 1 && blocks <= best.stages) {
-        best.b_stays = 1;
-        best.stages = (int)(best.stages / blocks * blocks);
-    }
-    // more than half of the SM's shared memory: a second CTA would wait for tensor memory
-    best.shared = std::max<size_t>((size_t)best.stages * stage + kFinishBytes + 1024, 120 * 1024);
-    const int columns = 2 * best.bn * (kind == kSplit ? 2 : 1);
+    best.stage = (size_t)parts * ((a_down ? part_bytes<true>(kTileM) : part_bytes<false>(kTileM)) +
+                                  (b_down ? part_bytes<true>(best.bn) : part_bytes<false>(best.bn)));
+    best.b_stays = !a_down && best.tiles_n == 1 && best.splits == 1;      // if the stages hold all of it
+    const int columns = best.bn * (kind == kSplit ? 2 : 1);
+    // as many tiles' sums as tensor memory holds: with two, a narrow tile waits for the round trip of one through the
+    // products, a barrier, the way out and a barrier back (1.5k cycles)
+    best.slots = std::min(kMaxSlots, 512 / columns);
     best.columns = 32;
-    while (best.columns < columns) best.columns <<= 1;
+    while (best.columns < columns * best.slots) best.columns <<= 1;
     return best;
+}
+
+// Stages and finishers once it is known how operands are loaded.
+static void plan_shared(Plan* p, bool bulk, int64_t blocks) {
+    const size_t room = kSharedLimit - 2048;
+    // twelve finishers where that leaves four stages
+    p->groups = bulk && 4 * p->stage + 3 * kFinishBytes <= room ? 3 : 2;
+    p->stages = (int)std::min<size_t>(kMaxStages, (room - p->groups * kFinishBytes) / p->stage);
+    p->b_stays = p->b_stays && blocks <= p->stages;
+    if (p->b_stays) p->stages = (int)(p->stages / blocks * blocks);
+    // more than half of the SM's shared memory: a second CTA would wait for tensor memory
+    p->shared = std::max<size_t>((size_t)p->stages * p->stage + p->groups * kFinishBytes + 1024, 120 * 1024);
 }
 
 // ---- launches -----------------------------------------------------------------------------------------------------------
@@ -857,9 +1115,9 @@ static bool operand_map(CUtensorMap* map, int kind, int type, const Operand& o, 
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int KIND, bool BULK, bool A_DOWN, bool B_DOWN>
+template <int KIND, bool BULK, bool A_DOWN, bool B_DOWN, bool STAYS>
 static cudaError_t launch_product(const GemmArgs& g, const Plan& p, const CUtensorMap& ma, const CUtensorMap& mb, cudaStream_t st) {
-    const auto kernel = layer_gemm_kernel<KIND, BULK, A_DOWN, B_DOWN>;
+    const auto kernel = layer_gemm_kernel<KIND, BULK, A_DOWN, B_DOWN, STAYS>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kSharedLimit - 1024));
     if (e != cudaSuccess) return e;
     kernel<<<(unsigned)std::min<int64_t>(g.items, sm_count()), kGemmThreads, p.shared, st>>>(g, ma, mb);
@@ -867,32 +1125,47 @@ static cudaError_t launch_product(const GemmArgs& g, const Plan& p, const CUtens
 }
 
 template <int KIND, bool A_DOWN, bool B_DOWN>
-static int run_product(GemmArgs g, int type, const Plan& p, cudaStream_t st) {
+static int run_product(GemmArgs g, int type, Plan p, cudaStream_t st) {
     constexpr int kBytes = KIND == kEight ? 1 : KIND == kSplit ? 4 : 2;
-    const auto wide = [&](const Operand& o) { return ((uintptr_t)o.at & 15) == 0 && o.stride * kBytes % 16 == 0; };
-    g.a.wide = wide(g.a);
-    g.b.wide = wide(g.b);
-    g.bn = p.bn;
-    g.stages = p.stages;
-    g.b_stays = p.b_stays;
-    g.columns = p.columns;
-    g.tiles_m = p.tiles_m;
-    g.tiles_n = p.tiles_n;
-    g.k_split = p.k_split;
-    g.items = p.tiles_m * p.tiles_n * p.splits;
-    g.desc = product_desc(kTileM, p.bn, KIND == kEight ? 0 : KIND == kSplit || type == ASHB_BF16 ? 1 : 0, A_DOWN, B_DOWN);
+    // rows start at multiples of 16 bytes; for loads of their own they end there too
+    const auto starts = [&](const Operand& o) { return ((uintptr_t)o.at & 15) == 0 && o.stride * kBytes % 16 == 0; };
+    g.a.wide = starts(g.a) && (A_DOWN ? g.m : g.k) * kBytes % 16 == 0;
+    g.b.wide = starts(g.b) && (B_DOWN ? g.n : g.k) * kBytes % 16 == 0;
     CUtensorMap ma{}, mb{};
-    cudaError_t e;
-    const bool bulk = KIND != kSplit && g.a.wide && g.b.wide &&
+    const bool bulk = KIND != kSplit && starts(g.a) && starts(g.b) &&
                       operand_map(&ma, KIND, type, g.a, A_DOWN ? g.k : g.m, A_DOWN ? g.m : g.k, A_DOWN ? 64 : kTileM) &&
                       operand_map(&mb, KIND, type, g.b, B_DOWN ? g.k : g.n, B_DOWN ? g.n : g.k, B_DOWN ? 64 : p.bn);
+    plan_shared(&p, bulk, ceil_div(g.k, kBlockK<KIND>));
+    g.bn = p.bn;
+    g.stages = p.stages;
+    g.slots = p.slots;
+    g.groups = p.groups;
+    g.b_stays = p.b_stays;
+    g.columns = p.columns;
+    const int64_t block = KIND == kEight ? 128 : 64;
+    ASHB_REQUIRE(p.tiles_m * p.tiles_n * p.splits < (int64_t)1 << 31, "a product of %lld x %lld values", (long long)g.m, (long long)g.n);
+    g.tiles_m = (uint32_t)p.tiles_m;
+    g.tiles_n = (uint32_t)p.tiles_n;
+    g.tiles = g.tiles_m * g.tiles_n;
+    g.splits = (uint32_t)p.splits;
+    g.items = g.tiles * g.splits;
+    g.blocks_k = (uint32_t)ceil_div(g.k, block);
+    g.split_blocks = (uint32_t)p.split_blocks;
+    g.block_k = (uint32_t)block;
+    g.desc = product_desc(kTileM, p.bn, KIND == kEight ? 0 : KIND == kSplit || type == ASHB_BF16 ? 1 : 0, A_DOWN, B_DOWN);
     if constexpr (KIND != kSplit) {
-        e = bulk ? launch_product<KIND, true, A_DOWN, B_DOWN>(g, p, ma, mb, st)
-                 : launch_product<KIND, false, A_DOWN, B_DOWN>(g, p, ma, mb, st);
-    } else {
-        e = launch_product<KIND, false, A_DOWN, B_DOWN>(g, p, ma, mb, st);
+        if (bulk) {
+            ASHB_CUDA_TRY((launch_product<KIND, true, A_DOWN, B_DOWN, false>(g, p, ma, mb, st)));
+            return ASHB_OK;
+        }
     }
-    ASHB_CUDA_TRY(e);
+    if constexpr (!A_DOWN) {
+        if (p.b_stays) {
+            ASHB_CUDA_TRY((launch_product<KIND, false, A_DOWN, B_DOWN, true>(g, p, ma, mb, st)));
+            return ASHB_OK;
+        }
+    }
+    ASHB_CUDA_TRY((launch_product<KIND, false, A_DOWN, B_DOWN, false>(g, p, ma, mb, st)));
     return ASHB_OK;
 }
 

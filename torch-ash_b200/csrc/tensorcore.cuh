@@ -20,12 +20,13 @@ __device__ __forceinline__ void bar_arrive(uint32_t bar) {
 __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
+// The thread may sleep for up to a microsecond inside: polling without it takes issue slots from the warps that work.
 __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
             "{\n\t"
             ".reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\t"
             "selp.u32 %0, 1, 0, p;\n\t"
             "}"
             : "=r"(ok)
@@ -34,9 +35,9 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
     return ok != 0;
 }
 
-// Polls of a barrier before a wait gives up: over a tenth of a second, where the longest wait of a healthy launch, for the
-// products of one tile, is milliseconds.
-constexpr int kWaitPolls = 1 << 24;
+// Polls of a barrier before a wait gives up: between a tenth of a second and four seconds, where the longest wait of a healthy
+// launch, for the products of one tile, is milliseconds.
+constexpr int kWaitPolls = 1 << 22;
 
 // Waits for phase `parity`.  False once the limit has run out here (`gave_up` is set) or anywhere else in the CTA.
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
