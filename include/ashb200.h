@@ -764,9 +764,10 @@ typedef struct ashb_row_table {
 } ashb_row_table;
 
 /* ashb_map_insert_values with tables that may be kept in 8 bits: the row of every NEW key is quantised as it is
- * written.  `tables` is a HOST array of at most 16. */
+ * written.  `tables` is a HOST array of at most 16; row_of_dev int32 [n] is scratch that becomes the row of each new key,
+ * -1 for the others. */
 int ashb_map_insert_rows(ashb_map* map, const int32_t* keys_dev, int64_t n, int n_tables, const ashb_row_table* tables,
-                         void* stream);
+                         int32_t* row_of_dev, void* stream);
 
 /* ashb_map_find, and the rows of tables kept in 8 bits: row i of a table's dst is what the row of key i reads back as, zeros
  * for a miss.  indices_dev may be NULL. */

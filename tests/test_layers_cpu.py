@@ -142,4 +142,4 @@ def test_library_refuses_cpu_tensors_and_bad_arguments():
     assert lib.ashb_read_rows(4, None, 4, ctypes.byref(t), None) == 1
     t = shim._RowTable(4096, 4096, 4096, 8, 1, 0)
     assert lib.ashb_read_rows(5, None, 4, ctypes.byref(t), None) == 1
-    assert lib.ashb_map_insert_rows(None, p, 3, 0, None, None) == 1 and lib.ashb_map_find_rows(None, p, 3, p, p, 0, None, None) == 1
+    assert lib.ashb_map_insert_rows(None, p, 3, 0, None, p, None) == 1 and lib.ashb_map_find_rows(None, p, 3, p, p, 0, None, None) == 1

@@ -12,6 +12,7 @@ device pointers and turns non-zero status codes into ``RuntimeError``.
 There is no CPU path: tensors must live on a CUDA device and the shared library
 must have been built (``python torch-ash_b200/build.py``).
 """
+import contextlib
 import ctypes
 import os
 import warnings
@@ -130,7 +131,7 @@ _lib.ashb_routed_backward.argtypes = [_vp, _int, _vp, _vp, _int, _int, _c.c_doub
 _lib.ashb_routed_send_g.argtypes = [_vp, _i64, _vp, _i64] + _ROUTED_LAYOUT + [_vp]
 _lib.ashb_routed_backward_backward.argtypes = [_vp, _int, _vp, _vp, _c.c_double, _vp, _int, _vp, _vp, _i64, _i64] + _ROUTED_LAYOUT + [_vp]
 _lib.ashb_routed_unpack_grad_x.argtypes = [_vp, _i64, _vp, _i64] + _ROUTED_LAYOUT + [_vp]
-_lib.ashb_map_insert_rows.argtypes = [_vp, _vp, _i64, _int, _vp, _vp]
+_lib.ashb_map_insert_rows.argtypes = [_vp, _vp, _i64, _int, _vp, _vp, _vp]
 _lib.ashb_map_find_rows.argtypes = [_vp, _vp, _i64, _vp, _vp, _int, _vp, _vp]
 _lib.ashb_quantize_rows.argtypes = [_i64, _vp, _vp]
 _lib.ashb_read_rows.argtypes = [_i64, _vp, _i64, _vp, _vp]
@@ -216,6 +217,15 @@ def _stream(device: torch.device) -> int:
     if _raw_stream is None or device.index is None:
         return torch.cuda.current_stream(device).cuda_stream
     return _raw_stream(device.index)   # without building a Stream object: several per cent of a small call
+
+
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_NOTHING = contextlib.nullcontext()
+
+
+def _on(device: torch.device):
+    """The device made current; nothing to do, and nothing spent on it, where it is."""
+    return _NOTHING if device.index == _current_device() else torch.cuda.device(device)
 
 
 def _cuda(t: torch.Tensor, name: str, dtype=None) -> torch.Tensor:
@@ -400,7 +410,9 @@ class HashMap:
                 entries[j] = _RowTable(v.data_ptr(), codes.data_ptr(), scales.data_ptr(), codes.shape[1],
                                        _ROW_FORMATS[codes.dtype], _VALUE_TYPES[v.dtype])
             keep.append(v)
-        _check(_lib.ashb_map_insert_rows(self._h, keys.data_ptr(), n, len(tables), entries, _stream(self._device)))
+        row_of = torch.empty(n, dtype=torch.int32, device=self._device)
+        _check(_lib.ashb_map_insert_rows(self._h, keys.data_ptr(), n, len(tables), entries, row_of.data_ptr(),
+                                         _stream(self._device)))
 
     def find_rows(self, keys: torch.Tensor, tables: dict, dtype: torch.dtype, with_indices: bool):
         """``(indices or None, masks, {name: rows read back})`` of tables kept in 8 bits, ``(codes, scales)`` each, in one
@@ -1612,7 +1624,7 @@ def quantize_rows(x: torch.Tensor, codes_dtype: torch.dtype):
     if scales.numel():
         table = _RowTable(x.data_ptr(), codes.data_ptr(), scales.data_ptr(), x.shape[-1], _ROW_FORMATS[codes_dtype],
                           _VALUE_TYPES[x.dtype])
-        with torch.cuda.device(x.device):
+        with _on(x.device):
             _check(_lib.ashb_quantize_rows(scales.numel(), _c.byref(table), _stream(x.device)))
     return codes, scales
 
@@ -1628,7 +1640,7 @@ def read_rows(codes: torch.Tensor, scales: torch.Tensor, indices, dtype: torch.d
     if out.numel():
         table = _RowTable(codes.data_ptr(), out.data_ptr(), scales.data_ptr(), codes.shape[-1], _ROW_FORMATS[codes.dtype],
                           _VALUE_TYPES[dtype])
-        with torch.cuda.device(codes.device):
+        with _on(codes.device):
             _check(_lib.ashb_read_rows(n, None if indices is None else indices.data_ptr(), scales.numel(), _c.byref(table),
                                        _stream(codes.device)))
     return out
@@ -1665,7 +1677,7 @@ def rms_norm_forward(x, weight, residual, eps: float, quantize: bool, with_rstd:
     total = empty(rows, width) if residual is not None else None
     rstd = empty(rows, dtype=torch.float32) if with_rstd else None
     if rows:
-        with torch.cuda.device(x.device):
+        with _on(x.device):
             _check(_lib.ashb_rms_norm_forward(_VALUE_TYPES[x.dtype], x.data_ptr(), x_stride, _ptr(residual), residual_stride,
                                               weight.data_ptr(), rows, width, eps, _ptr(y), _ptr(codes), _ptr(scales),
                                               _ptr(total), _ptr(rstd), _stream(x.device)))
@@ -1680,7 +1692,7 @@ def rms_norm_backward(dy, dsum, s, weight, rstd):
     dx, dw = torch.empty_like(s), torch.empty_like(weight)
     nbytes = _lib.ashb_rms_norm_workspace(rows, width)
     workspace = torch.empty(nbytes, dtype=torch.uint8, device=s.device)
-    with torch.cuda.device(s.device):
+    with _on(s.device):
         _check(_lib.ashb_rms_norm_backward(_VALUE_TYPES[s.dtype], dy.data_ptr(), _ptr(dsum), s.data_ptr(), weight.data_ptr(),
                                            rstd.data_ptr(), rows, width, dx.data_ptr(), dw.data_ptr(), _ptr(workspace), nbytes,
                                            _stream(s.device)))
@@ -1702,7 +1714,7 @@ def linear_forward(x, weight, bias, activation: str, residual, omega: float, wit
     y = torch.empty((rows, outputs), dtype=out_dtype, device=x.device)
     slope = torch.empty_like(y) if with_slope else None
     if rows:
-        with torch.cuda.device(x.device):
+        with _on(x.device):
             _check(_lib.ashb_linear_forward(
                 _E4M3_ROWS if scales is not None else _VALUE_TYPES[x.dtype], x.data_ptr(), x_stride, _ptr(x_scales),
                 weight.data_ptr(), weight_stride, _ptr(w_scales), _ptr(bias), _ptr(residual), residual_stride, rows, inputs,
@@ -1723,7 +1735,7 @@ def linear_backward(dy, slope, slope_kind: int, x, weight, want_dx: bool, want_d
     dw = empty(outputs, inputs) if want_dweight else None
     db = empty(outputs) if want_dbias else None
     kind = _VALUE_TYPES[dy.dtype]
-    with torch.cuda.device(dy.device):
+    with _on(dy.device):
         nbytes = _lib.ashb_linear_workspace(kind, rows, inputs, outputs, slope_kind, int(want_dweight), int(want_dbias))
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=dy.device) if nbytes else None
         _check(_lib.ashb_linear_backward(kind, dy.data_ptr(), _ptr(slope), slope_kind, x.data_ptr(), x_stride,

@@ -32,9 +32,9 @@ def _check_like(t: Optional[torch.Tensor], name: str, shape, like: torch.Tensor,
         return
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{name} must be a tensor, got {type(t).__name__}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise ValueError(f"{name} must be {dtype} as the other tensors of the call, got {t.dtype}")
     if t.device != like.device:
         raise ValueError(f"{name} is on {t.device}, x on {like.device}")
@@ -55,7 +55,11 @@ def _check_activation(activation: str, omega: float) -> None:
 
 
 def _recorded(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 # ------------------------------------------------------------------------------------------------ dense layer

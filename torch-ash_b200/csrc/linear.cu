@@ -28,6 +28,7 @@
 #include <algorithm>
 #include <cstring>
 
+#include "columnsums.cuh"
 #include "rowformat.cuh"
 #include "tensorcore.cuh"
 
@@ -978,45 +979,6 @@ __global__ void __launch_bounds__(256) slope_kernel(const T* __restrict__ dy, co
     }
 }
 
-// Sums over the first dimension of `partial` [count][n] in a fixed order: the weight's gradient from the splits and the
-// bias's from the CTAs above, one launch.  MANY: eight warps share the terms of 32 columns; else a thread sums a column.
-template <class T>
-struct Join {
-    const float* partial;
-    int64_t count, n;
-    T* out;
-    unsigned blocks;
-};
-template <class T>
-__global__ void __launch_bounds__(256) join_kernel(const Join<T> first, const Join<T> second) {
-    __shared__ float mine[8][32];
-    const bool is_first = blockIdx.x < first.blocks;
-    const Join<T>& j = is_first ? first : second;
-    const int64_t block = is_first ? blockIdx.x : blockIdx.x - first.blocks;
-    if (j.count <= 8) {
-        const int64_t col = block * 256 + threadIdx.x;
-        if (col >= j.n) return;
-        float v = 0.0f;
-        for (int64_t i = 0; i < j.count; ++i) v += j.partial[i * j.n + col];
-        j.out[col] = from_float<T>(v);
-        return;
-    }
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t col = block * 32 + lane;
-    float v = 0.0f;
-    if (col < j.n) {
-#pragma unroll 8
-        for (int64_t i = warp; i < j.count; i += 8) v += j.partial[i * j.n + col];
-    }
-    mine[warp][lane] = v;
-    __syncthreads();
-    if (warp != 0 || col >= j.n) return;
-    float t = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) t += mine[w][lane];
-    j.out[col] = from_float<T>(t);
-}
-
 // ---- plans --------------------------------------------------------------------------------------------------------------
 static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
@@ -1194,7 +1156,7 @@ static SlopePlan plan_slope(int type, int64_t rows, int64_t n, bool wide) {
     while (p.lanes < 32 && (int64_t)p.lanes * p.vec < n) p.lanes <<= 1;
     p.across = (unsigned)ceil_div(n, (int64_t)p.lanes * p.vec);
     const int64_t groups = 256 / p.lanes;
-    p.down = (unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows, groups * 4), ceil_div((int64_t)sm_count() * 8, p.across)));
+    p.down = (unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows, groups * 4), ceil_div((int64_t)sm_count() * 4, p.across)));
     return p;
 }
 // the largest `down` of both forms, for the workspace
@@ -1209,16 +1171,6 @@ static void launch_slope(const SlopePlan& p, const void* dy, const void* slope, 
     const T *g = static_cast<const T*>(dy), *s = static_cast<const T*>(slope);
     if (p.vec > 1) slope_kernel<T, 16 / sizeof(T)><<<grid, 256, 0, st>>>(g, s, kind, rows, n, p.lanes, static_cast<T*>(dz), partial);
     else slope_kernel<T, 1><<<grid, 256, 0, st>>>(g, s, kind, rows, n, p.lanes, static_cast<T*>(dz), partial);
-}
-
-template <class T>
-static void launch_join(const float* pw, int64_t count_w, int64_t n_w, void* dw, const float* pb, int64_t count_b, int64_t n_b,
-                        void* db, cudaStream_t st) {
-    const auto make = [](const float* p, int64_t count, int64_t n, void* out) {
-        return Join<T>{p, count, n, static_cast<T*>(out), p ? (unsigned)ceil_div(n, count <= 8 ? 256 : 32) : 0u};
-    };
-    const Join<T> w = make(pw, count_w, n_w, dw), b = make(pb, count_b, n_b, db);
-    if (w.blocks + b.blocks) join_kernel<T><<<w.blocks + b.blocks, 256, 0, st>>>(w, b);
 }
 
 static size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
@@ -1385,9 +1337,10 @@ int ashb_linear_backward(int type, const void* dy, const void* slope, int slope_
         }
         if (int rc = run_typed<true, true>(g, type, bp.pw, st)) return rc;
     }
-    if (type == ASHB_F32) launch_join<float>(pw, bp.pw.splits, outputs * inputs, dweight, pb, count_b, outputs, dbias, st);
-    else if (type == ASHB_F16) launch_join<__half>(pw, bp.pw.splits, outputs * inputs, dweight, pb, count_b, outputs, dbias, st);
-    else launch_join<__nv_bfloat16>(pw, bp.pw.splits, outputs * inputs, dweight, pb, count_b, outputs, dbias, st);
+    const Sums sw{pw, bp.pw.splits, outputs * inputs, dweight}, sb{pb, count_b, outputs, dbias};
+    if (type == ASHB_F32) launch_sums<float>(sw, sb, st);
+    else if (type == ASHB_F16) launch_sums<__half>(sw, sb, st);
+    else launch_sums<__nv_bfloat16>(sw, sb, st);
     ASHB_LAUNCH_CHECK();
     return ASHB_OK;
 }

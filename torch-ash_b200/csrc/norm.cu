@@ -14,6 +14,7 @@
 // small kernel: the same bits whenever the same call is made.
 #include <algorithm>
 
+#include "columnsums.cuh"
 #include "rowformat.cuh"
 
 namespace ashb {
@@ -296,26 +297,6 @@ __global__ void __launch_bounds__(256) norm_backward_long_kernel(const NormGradA
     }
 }
 
-// Columns summed over the CTAs' rows: 8 warps share the CTAs of 32 columns, joined in order.
-template <class T>
-__global__ void __launch_bounds__(256) column_sums_kernel(const float* __restrict__ partial, int64_t n, int64_t width,
-                                                          T* __restrict__ out) {
-    __shared__ float mine[8][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t col = (int64_t)blockIdx.x * 32 + lane;
-    float v = 0.0f;
-    if (col < width)
-        for (int64_t i = warp; i < n; i += 8) v += partial[i * width + col];
-    mine[warp][lane] = v;
-    __syncthreads();
-    if (warp == 0 && col < width) {
-        float t = 0.0f;
-#pragma unroll
-        for (int w = 0; w < 8; ++w) t += mine[w][lane];
-        out[col] = from_float<T>(t);
-    }
-}
-
 // ---- launches ----------------------------------------------------------------------------------------------------
 constexpr int64_t kLongRow = 8192;
 
@@ -422,7 +403,7 @@ static void backward_typed(const NormGradArgs& a, unsigned grid, void* dw, cudaS
         if (wide) go(std::integral_constant<int, kVec>{});
         else go(std::integral_constant<int, 1>{});
     }
-    column_sums_kernel<T><<<(unsigned)((a.width + 31) / 32), 256, 0, st>>>(a.partial, grid, a.width, static_cast<T*>(dw));
+    launch_sums<T>(Sums{a.partial, grid, a.width, dw}, Sums{}, st);
 }
 
 }  // namespace ashb

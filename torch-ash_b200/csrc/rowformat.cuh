@@ -104,6 +104,16 @@ __device__ __forceinline__ void store_n(T* __restrict__ p, const float (&v)[N]) 
     *reinterpret_cast<typename Word<N * sizeof(T)>::type*>(p) = w;
 }
 
+// The same store, first to leave L2: for what no kernel of the call reads again.
+template <class T, int N>
+__device__ __forceinline__ void store_n_passing(T* __restrict__ p, const float (&v)[N]) {
+    typename Word<N * sizeof(T)>::type w;
+    T* t = reinterpret_cast<T*>(&w);
+#pragma unroll
+    for (int k = 0; k < N; ++k) t[k] = from_float<T>(v[k]);
+    __stcs(reinterpret_cast<typename Word<N * sizeof(T)>::type*>(p), w);
+}
+
 inline int value_bytes(int dtype) { return dtype == ASHB_F32 ? 4 : 2; }
 inline bool is_value_type(int dtype) { return dtype == ASHB_F32 || dtype == ASHB_F16 || dtype == ASHB_BF16; }
 
