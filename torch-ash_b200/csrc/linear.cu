@@ -185,7 +185,9 @@ struct GemmArgs {
     uint32_t tiles_m, tiles_n, tiles, items;             // tiles = tiles_m * tiles_n, items = tiles * splits
     uint32_t splits, blocks_k, split_blocks, block_k;    // stages along k: all, of a split; values of a stage
     uint32_t desc;
-    int bn, stages, slots, groups, b_stays, columns;      // groups: of four finishers; columns: tensor memory to allocate
+    // groups: of four finishers; places: blocks of a finisher in shared memory; columns: tensor memory to allocate
+    int bn, stages, slots, groups, places, b_stays, columns;
+    int raws;      // split_gemm_kernel: stages of values as they came
 };
 
 // Consecutive values of an operand that make one 16-byte word of each of its parts, at p; `left` of them exist, none if it is
@@ -361,6 +363,17 @@ __device__ __forceinline__ void put_block(float* block, int lane, const float (&
     for (int q = 0; q < 8; ++q)
         *reinterpret_cast<float4*>(block + lane * 32 + ((q ^ (lane & 7)) << 2)) =
                 make_float4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
+}
+
+__device__ __forceinline__ void add_block(const float* block, int lane, float (&r)[32]) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+        const float4 s = *reinterpret_cast<const float4*>(block + lane * 32 + ((q ^ (lane & 7)) << 2));
+        r[4 * q] += s.x;
+        r[4 * q + 1] += s.y;
+        r[4 * q + 2] += s.z;
+        r[4 * q + 3] += s.w;
+    }
 }
 
 // What a lane of finish_wide wants besides the sums, fetched before they are waited for: its columns' bias and scales, and the
@@ -580,6 +593,49 @@ __device__ __forceinline__ void finish(const GemmArgs& g, const float* block, ty
     }
 }
 
+// Split products: a warp's share of a tile, the blocks `which` and `which` + 2 of 32 columns.  The two sums of a phase are added
+// in registers, those of later phases to what the block holds in shared memory (`block`: 32 x 32 values, of each block where
+// there are several phases).  False: a wait gave up.
+template <bool FORWARD>
+__device__ __forceinline__ bool finish_split(const GemmArgs& g, const Tile& t, int phase_blocks, Turn& slot, uint32_t tmem,
+                                             uint32_t sums_full, uint32_t sums_empty, volatile int* gave_up, float* block,
+                                             int quarter, int which, int lane) {
+    const int n_blocks = (g.bn + 31) >> 5;
+    const int64_t row0 = (int64_t)t.m * kTileM + quarter * 32, col0 = (int64_t)t.n * g.bn;
+    const bool several = t.blocks > phase_blocks;
+    Ahead<float> ahead;
+#pragma unroll 1
+    for (int b0 = 0; b0 < t.blocks; b0 += phase_blocks, slot.next(g.slots)) {
+        const bool last = b0 + phase_blocks >= t.blocks;
+        if (!__all_sync(0xffffffffu, bar_wait(sums_full + 8 * slot.at, slot.parity, gave_up))) return false;
+        tc_fence_after();
+        const uint32_t at = tmem + (uint32_t)(slot.at * 2 * g.bn) + ((uint32_t)(quarter * 32) << 16);
+#pragma unroll 1
+        for (int mine = which; mine < n_blocks; mine += 2) {
+            float* place = block + (several ? (mine >> 1) * 1024 : 0);
+            if (FORWARD && last) ahead.fetch(g.f, lane, row0, col0 + mine * 32, g.m, g.n);
+            float r[32], small[32];
+            tmem_load32(at + (uint32_t)(mine * 32), r);
+            tmem_load32(at + (uint32_t)(g.bn + mine * 32), small);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) r[j] += small[j];
+            if (b0 > 0) add_block(place, lane, r);
+            put_block(place, lane, r);
+            __syncwarp();
+            if (mine + 2 >= n_blocks) {
+                tc_fence_before();
+                if (lane == 0) bar_arrive(sums_empty + 8 * slot.at);
+            }
+            if (last) {
+                finish<kSplit, FORWARD>(g, place, ahead, lane, row0, col0 + mine * 32, t.split);
+                __syncwarp();
+            }
+        }
+        if (which >= n_blocks && lane == 0) bar_arrive(sums_empty + 8 * slot.at);
+    }
+    return true;
+}
+
 struct GemmShared {
     uint64_t full[kMaxStages], empty[kMaxStages], sums_full[kMaxSlots], sums_empty[kMaxSlots], drained;
     uint32_t tmem;
@@ -789,7 +845,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) layer_gemm_kernel(const GemmA
     } else if (warp >= kFirstFinisher<BULK> && warp < kFirstFinisher<BULK> + 4 * g.groups) {
         // lanes of tensor memory that the warp may read, and its group: the blocks of 32 columns go to the groups in turn
         const int quarter = warp & 3, which = (warp - kFirstFinisher<BULK>) >> 2;
-        float* block = blocks + (size_t)(warp - kFirstFinisher<BULK>) * 32 * 32;
+        float* block = blocks + (size_t)(warp - kFirstFinisher<BULK>) * 32 * 32 * g.places;
         const int n_blocks = (g.bn + 31) >> 5;
         Turn slot;
         typename AheadOf<KIND>::type ahead;
@@ -799,44 +855,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) layer_gemm_kernel(const GemmA
             const int64_t row0 = (int64_t)t.m * kTileM + quarter * 32, col0 = (int64_t)t.n * g.bn;
             bool ok = true;
             if constexpr (KIND == kSplit) {
-                float sums[2][32];
-#pragma unroll
-                for (int c = 0; c < 2; ++c)
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) sums[c][j] = 0.0f;
-                for (int b0 = 0; b0 < t.blocks; b0 += kPhaseBlocks, slot.next(g.slots)) {
-                    ok = __all_sync(0xffffffffu, bar_wait(sums_full + 8 * slot.at, slot.parity, gave_up));
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t at = tmem + (uint32_t)slot.at * slot_columns + ((uint32_t)(quarter * 32) << 16);
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const int mine = which + 2 * c;
-                        if (mine >= n_blocks) continue;
-                        float r[32];
-                        tmem_load32(at + (uint32_t)(g.bn + mine * 32), r);
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) sums[c][j] += r[j];
-                        tmem_load32(at + (uint32_t)(mine * 32), r);
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) sums[c][j] += r[j];
-                    }
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) bar_arrive(sums_empty + 8 * slot.at);
-                }
-                if (!ok) break;
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const int mine = which + 2 * c;
-                    if (mine >= n_blocks) continue;
-                    // not ahead of the sums: the registers are theirs until now
-                    if (kForward) ahead.fetch(g.f, lane, row0, col0 + mine * 32, g.m, g.n);
-                    put_block(block, lane, sums[c]);
-                    __syncwarp();
-                    finish<KIND, kForward>(g, block, ahead, lane, row0, col0 + mine * 32, t.split);
-                    __syncwarp();
-                }
+                if (!finish_split<kForward>(g, t, kPhaseBlocks, slot, tmem, sums_full, sums_empty, gave_up, block, quarter, which,
+                                            lane))
+                    break;
             } else {
                 for (; blk < n_blocks && ok; blk += g.groups) {
                     if (kForward) ahead.fetch(g.f, lane, row0, col0 + blk * 32, g.m, g.n);
@@ -863,6 +884,234 @@ __global__ void __launch_bounds__(kGemmThreads, 1) layer_gemm_kernel(const GemmA
     __syncthreads();
     tc_fence_after();
     if (warp == kProductWarp<BULK>) tmem_free(tmem, (uint32_t)g.columns);
+}
+
+// ---- split products from bulk copies ---------------------------------------------------------------------------------------
+// The product kernel of float32 operands whose rows are multiples of 16 bytes.  The copies bring values as they are into a ring
+// of their own, 32 along k a stage, so that several tiles are under way without a register; six warps split them into the
+// parts' tiles by a short loop.  Splitting on the way from registers instead took 40 registers for a tile under way and a loop
+// so long that it and the finishers' did not fit the instruction cache together (1M rows 64 -> 64: 145 us, %(none)s this way).
+constexpr int kSplitBlock = 32, kSplitPhase = 512 / kSplitBlock, kSplitters = 6;
+constexpr int kMaxRaws = 6;
+
+struct SplitShared {
+    uint64_t raw_full[kMaxRaws], raw_empty[kMaxRaws], full[kMaxStages], empty[kMaxStages], sums_full[kMaxSlots],
+            sums_empty[kMaxSlots], drained;
+    uint32_t tmem;
+    int gave_up;
+};
+
+// Bytes of one part of a tile of `extent` values across and 32 along k.
+template <bool DOWN>
+__host__ __device__ constexpr uint32_t split_bytes(int extent) {
+    return DOWN ? (uint32_t)((extent + 63) / 64) * 4096u : (uint32_t)extent * 64u;
+}
+
+__device__ __forceinline__ float4 get16(uint32_t at) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at));
+    return v;
+}
+
+// Eight values a step.  Along rows: the raw tile has `extent` rows of 32 values, a part as many of 64 bytes.  Down rows: boxes of
+// 32 rows of 32 values, a part boxes of 32 rows of 64.  Both sides swizzled: two lanes of eight share a bank at most.
+template <bool DOWN>
+__device__ __forceinline__ void split_tile(uint32_t raw, uint32_t parts, int extent, int thread) {
+    const uint32_t part = split_bytes<DOWN>(extent);
+#pragma unroll 2
+    for (int i = thread; i < extent * 4; i += kSplitters * 32) {
+        const int r = i >> 2, c = i & 3;
+        const uint32_t row = raw + (uint32_t)r * 128u;      // rows of boxes follow one another too
+        const float4 a = get16(row + (uint32_t)(((2 * c) ^ (r & 7)) << 4)), b = get16(row + (uint32_t)(((2 * c + 1) ^ (r & 7)) << 4));
+        Eight32 e;
+        e.v[0] = a.x; e.v[1] = a.y; e.v[2] = a.z; e.v[3] = a.w;
+        e.v[4] = b.x; e.v[5] = b.y; e.v[6] = b.z; e.v[7] = b.w;
+        uint32_t to;
+        if (DOWN) {
+            const int box = r >> 5, k = r & 31, word = (box & 1) * 4 + c;
+            to = parts + (uint32_t)(box >> 1) * 4096u + (uint32_t)k * 128u + (uint32_t)((word ^ (k & 7)) << 4);
+        } else {
+            to = parts + (uint32_t)r * 64u + (uint32_t)((c ^ ((r >> 1) & 3)) << 4);
+        }
+        put8(to, part, e);
+    }
+}
+
+template <bool A_DOWN, bool B_DOWN>
+__global__ void __launch_bounds__(kGemmThreads, 1) split_gemm_kernel(const GemmArgs g, const __grid_constant__ CUtensorMap map_a,
+                                                                     const __grid_constant__ CUtensorMap map_b) {
+    extern __shared__ __align__(1024) uint8_t dynamic[];
+    __shared__ SplitShared sh;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t base = (smem_of(dynamic) + 1023u) & ~1023u;
+    const uint32_t a_part = split_bytes<A_DOWN>(kTileM), b_part = split_bytes<B_DOWN>(g.bn);
+    const uint32_t raw_a = kTileM * 128u, raw_b = (uint32_t)g.bn * 128u;
+    // raw stages, parts' stages, all of B's parts where it stays, the finishers' blocks
+    const uint32_t raw_bytes = raw_a + (g.b_stays ? 0u : raw_b), stage_bytes = 3 * (a_part + (g.b_stays ? 0u : b_part));
+    const uint32_t raws = base, stages = raws + raw_bytes * g.raws, all_b = stages + stage_bytes * g.stages;
+    float* blocks = reinterpret_cast<float*>(dynamic + (all_b - smem_of(dynamic)) + (g.b_stays ? (size_t)3 * b_part * g.blocks_k : 0));
+    volatile int* gave_up = &sh.gave_up;
+    const uint32_t raw_full = smem_of(sh.raw_full), raw_empty = smem_of(sh.raw_empty), full = smem_of(sh.full),
+                   empty = smem_of(sh.empty), sums_full = smem_of(sh.sums_full), sums_empty = smem_of(sh.sums_empty);
+
+    if (threadIdx.x == 0) {
+        sh.gave_up = 0;
+        for (int s = 0; s < g.raws; ++s) {
+            bar_init(raw_full + 8 * s, 1);
+            bar_init(raw_empty + 8 * s, kSplitters);
+        }
+        for (int s = 0; s < g.stages; ++s) {
+            bar_init(full + 8 * s, kSplitters);
+            bar_init(empty + 8 * s, 1);
+        }
+        for (int h = 0; h < g.slots; ++h) {
+            bar_init(sums_full + 8 * h, 1);
+            bar_init(sums_empty + 8 * h, 8);
+        }
+        bar_init(smem_of(&sh.drained), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tmem_alloc(smem_of(&sh.tmem), (uint32_t)g.columns);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            Turn raw;
+            int fills = 0;      // up to the ring's size
+            bool ok = true;
+            const auto room = [&](uint32_t bytes) {
+                if (!(ok = bar_wait(raw_empty + 8 * raw.at, raw.parity ^ 1u, gave_up))) return false;
+                bar_expect(raw_full + 8 * raw.at, bytes);
+                fills = min(fills + 1, g.raws);
+                return true;
+            };
+            const auto load = [&](auto down, const CUtensorMap* map, uint32_t to, int across, int extent, int k) {
+                if constexpr (decltype(down)::value) {
+                    for (int box = 0; box * 32 < extent; ++box)
+                        tma_load_2d(to + box * 4096, map, across + box * 32, k, raw_full + 8 * raw.at);
+                } else {
+                    tma_load_2d(to, map, k, across, raw_full + 8 * raw.at);
+                }
+            };
+            if (g.b_stays)
+                for (int b = 0; b < (int)g.blocks_k && ok; ++b) {
+                    if (!room(raw_b)) break;
+                    load(std::integral_constant<bool, B_DOWN>{}, &map_b, raws + raw.at * raw_bytes, 0, g.bn, b * kSplitBlock);
+                    raw.next(g.raws);
+                }
+            for (uint32_t item = blockIdx.x; item < g.items && ok; item += gridDim.x) {
+                const Tile t = tile_of(g, item);
+                int k = (int)t.k0;
+                for (int b = 0; b < t.blocks; ++b, k += kSplitBlock) {
+                    if (!room(raw_bytes)) break;
+                    const uint32_t to = raws + raw.at * raw_bytes;
+                    load(std::integral_constant<bool, A_DOWN>{}, &map_a, to, t.m * kTileM, kTileM, k);
+                    if (!g.b_stays) load(std::integral_constant<bool, B_DOWN>{}, &map_b, to + raw_a, t.n * g.bn, g.bn, k);
+                    raw.next(g.raws);
+                }
+            }
+            if (!ok) {      // the copies still under way end before the CTA does
+                for (int i = 0; i < fills; ++i) {
+                    if (raw.at == 0) raw.parity ^= 1u;
+                    raw.at = (raw.at == 0 ? g.raws : raw.at) - 1;
+                    bar_drain(raw_full + 8 * raw.at, raw.parity);
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            Turn turn, slot;
+            bool ok = true;
+            // a step along k: 32 bytes along rows, 16 rows of 128 bytes down them
+            constexpr uint64_t a_step = (A_DOWN ? 2048 : 32) >> 4, b_step = (B_DOWN ? 2048 : 32) >> 4;
+            const uint64_t ap = a_part >> 4, bp = b_part >> 4;
+            for (uint32_t item = blockIdx.x; item < g.items && ok; item += gridDim.x) {
+                const Tile t = tile_of(g, item);
+                int left = (int)min((int64_t)t.blocks * kSplitBlock, g.k - t.k0);
+                for (int b0 = 0; b0 < t.blocks && ok; slot.next(g.slots)) {
+                    const int b1 = min(t.blocks, b0 + kSplitPhase);
+                    const uint32_t sums = tmem + (uint32_t)(slot.at * 2 * g.bn), small = sums + (uint32_t)g.bn;
+                    if (!(ok = bar_wait(sums_empty + 8 * slot.at, slot.parity ^ 1u, gave_up))) break;
+                    bool add = false;
+                    for (; b0 < b1; ++b0, left -= kSplitBlock, turn.next(g.stages)) {
+                        if (!(ok = bar_wait(full + 8 * turn.at, turn.parity, gave_up))) break;
+                        tc_fence_after();
+                        const uint32_t at = stages + (uint32_t)turn.at * stage_bytes;
+                        const uint32_t at_b = g.b_stays ? all_b + (uint32_t)b0 * 3u * b_part : at + 3 * a_part;
+                        uint64_t a = tile_desc<A_DOWN ? 128 : 64>(at, 4096), b = tile_desc<B_DOWN ? 128 : 64>(at_b, 4096);
+                        const int steps = left > 16 ? 2 : 1;
+                        for (int i = 0; i < steps; ++i, a += a_step, b += b_step) {
+                            product<false>(sums, a, b, g.desc, add);
+                            product<false>(small, a + 2 * ap, b, g.desc, add);
+                            product<false>(small, a, b + 2 * bp, g.desc, true);
+                            product<false>(small, a + ap, b + bp, g.desc, true);
+                            product<false>(small, a + ap, b, g.desc, true);
+                            product<false>(small, a, b + bp, g.desc, true);
+                            add = true;
+                        }
+                        products_done(empty + 8 * turn.at);
+                    }
+                    if (ok) products_done(sums_full + 8 * slot.at);
+                }
+            }
+            if (!ok) {
+                products_done(smem_of(&sh.drained));
+                bar_drain(smem_of(&sh.drained), 0);
+                atomicAdd(&g_layer_timeouts, 1u);
+            }
+        }
+    } else if (warp < 2 + kSplitters) {
+        const int thread = threadIdx.x - 64;
+        Turn raw, turn;
+        bool ok = true;
+        // a warp is done with a raw stage, or has its share of a stage of parts in place
+        const auto tell = [&](uint32_t bar) {
+            __syncwarp();
+            if (lane == 0) bar_arrive(bar);
+        };
+        if (g.b_stays)
+            for (int b = 0; b < (int)g.blocks_k && ok; ++b) {
+                ok = __all_sync(0xffffffffu, bar_wait(raw_full + 8 * raw.at, raw.parity, gave_up));
+                if (!ok) break;
+                split_tile<B_DOWN>(raws + raw.at * raw_bytes, all_b + (uint32_t)b * 3u * b_part, g.bn, thread);
+                tell(raw_empty + 8 * raw.at);
+                raw.next(g.raws);
+            }
+        for (uint32_t item = blockIdx.x; item < g.items && ok; item += gridDim.x) {
+            const Tile t = tile_of(g, item);
+            for (int b = 0; b < t.blocks && ok; ++b) {
+                ok = __all_sync(0xffffffffu, bar_wait(empty + 8 * turn.at, turn.parity ^ 1u, gave_up) &&
+                                                     bar_wait(raw_full + 8 * raw.at, raw.parity, gave_up));
+                if (!ok) break;
+                const uint32_t from = raws + raw.at * raw_bytes, to = stages + (uint32_t)turn.at * stage_bytes;
+                split_tile<A_DOWN>(from, to, kTileM, thread);
+                if (!g.b_stays) split_tile<B_DOWN>(from + raw_a, to + 3 * a_part, g.bn, thread);
+                fence_async_shared();
+                tell(raw_empty + 8 * raw.at);
+                if (lane == 0) bar_arrive(full + 8 * turn.at);
+                raw.next(g.raws);
+                turn.next(g.stages);
+            }
+        }
+    } else {
+        const int quarter = warp & 3, which = (warp - 8) >> 2;
+        float* block = blocks + (size_t)(warp - 8) * 1024 * g.places;
+        Turn slot;
+        for (uint32_t item = blockIdx.x; item < g.items; item += gridDim.x) {
+            const Tile t = tile_of(g, item);
+            if (!finish_split<!A_DOWN && !B_DOWN>(g, t, kSplitPhase, slot, tmem, sums_full, sums_empty, gave_up, block, quarter, which,
+                                                  lane))
+                break;
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1) tmem_free(tmem, (uint32_t)g.columns);
 }
 
 // ---- few rows ------------------------------------------------------------------------------------------------------
@@ -983,7 +1232,7 @@ __global__ void __launch_bounds__(256) slope_kernel(const T* __restrict__ dy, co
 static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 struct Plan {
-    int bn, stages, slots, groups, b_stays, columns;
+    int bn, stages, raws, slots, groups, places, b_stays, columns;
     size_t stage;
     int64_t tiles_m, tiles_n, splits, split_blocks;
     size_t shared;
@@ -1040,15 +1289,42 @@ static Plan plan_product(int kind, bool a_down, bool b_down, int64_t m, int64_t 
 }
 
 // Stages and finishers once it is known how operands are loaded.
-static void plan_shared(Plan* p, bool bulk, int64_t blocks) {
+static void plan_shared(Plan* p, int kind, bool bulk, int64_t blocks) {
     const size_t room = kSharedLimit - 2048;
+    p->places = kind == kSplit && ceil_div(p->split_blocks, kPhaseBlocks) > 1 && p->bn > 64 ? 2 : 1;
+    const size_t finish = kFinishBytes * p->places;
     // twelve finishers where that leaves four stages
-    p->groups = bulk && 4 * p->stage + 3 * kFinishBytes <= room ? 3 : 2;
-    p->stages = (int)std::min<size_t>(kMaxStages, (room - p->groups * kFinishBytes) / p->stage);
+    p->groups = bulk && 4 * p->stage + 3 * finish <= room ? 3 : 2;
+    p->stages = (int)std::min<size_t>(kMaxStages, (room - p->groups * finish) / p->stage);
     p->b_stays = p->b_stays && blocks <= p->stages;
     if (p->b_stays) p->stages = (int)(p->stages / blocks * blocks);
     // more than half of the SM's shared memory: a second CTA would wait for tensor memory
-    p->shared = std::max<size_t>((size_t)p->stages * p->stage + p->groups * kFinishBytes + 1024, 120 * 1024);
+    p->shared = std::max<size_t>((size_t)p->stages * p->stage + p->groups * finish + 1024, 120 * 1024);
+}
+
+// The same of split_gemm_kernel.  Blocks are half as long as the plan counts them.
+static void plan_split(Plan* p, bool a_down, bool b_down, int64_t k) {
+    const int64_t blocks = ceil_div(k, kSplitBlock);
+    p->split_blocks *= 2;
+    p->places = p->split_blocks > kSplitPhase && p->bn > 64 ? 2 : 1;
+    p->groups = 2;
+    const size_t a = 3 * (a_down ? split_bytes<true>(kTileM) : split_bytes<false>(kTileM));
+    const size_t b = 3 * (b_down ? split_bytes<true>(p->bn) : split_bytes<false>(p->bn));
+    const size_t raw_a = kTileM * 128, raw_b = (size_t)p->bn * 128, finish = kFinishBytes * p->groups * p->places;
+    const size_t room = kSharedLimit - 2048 - finish;
+    // B stays where two stages of A's parts and three of its values fit beside it
+    p->b_stays = p->b_stays && b * blocks + 2 * a + 3 * raw_a <= room;
+    const size_t stay = p->b_stays ? b * blocks : 0, stage = a + (p->b_stays ? 0 : b), raw = raw_a + (p->b_stays ? 0 : raw_b);
+    // stages of parts, then of values, in turn while they fit
+    p->stages = 2;
+    p->raws = 2;
+    size_t used = stay + 2 * stage + 2 * raw;
+    for (bool more = true; more;) {
+        more = false;
+        if (p->raws < kMaxRaws && p->raws <= p->stages + 1 && used + raw <= room) { ++p->raws; used += raw; more = true; }
+        if (p->stages < 4 && used + stage <= room) { ++p->stages; used += stage; more = true; }
+    }
+    p->shared = std::max<size_t>(used + finish + 1024, 120 * 1024);
 }
 
 // ---- launches -----------------------------------------------------------------------------------------------------------
@@ -1066,10 +1342,11 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_tiled() {
 
 // Map of an operand for copies of `box_rows` rows of 128 bytes.
 static bool operand_map(CUtensorMap* map, int kind, int type, const Operand& o, int64_t rows, int64_t cols, int box_rows) {
-    const int bytes = kind == kEight ? 1 : 2;
+    const int bytes = kind == kEight ? 1 : kind == kSplit ? 4 : 2;
     const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)(o.stride * bytes)};
     const cuuint32_t box[2] = {(cuuint32_t)(kRowBytes / bytes), (cuuint32_t)box_rows}, steps[2] = {1, 1};
     const CUtensorMapDataType t = kind == kEight ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                  : kind == kSplit ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                   : type == ASHB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     const auto encode = encode_tiled();
     return encode != nullptr &&
@@ -1077,9 +1354,9 @@ static bool operand_map(CUtensorMap* map, int kind, int type, const Operand& o, 
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int KIND, bool BULK, bool A_DOWN, bool B_DOWN, bool STAYS>
-static cudaError_t launch_product(const GemmArgs& g, const Plan& p, const CUtensorMap& ma, const CUtensorMap& mb, cudaStream_t st) {
-    const auto kernel = layer_gemm_kernel<KIND, BULK, A_DOWN, B_DOWN, STAYS>;
+template <class Kernel>
+static cudaError_t launch_kernel(Kernel kernel, const GemmArgs& g, const Plan& p, const CUtensorMap& ma, const CUtensorMap& mb,
+                                 cudaStream_t st) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kSharedLimit - 1024));
     if (e != cudaSuccess) return e;
     kernel<<<(unsigned)std::min<int64_t>(g.items, sm_count()), kGemmThreads, p.shared, st>>>(g, ma, mb);
@@ -1094,17 +1371,21 @@ static int run_product(GemmArgs g, int type, Plan p, cudaStream_t st) {
     g.a.wide = starts(g.a) && (A_DOWN ? g.m : g.k) * kBytes % 16 == 0;
     g.b.wide = starts(g.b) && (B_DOWN ? g.n : g.k) * kBytes % 16 == 0;
     CUtensorMap ma{}, mb{};
-    const bool bulk = KIND != kSplit && starts(g.a) && starts(g.b) &&
-                      operand_map(&ma, KIND, type, g.a, A_DOWN ? g.k : g.m, A_DOWN ? g.m : g.k, A_DOWN ? 64 : kTileM) &&
-                      operand_map(&mb, KIND, type, g.b, B_DOWN ? g.k : g.n, B_DOWN ? g.n : g.k, B_DOWN ? 64 : p.bn);
-    plan_shared(&p, bulk, ceil_div(g.k, kBlockK<KIND>));
+    const int down = KIND == kSplit ? kSplitBlock : 64;      // rows of a box that k runs down
+    const bool bulk = starts(g.a) && starts(g.b) &&
+                      operand_map(&ma, KIND, type, g.a, A_DOWN ? g.k : g.m, A_DOWN ? g.m : g.k, A_DOWN ? down : kTileM) &&
+                      operand_map(&mb, KIND, type, g.b, B_DOWN ? g.k : g.n, B_DOWN ? g.n : g.k, B_DOWN ? down : p.bn);
+    if (KIND == kSplit && bulk) plan_split(&p, A_DOWN, B_DOWN, g.k);
+    else plan_shared(&p, KIND, bulk, ceil_div(g.k, kBlockK<KIND>));
     g.bn = p.bn;
     g.stages = p.stages;
     g.slots = p.slots;
     g.groups = p.groups;
+    g.places = p.places;
+    g.raws = p.raws;
     g.b_stays = p.b_stays;
     g.columns = p.columns;
-    const int64_t block = KIND == kEight ? 128 : 64;
+    const int64_t block = KIND == kEight ? 128 : KIND == kSplit && bulk ? kSplitBlock : 64;
     ASHB_REQUIRE(p.tiles_m * p.tiles_n * p.splits < (int64_t)1 << 31, "a product of %lld x %lld values", (long long)g.m, (long long)g.n);
     g.tiles_m = (uint32_t)p.tiles_m;
     g.tiles_n = (uint32_t)p.tiles_n;
@@ -1117,17 +1398,23 @@ static int run_product(GemmArgs g, int type, Plan p, cudaStream_t st) {
     g.desc = product_desc(kTileM, p.bn, KIND == kEight ? 0 : KIND == kSplit || type == ASHB_BF16 ? 1 : 0, A_DOWN, B_DOWN);
     if constexpr (KIND != kSplit) {
         if (bulk) {
-            ASHB_CUDA_TRY((launch_product<KIND, true, A_DOWN, B_DOWN, false>(g, p, ma, mb, st)));
+            ASHB_CUDA_TRY((launch_kernel(layer_gemm_kernel<KIND, true, A_DOWN, B_DOWN, false>, g, p, ma, mb, st)));
+            return ASHB_OK;
+        }
+    }
+    if constexpr (KIND == kSplit) {
+        if (bulk) {
+            ASHB_CUDA_TRY((launch_kernel(split_gemm_kernel<A_DOWN, B_DOWN>, g, p, ma, mb, st)));
             return ASHB_OK;
         }
     }
     if constexpr (!A_DOWN) {
         if (p.b_stays) {
-            ASHB_CUDA_TRY((launch_product<KIND, false, A_DOWN, B_DOWN, true>(g, p, ma, mb, st)));
+            ASHB_CUDA_TRY((launch_kernel(layer_gemm_kernel<KIND, false, A_DOWN, B_DOWN, true>, g, p, ma, mb, st)));
             return ASHB_OK;
         }
     }
-    ASHB_CUDA_TRY((launch_product<KIND, false, A_DOWN, B_DOWN, false>(g, p, ma, mb, st)));
+    ASHB_CUDA_TRY((launch_kernel(layer_gemm_kernel<KIND, false, A_DOWN, B_DOWN, false>, g, p, ma, mb, st)));
     return ASHB_OK;
 }
 

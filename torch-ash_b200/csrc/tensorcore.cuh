@@ -93,12 +93,15 @@ __device__ __forceinline__ void tmem_load32(uint32_t at, float (&r)[32]) {
 }
 
 // ---- products --------------------------------------------------------------------------------------------------------
-// A shared-memory tile in the 128-byte swizzle: groups of 8 rows of 128 bytes, 1024 bytes apart, the 16-byte word w of row r
-// at word w ^ (r & 7).  Rows are the tile's rows where the summed dimension lies along them; where the other dimension does
-// (64 values a row), `box` is the distance between blocks of 64 of them.  The tile starts at a multiple of 1024 bytes.
+// A shared-memory tile in a swizzle of rows of ROW_BYTES: groups of 8 rows follow one another, the 16-byte word w of row r at
+// word w ^ (r & 7) of rows of 128 bytes, at w ^ (r / 2 & 3) of rows of 64.  Rows are the tile's rows where the summed
+// dimension runs along them; where the other dimension does (64 values in 128 bytes), `box` is the distance between blocks of
+// 64 of them.  The tile starts at a multiple of 1024 bytes (512 for rows of 64).
+template <int ROW_BYTES = 128>
 __device__ __forceinline__ uint64_t tile_desc(uint32_t at, uint32_t box) {
-    return (uint64_t)((at >> 4) & 0x3FFFu) | (uint64_t)((box >> 4) & 0x3FFFu) << 16 | (uint64_t)(1024u >> 4) << 32 |
-           (uint64_t)1 << 46 | (uint64_t)2 << 61;
+    static_assert(ROW_BYTES == 128 || ROW_BYTES == 64, "");
+    return (uint64_t)((at >> 4) & 0x3FFFu) | (uint64_t)((box >> 4) & 0x3FFFu) << 16 | (uint64_t)((8u * ROW_BYTES) >> 4) << 32 |
+           (uint64_t)1 << 46 | (uint64_t)(ROW_BYTES == 128 ? 2 : 4) << 61;
 }
 
 // Instruction word: float32 sums of an M x N tile.  `format` of both operands: f16 0, bf16 1 (kind::f16); e4m3 0
