@@ -47,7 +47,6 @@ constexpr int kPhaseBlocks = 8;           // blocks of 64 between the float32 su
 constexpr int kMaxStages = 8;
 constexpr int kMaxSlots = 8;              // tiles whose sums are in tensor memory
 constexpr size_t kSharedLimit = 232448;
-constexpr size_t kFinishBytes = 4 * 32 * 32 * sizeof(float);      // of a group of four finishers
 
 enum Activation { kNone = ASHB_ACT_NONE, kRelu = ASHB_ACT_RELU, kSilu = ASHB_ACT_SILU, kGelu = ASHB_ACT_GELU, kSin = ASHB_ACT_SIN };
 
@@ -188,6 +187,8 @@ struct GemmArgs {
     // groups: of four finishers; places: blocks of a finisher in shared memory; columns: tensor memory to allocate
     int bn, stages, slots, groups, places, b_stays, columns;
     int raws;      // split_gemm_kernel: stages of values as they came
+    int bulk_out, bufs;      // finishing by bulk copies, from this many blocks in turn
+    int64_t finish_bytes;    // of shared memory, a finisher's
 };
 
 // Consecutive values of an operand that make one 16-byte word of each of its parts, at p; `left` of them exist, none if it is
@@ -593,6 +594,191 @@ __device__ __forceinline__ void finish(const GemmArgs& g, const float* block, ty
     }
 }
 
+// ---- finishing by bulk copies -------------------------------------------------------------------------------------------
+// Where rows of the output (and slope and residual) are multiples of 16 bytes: a lane keeps the row of the tile that tensor
+// memory gives it, takes the columns' biases from shared memory, where all lanes read the same word, writes its row to a
+// swizzled block there and one lane sends the block off as a tile; residuals come in the same way, into the block they leave
+// from.  No addresses, no bounds and no second pass through shared memory: a third of the instructions of a block that leaves
+// by stores of its own.
+struct FinishMaps {
+    CUtensorMap out, slope, residual;
+};
+
+template <class T>
+__device__ __forceinline__ uint32_t block_word(uint32_t row, int lane, int word) {      // 16-byte word of a lane's row
+    return row + (uint32_t)((word ^ (sizeof(T) == 4 ? lane & 7 : (lane >> 1) & 3)) << 4);
+}
+__device__ __forceinline__ uint4 get_word(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+    return v;
+}
+// Eight values of a lane's row, from column 8 j.
+template <class T>
+__device__ __forceinline__ void put_eight(uint32_t row, int lane, int j, const float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        put16(block_word<T>(row, lane, 2 * j), make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])));
+        put16(block_word<T>(row, lane, 2 * j + 1), make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])));
+    } else {
+        uint4 w;
+        T* t = reinterpret_cast<T*>(&w);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) t[k] = from_float<T>(v[k]);
+        put16(block_word<T>(row, lane, j), w);
+    }
+}
+template <class T>
+__device__ __forceinline__ void add_eight(uint32_t row, int lane, int j, float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        const uint4 a = get_word(block_word<T>(row, lane, 2 * j)), b = get_word(block_word<T>(row, lane, 2 * j + 1));
+        const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] += __uint_as_float(w[k]);
+    } else {
+        const uint4 a = get_word(block_word<T>(row, lane, j));
+        const T* t = reinterpret_cast<const T*>(&a);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] += to_float(t[k]);
+    }
+}
+
+// 32 columns of the warp's lanes, from tensor memory to the blocks at `out` and `slope`.  A short loop: its code stays where
+// instructions are fetched from.  columns: the biases (and e4m3 scales, 128 bytes on) of the columns.
+template <int KIND, class T, int ACT, bool SLOPE>
+__device__ __forceinline__ void bulk_block(const GemmArgs& g, uint32_t sums, uint32_t out, uint32_t slope, uint32_t columns, float row_scale,
+                                           int lane) {
+    const bool has_residual = g.f.residual != nullptr, has_bias = g.f.bias != nullptr;
+    const uint32_t out_row = out + (uint32_t)lane * (32 * sizeof(T)), slope_row = slope + (uint32_t)lane * (32 * sizeof(T));
+#pragma unroll 1
+    for (int j = 0; j < 4; ++j) {
+        float z[8], d[8];
+        if constexpr (KIND == kSplit) {
+            float small[8];
+            tmem_load8_twice(sums + 8u * j, sums + (uint32_t)g.bn + 8u * j, z, small);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) z[k] += small[k];
+        } else {
+            tmem_load8(sums + 8u * j, z);
+        }
+        if constexpr (KIND == kEight) {
+            const uint4 a = get_word(columns + 128u + 32u * j), b = get_word(columns + 144u + 32u * j);
+            const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int k = 0; k < 8; ++k) z[k] *= row_scale * __uint_as_float(w[k]);
+        }
+        if (has_bias) {
+            const uint4 a = get_word(columns + 32u * j), b = get_word(columns + 16u + 32u * j);
+            const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int k = 0; k < 8; ++k) z[k] += __uint_as_float(w[k]);
+        }
+        activate<ACT, SLOPE, sizeof(T) == 2>(g.f.omega, z, d);
+        if (SLOPE) put_eight<T>(slope_row, lane, j, d);
+        if (has_residual) add_eight<T>(out_row, lane, j, z);
+        put_eight<T>(out_row, lane, j, z);
+    }
+}
+
+template <int KIND, bool FORWARD, class T>
+__device__ __forceinline__ void bulk_typed(const GemmArgs& g, uint32_t sums, uint32_t out, uint32_t slope, uint32_t columns, float row_scale,
+                                           int lane) {
+    if constexpr (!FORWARD) {
+        bulk_block<KIND, T, kNone, false>(g, sums, out, slope, columns, row_scale, lane);
+    } else {
+        by_activation(g.f.activation, [&](auto act) {
+            constexpr int ACT = decltype(act)::value;
+            if constexpr (KIND != kEight && ACT != kNone) {
+                if (g.f.slope) {
+                    bulk_block<KIND, T, ACT, true>(g, sums, out, slope, columns, row_scale, lane);
+                    return;
+                }
+            }
+            bulk_block<KIND, T, ACT, false>(g, sums, out, slope, columns, row_scale, lane);
+        });
+    }
+}
+
+// The finishers of a kernel, by warp: `number` of 4 * groups.  scratch: this warp's blocks (g.bufs of out, then as many of
+// slope) and columns; arrivals: its g.bufs barriers for residuals.  A tile's blocks of 32 columns go to the groups in turn.
+template <int KIND, bool FORWARD>
+__device__ __forceinline__ void finish_bulk(const GemmArgs& g, const FinishMaps& maps, int number, int lane, uint32_t tmem,
+                                            uint32_t slot_columns, uint32_t sums_full, uint32_t sums_empty, uint32_t scratch,
+                                            uint32_t arrivals, volatile int* gave_up) {
+    const int quarter = threadIdx.x >> 5 & 3, n_blocks = (g.bn + 31) >> 5;
+    const uint32_t block = g.f.partial || g.f.type == ASHB_F32 ? 4096u : 2048u;
+    const uint32_t columns = scratch + block * g.bufs * (g.f.slope ? 2 : 1);
+    Turn slot, buf;
+    int blk = number >> 2;
+    bool ok = true;
+    for (uint32_t item = blockIdx.x; item < g.items && ok; item += gridDim.x) {
+        const Tile t = tile_of(g, item);
+        const int row0 = t.m * kTileM + quarter * 32;
+        for (; blk < n_blocks; blk += g.groups) {
+            const int col = t.n * g.bn + blk * 32;
+            const bool inside = row0 < g.m && col < g.n;
+            const uint32_t out = scratch + block * buf.at, slope = out + block * g.bufs;
+            float row_scale = 1.0f;
+            if (inside) {
+                if (lane == 0) {      // what left from this block has been read
+                    if (g.bufs == 2) tma_wait_read<1>();
+                    else tma_wait_read<0>();
+                }
+                __syncwarp();
+                if (FORWARD) {
+                    if (g.f.residual && lane == 0) {
+                        bar_expect(arrivals + 8 * buf.at, block);
+                        tma_load_3d(out, &maps.residual, col, row0, 0, arrivals + 8 * buf.at);
+                    }
+                    const int mine = col + lane;
+                    float b = 0.0f;
+                    if (g.f.bias && mine < g.n) {
+                        if (g.f.type == ASHB_F32) b = __ldg(static_cast<const float*>(g.f.bias) + mine);
+                        else if (g.f.type == ASHB_F16) b = to_float(static_cast<const __half*>(g.f.bias)[mine]);
+                        else b = to_float(static_cast<const __nv_bfloat16*>(g.f.bias)[mine]);
+                    }
+                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(columns + 4u * lane), "f"(b) : "memory");
+                    if constexpr (KIND == kEight) {
+                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(columns + 128u + 4u * lane), "f"(mine < g.n ? __ldg(g.f.b_scales + mine) : 0.0f)
+                                     : "memory");
+                        row_scale = row0 + lane < g.m ? __ldg(g.f.a_scales + row0 + lane) : 0.0f;
+                    }
+                    __syncwarp();
+                }
+            }
+            ok = bar_wait(sums_full + 8 * slot.at, slot.parity, gave_up);
+            if (FORWARD && inside && g.f.residual) ok = bar_wait(arrivals + 8 * buf.at, buf.parity, gave_up) && ok;
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) {
+                if (FORWARD && inside && g.f.residual) bar_drain(arrivals + 8 * buf.at, buf.parity);
+                break;
+            }
+            tc_fence_after();
+            if (inside) {
+                const uint32_t sums = tmem + (uint32_t)slot.at * slot_columns + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(blk * 32);
+                if (KIND == kSplit || (!FORWARD && g.f.partial) || (KIND == kEight && g.f.type == ASHB_F32))
+                    bulk_typed<KIND, FORWARD, float>(g, sums, out, slope, columns, row_scale, lane);
+                else if (g.f.type == ASHB_F16) bulk_typed<KIND, FORWARD, __half>(g, sums, out, slope, columns, row_scale, lane);
+                else bulk_typed<KIND, FORWARD, __nv_bfloat16>(g, sums, out, slope, columns, row_scale, lane);
+                tc_fence_before();
+                fence_async_shared();
+            }
+            __syncwarp();
+            if (lane == 0) {
+                bar_arrive(sums_empty + 8 * slot.at);
+                if (inside) {
+                    tma_store_3d(&maps.out, col, row0, t.split, out);
+                    if (FORWARD && g.f.slope) tma_store_3d(&maps.slope, col, row0, 0, slope);
+                    tma_commit();
+                }
+            }
+            if (inside) buf.next(g.bufs);
+        }
+        blk -= n_blocks;
+        slot.next(g.slots);
+    }
+    if (lane == 0) tma_wait_read<0>();
+}
+
 // Split products: a warp's share of a tile, the blocks `which` and `which` + 2 of 32 columns.  The two sums of a phase are added
 // in registers, those of later phases to what the block holds in shared memory (`block`: 32 x 32 values, of each block where
 // there are several phases).  False: a wait gave up.
@@ -637,7 +823,7 @@ __device__ __forceinline__ bool finish_split(const GemmArgs& g, const Tile& t, i
 }
 
 struct GemmShared {
-    uint64_t full[kMaxStages], empty[kMaxStages], sums_full[kMaxSlots], sums_empty[kMaxSlots], drained;
+    uint64_t full[kMaxStages], empty[kMaxStages], sums_full[kMaxSlots], sums_empty[kMaxSlots], residual[24], drained;
     uint32_t tmem;
     int gave_up;
 };
@@ -647,7 +833,8 @@ struct GemmShared {
 // STAYS (loaders with loads of their own): B is loaded once; the registers that held it hold a second tile of A under way.
 template <int KIND, bool BULK, bool A_DOWN, bool B_DOWN, bool STAYS>
 __global__ void __launch_bounds__(kGemmThreads, 1) layer_gemm_kernel(const GemmArgs g, const __grid_constant__ CUtensorMap map_a,
-                                                                     const __grid_constant__ CUtensorMap map_b) {
+                                                                     const __grid_constant__ CUtensorMap map_b,
+                                                                     const __grid_constant__ FinishMaps maps) {
     extern __shared__ __align__(1024) uint8_t dynamic[];
     __shared__ GemmShared sh;
     constexpr int kBlock = kBlockK<KIND>, kPartsOf = kParts<KIND>, kStep = KIND == kEight ? 32 : 16;
@@ -669,8 +856,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) layer_gemm_kernel(const GemmA
         }
         for (int h = 0; h < g.slots; ++h) {
             bar_init(sums_full + 8 * h, 1);
-            bar_init(sums_empty + 8 * h, KIND == kSplit ? 8 : 4 * ((g.bn + 31) >> 5));
+            bar_init(sums_empty + 8 * h, KIND == kSplit && !g.bulk_out ? 8 : 4 * ((g.bn + 31) >> 5));
         }
+        for (int i = 0; i < 24; ++i) bar_init(smem_of(sh.residual) + 8 * i, 1);
         bar_init(smem_of(&sh.drained), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -793,7 +981,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) layer_gemm_kernel(const GemmA
             }
         }
     } else if (warp == kProductWarp<BULK>) {
-        if (lane == 0) {
+        {
+            const uint32_t mine = elected();
             Turn turn, slot;
             bool ok = true;
             for (uint32_t item = blockIdx.x; item < g.items && ok; item += gridDim.x) {
@@ -817,40 +1006,45 @@ __global__ void __launch_bounds__(kGemmThreads, 1) layer_gemm_kernel(const GemmA
                             const uint64_t ap = a_part >> 4, bp = b_part >> 4;
                             const uint32_t small = sums + (uint32_t)g.bn;
                             for (int i = 0; i < steps; ++i, a += a_step, b += b_step) {
-                                product<false>(sums, a, b, g.desc, add);
-                                product<false>(small, a + 2 * ap, b, g.desc, add);
-                                product<false>(small, a, b + 2 * bp, g.desc, true);
-                                product<false>(small, a + ap, b + bp, g.desc, true);
-                                product<false>(small, a + ap, b, g.desc, true);
-                                product<false>(small, a, b + bp, g.desc, true);
+                                product<false>(mine, sums, a, b, g.desc, add);
+                                product<false>(mine, small, a + 2 * ap, b, g.desc, add);
+                                product<false>(mine, small, a, b + 2 * bp, g.desc, true);
+                                product<false>(mine, small, a + ap, b + bp, g.desc, true);
+                                product<false>(mine, small, a + ap, b, g.desc, true);
+                                product<false>(mine, small, a, b + bp, g.desc, true);
                                 add = true;
                             }
                         } else {
                             for (int i = 0; i < steps; ++i, a += a_step, b += b_step) {
-                                product<KIND == kEight>(sums, a, b, g.desc, add);
+                                product<KIND == kEight>(mine, sums, a, b, g.desc, add);
                                 add = true;
                             }
                         }
-                        products_done(empty + 8 * turn.at);
+                        products_done(mine, empty + 8 * turn.at);
                     }
-                    if (ok) products_done(sums_full + 8 * slot.at);
+                    if (ok) products_done(mine, sums_full + 8 * slot.at);
                 }
             }
             if (!ok) {      // tensor memory is not given back under products still running
-                products_done(smem_of(&sh.drained));
+                products_done(mine, smem_of(&sh.drained));
                 bar_drain(smem_of(&sh.drained), 0);
-                atomicAdd(&g_layer_timeouts, 1u);
+                if (mine) atomicAdd(&g_layer_timeouts, 1u);
             }
         }
     } else if (warp >= kFirstFinisher<BULK> && warp < kFirstFinisher<BULK> + 4 * g.groups) {
         // lanes of tensor memory that the warp may read, and its group: the blocks of 32 columns go to the groups in turn
         const int quarter = warp & 3, which = (warp - kFirstFinisher<BULK>) >> 2;
+        if (g.bulk_out) {
+            const int number = warp - kFirstFinisher<BULK>;
+            finish_bulk<KIND, kForward>(g, maps, number, lane, tmem, slot_columns, sums_full, sums_empty,
+                                        smem_of(blocks) + (uint32_t)(number * g.finish_bytes), smem_of(sh.residual) + 16 * number, gave_up);
+        }
         float* block = blocks + (size_t)(warp - kFirstFinisher<BULK>) * 32 * 32 * g.places;
         const int n_blocks = (g.bn + 31) >> 5;
         Turn slot;
         typename AheadOf<KIND>::type ahead;
         int blk = which;
-        for (uint32_t item = blockIdx.x; item < g.items; item += gridDim.x) {
+        for (uint32_t item = blockIdx.x; item < g.items && !g.bulk_out; item += gridDim.x) {
             const Tile t = tile_of(g, item);
             const int64_t row0 = (int64_t)t.m * kTileM + quarter * 32, col0 = (int64_t)t.n * g.bn;
             bool ok = true;
@@ -896,7 +1090,7 @@ constexpr int kMaxRaws = 6;
 
 struct SplitShared {
     uint64_t raw_full[kMaxRaws], raw_empty[kMaxRaws], full[kMaxStages], empty[kMaxStages], sums_full[kMaxSlots],
-            sums_empty[kMaxSlots], drained;
+            sums_empty[kMaxSlots], residual[24], drained;
     uint32_t tmem;
     int gave_up;
 };
@@ -939,7 +1133,8 @@ __device__ __forceinline__ void split_tile(uint32_t raw, uint32_t parts, int ext
 
 template <bool A_DOWN, bool B_DOWN>
 __global__ void __launch_bounds__(kGemmThreads, 1) split_gemm_kernel(const GemmArgs g, const __grid_constant__ CUtensorMap map_a,
-                                                                     const __grid_constant__ CUtensorMap map_b) {
+                                                                     const __grid_constant__ CUtensorMap map_b,
+                                                                     const __grid_constant__ FinishMaps maps) {
     extern __shared__ __align__(1024) uint8_t dynamic[];
     __shared__ SplitShared sh;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -966,8 +1161,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) split_gemm_kernel(const GemmA
         }
         for (int h = 0; h < g.slots; ++h) {
             bar_init(sums_full + 8 * h, 1);
-            bar_init(sums_empty + 8 * h, 8);
+            bar_init(sums_empty + 8 * h, g.bulk_out ? 4 * ((g.bn + 31) >> 5) : 8);
         }
+        for (int i = 0; i < 24; ++i) bar_init(smem_of(sh.residual) + 8 * i, 1);
         bar_init(smem_of(&sh.drained), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -1022,7 +1218,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) split_gemm_kernel(const GemmA
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
+        {
+            const uint32_t mine = elected();
             Turn turn, slot;
             bool ok = true;
             // a step along k: 32 bytes along rows, 16 rows of 128 bytes down them
@@ -1044,23 +1241,23 @@ __global__ void __launch_bounds__(kGemmThreads, 1) split_gemm_kernel(const GemmA
                         uint64_t a = tile_desc<A_DOWN ? 128 : 64>(at, 4096), b = tile_desc<B_DOWN ? 128 : 64>(at_b, 4096);
                         const int steps = left > 16 ? 2 : 1;
                         for (int i = 0; i < steps; ++i, a += a_step, b += b_step) {
-                            product<false>(sums, a, b, g.desc, add);
-                            product<false>(small, a + 2 * ap, b, g.desc, add);
-                            product<false>(small, a, b + 2 * bp, g.desc, true);
-                            product<false>(small, a + ap, b + bp, g.desc, true);
-                            product<false>(small, a + ap, b, g.desc, true);
-                            product<false>(small, a, b + bp, g.desc, true);
+                            product<false>(mine, sums, a, b, g.desc, add);
+                            product<false>(mine, small, a + 2 * ap, b, g.desc, add);
+                            product<false>(mine, small, a, b + 2 * bp, g.desc, true);
+                            product<false>(mine, small, a + ap, b + bp, g.desc, true);
+                            product<false>(mine, small, a + ap, b, g.desc, true);
+                            product<false>(mine, small, a, b + bp, g.desc, true);
                             add = true;
                         }
-                        products_done(empty + 8 * turn.at);
+                        products_done(mine, empty + 8 * turn.at);
                     }
-                    if (ok) products_done(sums_full + 8 * slot.at);
+                    if (ok) products_done(mine, sums_full + 8 * slot.at);
                 }
             }
             if (!ok) {
-                products_done(smem_of(&sh.drained));
+                products_done(mine, smem_of(&sh.drained));
                 bar_drain(smem_of(&sh.drained), 0);
-                atomicAdd(&g_layer_timeouts, 1u);
+                if (mine) atomicAdd(&g_layer_timeouts, 1u);
             }
         }
     } else if (warp < 2 + kSplitters) {
@@ -1098,9 +1295,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1) split_gemm_kernel(const GemmA
         }
     } else {
         const int quarter = warp & 3, which = (warp - 8) >> 2;
+        if (g.bulk_out)
+            finish_bulk<kSplit, !A_DOWN && !B_DOWN>(g, maps, warp - 8, lane, tmem, 2u * g.bn, sums_full, sums_empty,
+                                                    smem_of(blocks) + (uint32_t)((warp - 8) * g.finish_bytes),
+                                                    smem_of(sh.residual) + 16 * (warp - 8), gave_up);
         float* block = blocks + (size_t)(warp - 8) * 1024 * g.places;
         Turn slot;
-        for (uint32_t item = blockIdx.x; item < g.items; item += gridDim.x) {
+        for (uint32_t item = blockIdx.x; item < g.items && !g.bulk_out; item += gridDim.x) {
             const Tile t = tile_of(g, item);
             if (!finish_split<!A_DOWN && !B_DOWN>(g, t, kSplitPhase, slot, tmem, sums_full, sums_empty, gave_up, block, quarter, which,
                                                   lane))
@@ -1232,7 +1433,8 @@ __global__ void __launch_bounds__(256) slope_kernel(const T* __restrict__ dy, co
 static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 struct Plan {
-    int bn, stages, raws, slots, groups, places, b_stays, columns;
+    int bn, stages, raws, slots, groups, places, bulk_out, bufs, b_stays, columns;
+    int64_t finish_bytes;
     size_t stage;
     int64_t tiles_m, tiles_n, splits, split_blocks;
     size_t shared;
@@ -1288,32 +1490,53 @@ static Plan plan_product(int kind, bool a_down, bool b_down, int64_t m, int64_t 
     return best;
 }
 
-// Stages and finishers once it is known how operands are loaded.
-static void plan_shared(Plan* p, int kind, bool bulk, int64_t blocks) {
+// A finisher's shared memory: blocks that leave by bulk copies, and their columns' biases and scales, or a block (two, where
+// sums of several phases wait in them) whose values are stored.
+static size_t finisher_bytes(const Plan& p, int block, bool slope) {
+    return p.bulk_out ? (size_t)(block * p.bufs * (slope ? 2 : 1) + 1024) : (size_t)4096 * p.places;
+}
+
+// Stages and finishers once it is known how operands are loaded and results stored.  block: bytes of one that leaves by bulk copies.
+static void plan_shared(Plan* p, int kind, bool bulk, int64_t blocks, int block, bool slope) {
     const size_t room = kSharedLimit - 2048;
-    p->places = kind == kSplit && ceil_div(p->split_blocks, kPhaseBlocks) > 1 && p->bn > 64 ? 2 : 1;
-    const size_t finish = kFinishBytes * p->places;
-    // twelve finishers where that leaves four stages
-    p->groups = bulk && 4 * p->stage + 3 * finish <= room ? 3 : 2;
-    p->stages = (int)std::min<size_t>(kMaxStages, (room - p->groups * finish) / p->stage);
+    const bool phases = kind == kSplit && ceil_div(p->split_blocks, kPhaseBlocks) > 1;
+    p->bulk_out = p->bulk_out && !phases;
+    p->places = phases && p->bn > 64 ? 2 : 1;
+    // twelve finishers and two blocks each where that leaves four stages
+    p->groups = bulk ? 3 : 2;
+    p->bufs = 2;
+    const auto finish = [&] { return 4 * p->groups * finisher_bytes(*p, block, slope); };
+    if (4 * p->stage + finish() > room) p->bufs = 1;
+    if (4 * p->stage + finish() > room) p->groups = 2;
+    p->finish_bytes = (int64_t)finisher_bytes(*p, block, slope);
+    p->stages = (int)std::min<size_t>(kMaxStages, (room - finish()) / p->stage);
     p->b_stays = p->b_stays && blocks <= p->stages;
     if (p->b_stays) p->stages = (int)(p->stages / blocks * blocks);
     // more than half of the SM's shared memory: a second CTA would wait for tensor memory
-    p->shared = std::max<size_t>((size_t)p->stages * p->stage + p->groups * finish + 1024, 120 * 1024);
+    p->shared = std::max<size_t>((size_t)p->stages * p->stage + finish() + 1024, 120 * 1024);
 }
 
 // The same of split_gemm_kernel.  Blocks are half as long as the plan counts them.
-static void plan_split(Plan* p, bool a_down, bool b_down, int64_t k) {
+static void plan_split(Plan* p, bool a_down, bool b_down, int64_t k, bool slope) {
     const int64_t blocks = ceil_div(k, kSplitBlock);
     p->split_blocks *= 2;
-    p->places = p->split_blocks > kSplitPhase && p->bn > 64 ? 2 : 1;
+    const bool phases = p->split_blocks > kSplitPhase;
+    p->bulk_out = p->bulk_out && !phases;
+    p->places = phases && p->bn > 64 ? 2 : 1;
     p->groups = 2;
     const size_t a = 3 * (a_down ? split_bytes<true>(kTileM) : split_bytes<false>(kTileM));
     const size_t b = 3 * (b_down ? split_bytes<true>(p->bn) : split_bytes<false>(p->bn));
-    const size_t raw_a = kTileM * 128, raw_b = (size_t)p->bn * 128, finish = kFinishBytes * p->groups * p->places;
-    const size_t room = kSharedLimit - 2048 - finish;
-    // B stays where two stages of A's parts and three of its values fit beside it
-    p->b_stays = p->b_stays && b * blocks + 2 * a + 3 * raw_a <= room;
+    const size_t raw_a = kTileM * 128, raw_b = (size_t)p->bn * 128, all = kSharedLimit - 2048;
+    // B stays where two stages of A's parts and three of its values fit beside it and the smallest finishers
+    const size_t least = 8 * (size_t)(p->bulk_out ? 4096 * (slope ? 2 : 1) + 1024 : 4096 * p->places);
+    p->b_stays = p->b_stays && b * blocks + 2 * a + 3 * raw_a + least <= all;
+    const size_t operands = p->b_stays ? b * blocks + 2 * a + 3 * raw_a : 2 * (a + b + raw_a + raw_b);
+    // two blocks of a finisher, else one, else blocks that are stored value by value
+    p->bufs = 2;
+    if (8 * finisher_bytes(*p, 4096, slope) + operands > all) p->bufs = 1;
+    if (8 * finisher_bytes(*p, 4096, slope) + operands > all) p->bulk_out = 0;
+    p->finish_bytes = (int64_t)finisher_bytes(*p, 4096, slope);
+    const size_t finish = 8 * (size_t)p->finish_bytes, room = all - finish;
     const size_t stay = p->b_stays ? b * blocks : 0, stage = a + (p->b_stays ? 0 : b), raw = raw_a + (p->b_stays ? 0 : raw_b);
     // stages of parts, then of values, in turn while they fit
     p->stages = 2;
@@ -1354,12 +1577,36 @@ static bool operand_map(CUtensorMap* map, int kind, int type, const Operand& o, 
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Map of what leaves (or of residuals): blocks of 32 x 32, `splits` times m rows of n values.
+static bool block_map(CUtensorMap* map, const void* at, int type, int64_t stride, int64_t m, int64_t n, int64_t splits) {
+    const int bytes = value_bytes(type);
+    if (((uintptr_t)at & 15) != 0 || stride * bytes % 16 != 0) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)n, (cuuint64_t)m, (cuuint64_t)splits};
+    const cuuint64_t strides[2] = {(cuuint64_t)(stride * bytes), (cuuint64_t)(stride * m * bytes)};
+    const cuuint32_t box[3] = {32, 32, 1}, steps[3] = {1, 1, 1};
+    const CUtensorMapDataType t = type == ASHB_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                  : type == ASHB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const auto encode = encode_tiled();
+    return encode != nullptr &&
+           encode(map, t, 3, const_cast<void*>(at), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  bytes == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+static bool finish_maps(FinishMaps* maps, const GemmArgs& g, int64_t splits) {
+    const Finish& f = g.f;
+    const int type = f.partial ? ASHB_F32 : f.type;
+    return block_map(&maps->out, f.partial ? (const void*)f.partial : f.out, type, g.n, g.m, g.n, splits) &&
+           (!f.slope || block_map(&maps->slope, f.slope, type, g.n, g.m, g.n, 1)) &&
+           (!f.residual || block_map(&maps->residual, f.residual, type, f.residual_stride, g.m, g.n, 1));
+}
+
 template <class Kernel>
 static cudaError_t launch_kernel(Kernel kernel, const GemmArgs& g, const Plan& p, const CUtensorMap& ma, const CUtensorMap& mb,
-                                 cudaStream_t st) {
+                                 const FinishMaps& maps, cudaStream_t st) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kSharedLimit - 1024));
     if (e != cudaSuccess) return e;
-    kernel<<<(unsigned)std::min<int64_t>(g.items, sm_count()), kGemmThreads, p.shared, st>>>(g, ma, mb);
+    kernel<<<(unsigned)std::min<int64_t>(g.items, sm_count()), kGemmThreads, p.shared, st>>>(g, ma, mb, maps);
     return cudaGetLastError();
 }
 
@@ -1375,8 +1622,13 @@ static int run_product(GemmArgs g, int type, Plan p, cudaStream_t st) {
     const bool bulk = starts(g.a) && starts(g.b) &&
                       operand_map(&ma, KIND, type, g.a, A_DOWN ? g.k : g.m, A_DOWN ? g.m : g.k, A_DOWN ? down : kTileM) &&
                       operand_map(&mb, KIND, type, g.b, B_DOWN ? g.k : g.n, B_DOWN ? g.n : g.k, B_DOWN ? down : p.bn);
-    if (KIND == kSplit && bulk) plan_split(&p, A_DOWN, B_DOWN, g.k);
-    else plan_shared(&p, KIND, bulk, ceil_div(g.k, kBlockK<KIND>));
+    FinishMaps maps{};
+    p.bulk_out = finish_maps(&maps, g, p.splits);
+    if (KIND == kSplit && bulk) plan_split(&p, A_DOWN, B_DOWN, g.k, g.f.slope != nullptr);
+    else plan_shared(&p, KIND, bulk, ceil_div(g.k, kBlockK<KIND>), g.f.partial || g.f.type == ASHB_F32 ? 4096 : 2048, g.f.slope != nullptr);
+    g.bulk_out = p.bulk_out;
+    g.bufs = p.bufs;
+    g.finish_bytes = p.finish_bytes;
     g.bn = p.bn;
     g.stages = p.stages;
     g.slots = p.slots;
@@ -1398,23 +1650,23 @@ static int run_product(GemmArgs g, int type, Plan p, cudaStream_t st) {
     g.desc = product_desc(kTileM, p.bn, KIND == kEight ? 0 : KIND == kSplit || type == ASHB_BF16 ? 1 : 0, A_DOWN, B_DOWN);
     if constexpr (KIND != kSplit) {
         if (bulk) {
-            ASHB_CUDA_TRY((launch_kernel(layer_gemm_kernel<KIND, true, A_DOWN, B_DOWN, false>, g, p, ma, mb, st)));
+            ASHB_CUDA_TRY((launch_kernel(layer_gemm_kernel<KIND, true, A_DOWN, B_DOWN, false>, g, p, ma, mb, maps, st)));
             return ASHB_OK;
         }
     }
     if constexpr (KIND == kSplit) {
         if (bulk) {
-            ASHB_CUDA_TRY((launch_kernel(split_gemm_kernel<A_DOWN, B_DOWN>, g, p, ma, mb, st)));
+            ASHB_CUDA_TRY((launch_kernel(split_gemm_kernel<A_DOWN, B_DOWN>, g, p, ma, mb, maps, st)));
             return ASHB_OK;
         }
     }
     if constexpr (!A_DOWN) {
         if (p.b_stays) {
-            ASHB_CUDA_TRY((launch_kernel(layer_gemm_kernel<KIND, false, A_DOWN, B_DOWN, true>, g, p, ma, mb, st)));
+            ASHB_CUDA_TRY((launch_kernel(layer_gemm_kernel<KIND, false, A_DOWN, B_DOWN, true>, g, p, ma, mb, maps, st)));
             return ASHB_OK;
         }
     }
-    ASHB_CUDA_TRY((launch_kernel(layer_gemm_kernel<KIND, false, A_DOWN, B_DOWN, false>, g, p, ma, mb, st)));
+    ASHB_CUDA_TRY((launch_kernel(layer_gemm_kernel<KIND, false, A_DOWN, B_DOWN, false>, g, p, ma, mb, maps, st)));
     return ASHB_OK;
 }
 

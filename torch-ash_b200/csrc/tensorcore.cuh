@@ -62,6 +62,23 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
             "l"(map), "r"(x), "r"(y), "r"(bar)
             : "memory");
 }
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+    asm volatile(
+            "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+            "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+            : "memory");
+}
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, int x, int y, int z, uint32_t src) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map), "r"(x), "r"(y), "r"(z),
+                 "r"(src)
+                 : "memory");
+}
+__device__ __forceinline__ void tma_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// Until all but the last PENDING groups of this thread's stores have read their shared memory.
+template <int PENDING>
+__device__ __forceinline__ void tma_wait_read() {
+    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(PENDING) : "memory");
+}
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // ---- tensor memory -------------------------------------------------------------------------------------------------
@@ -92,6 +109,36 @@ __device__ __forceinline__ void tmem_load32(uint32_t at, float (&r)[32]) {
     for (int c = 0; c < 32; ++c) r[c] = __uint_as_float(u[c]);
 }
 
+// Eight columns.
+__device__ __forceinline__ void tmem_load8(uint32_t at, float (&r)[8]) {
+    uint32_t u[8];
+    asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\t"
+            "tcgen05.wait::ld.sync.aligned;"
+            : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7])
+            : "r"(at)
+            : "memory");
+#pragma unroll
+    for (int c = 0; c < 8; ++c) r[c] = __uint_as_float(u[c]);
+}
+// Eight columns of each of two sums.
+__device__ __forceinline__ void tmem_load8_twice(uint32_t at, uint32_t at2, float (&r)[8], float (&s)[8]) {
+    uint32_t u[8], v[8];
+    asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%16];\n\t"
+            "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8,%9,%10,%11,%12,%13,%14,%15}, [%17];\n\t"
+            "tcgen05.wait::ld.sync.aligned;"
+            : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(v[0]), "=r"(v[1]),
+              "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+            : "r"(at), "r"(at2)
+            : "memory");
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+        r[c] = __uint_as_float(u[c]);
+        s[c] = __uint_as_float(v[c]);
+    }
+}
+
 // ---- products --------------------------------------------------------------------------------------------------------
 // A shared-memory tile in a swizzle of rows of ROW_BYTES: groups of 8 rows follow one another, the 16-byte word w of row r at
 // word w ^ (r & 7) of rows of 128 bytes, at w ^ (r / 2 & 3) of rows of 64.  Rows are the tile's rows where the summed
@@ -111,28 +158,51 @@ constexpr uint32_t product_desc(int m, int n, int format, bool a_rows, bool b_ro
            (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24;
 }
 
+// The warp that issues products runs as a whole and one lane of it issues: what the instructions take then stays in registers
+// that the warp shares, where a branch for one lane has every operand moved there first (a product of 64 columns took 85
+// cycles to issue, and 32 to run).
+__device__ __forceinline__ uint32_t elected() {
+    uint32_t mine;
+    asm volatile(
+            "{\n\t"
+            ".reg .pred p;\n\t"
+            "elect.sync _|p, 0xffffffff;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t"
+            "}"
+            : "=r"(mine));
+    return mine;
+}
+
 template <bool EIGHT_BITS>
-__device__ __forceinline__ void product(uint32_t to, uint64_t a, uint64_t b, uint32_t desc, bool add) {
+__device__ __forceinline__ void product(uint32_t mine, uint32_t to, uint64_t a, uint64_t b, uint32_t desc, bool add) {
     if constexpr (EIGHT_BITS)
         asm volatile(
                 "{\n\t"
-                ".reg .pred p;\n\t"
+                ".reg .pred p, q;\n\t"
                 "setp.ne.b32 p, %4, 0;\n\t"
-                "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
-                "}" ::"r"(to), "l"(a), "l"(b), "r"(desc), "r"((uint32_t)add)
+                "setp.ne.b32 q, %5, 0;\n\t"
+                "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
+                "}" ::"r"(to), "l"(a), "l"(b), "r"(desc), "r"((uint32_t)add), "r"(mine)
                 : "memory");
     else
         asm volatile(
                 "{\n\t"
-                ".reg .pred p;\n\t"
+                ".reg .pred p, q;\n\t"
                 "setp.ne.b32 p, %4, 0;\n\t"
-                "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
-                "}" ::"r"(to), "l"(a), "l"(b), "r"(desc), "r"((uint32_t)add)
+                "setp.ne.b32 q, %5, 0;\n\t"
+                "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+                "}" ::"r"(to), "l"(a), "l"(b), "r"(desc), "r"((uint32_t)add), "r"(mine)
                 : "memory");
 }
 // Arrives on `bar` once the products issued before are done.
-__device__ __forceinline__ void products_done(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+__device__ __forceinline__ void products_done(uint32_t mine, uint32_t bar) {
+    asm volatile(
+            "{\n\t"
+            ".reg .pred q;\n\t"
+            "setp.ne.b32 q, %1, 0;\n\t"
+            "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t"
+            "}" ::"r"(bar), "r"(mine)
+            : "memory");
 }
 
 }  // namespace ashb
