@@ -26,6 +26,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstring>
 
 #include "columnsums.cuh"
@@ -58,12 +59,13 @@ __device__ unsigned int g_layer_timeouts = 0;
 
 // sin(x + turn pi / 2), turn 0 or 1.  Reduction by a multiple k of pi in two parts (W. J. Cody, W. Waite, Software Manual for
 // the Elementary Functions, 1980): k times the first part is a multiple of x's last place, so the first step is exact.
-// Then the Taylor series to the 13th power, whose remainder within pi / 2 is below 2^-29.  Phases beyond 2^17, where a
-// float32 phase is good to 2^-7 at best, take the library's reduction.
+// Then an odd polynomial fitted to the sine on 1.01 times (-pi / 2, pi / 2), the largest error made least: of degree 9 it is
+// 5.2e-9, of degree 7 (for results rounded to 16 bits) 9.6e-7.  Phases beyond 2^17, where a float32 phase is good to 2^-7 at
+// best, take the library's reduction.
 constexpr float kLongPhase = 131072.0f;
 __device__ __noinline__ float long_phase(float x, int turn) { return turn ? cosf(x) : sinf(x); }
 
-template <int TURN>
+template <int TURN, bool ROUNDED>
 __device__ __forceinline__ float short_phase(float x) {
     constexpr float kRound = 12582912.0f;             // 1.5 * 2^23: what is added to it is rounded to a whole number
     // cos x = (-1)^(m+1) sin(x - (m + 1/2) pi)
@@ -73,11 +75,15 @@ __device__ __forceinline__ float short_phase(float x) {
     float r = fmaf(-k, 3.14159274f, x);               // pi rounded to float32
     r = fmaf(-k, -8.74227766e-8f, r);                 // and what that leaves
     const float u = r * r;
-    float p = fmaf(u, 1.6059044e-10f, -2.5052108e-8f);      // 1/13!, -1/11!
-    p = fmaf(u, p, 2.7557319e-6f);
-    p = fmaf(u, p, -1.9841270e-4f);
-    p = fmaf(u, p, 8.3333333e-3f);
-    p = fmaf(u, p, -1.6666667e-1f);
+    float p;
+    if (ROUNDED) {
+        p = fmaf(u, -0.00018465964f, 0.008311534f);
+        p = fmaf(u, p, -0.16665621f);
+    } else {
+        p = fmaf(u, 2.5970119e-06f, -0.00019805235f);
+        p = fmaf(u, p, 0.008332998f);
+        p = fmaf(u, p, -0.16666657f);
+    }
     return __uint_as_float(__float_as_uint(fmaf(u * r, p, r)) ^ sign);
 }
 
@@ -109,8 +115,8 @@ __device__ __forceinline__ float activate_one(float omega, float z, float& slope
             return z * c;
         }
     } else if constexpr (ACT == kSin) {
-        if (SLOPE) slope = omega * short_phase<1>(omega * z);
-        return short_phase<0>(omega * z);
+        if (SLOPE) slope = omega * short_phase<1, ROUNDED>(omega * z);
+        return short_phase<0, ROUNDED>(omega * z);
     } else {
         if (SLOPE) slope = 1.0f;
         return z;
@@ -1464,9 +1470,12 @@ static Plan plan_product(int kind, bool a_down, bool b_down, int64_t m, int64_t 
         p.tiles_m = ceil_div(m, kTileM);
         p.tiles_n = ceil_div(n, bn);
         const int64_t tiles = p.tiles_m * p.tiles_n, blocks = ceil_div(k, block);
-        const int64_t most = may_split ? std::min<int64_t>(std::max<int64_t>(1, blocks / 4), ceil_div(2 * sms, tiles)) : 1;
-        for (int64_t s = 1; s <= most; ++s) {
-            const int64_t per = ceil_div(blocks, s), splits = ceil_div(blocks, per);
+        const int64_t most = may_split ? std::max<int64_t>(1, blocks / 4) : 1;
+        // no splits, or as many as make one or two rounds of the SMs
+        const int64_t tries[3] = {1, std::min(most, sms / tiles), std::min(most, 2 * sms / tiles)};
+        for (int i = 0; i < 3; ++i) {
+            if (tries[i] < 1 || (i > 0 && tries[i] <= tries[i - 1])) continue;
+            const int64_t per = ceil_div(blocks, tries[i]), splits = ceil_div(blocks, per);
             // a split writes and reads its sums once more: 8 bytes a value at about 3000 bytes a cycle of the whole GPU
             const double join = splits > 1 ? 8.0 * splits * m * n / 3000.0 + 3000.0 : 0.0;
             const double c = cycles(kind, bn, per, tiles * splits, sms) + join;
@@ -1601,11 +1610,20 @@ static bool finish_maps(FinishMaps* maps, const GemmArgs& g, int64_t splits) {
            (!f.residual || block_map(&maps->residual, f.residual, type, f.residual_stride, g.m, g.n, 1));
 }
 
-template <class Kernel>
-static cudaError_t launch_kernel(Kernel kernel, const GemmArgs& g, const Plan& p, const CUtensorMap& ma, const CUtensorMap& mb,
+template <auto kernel>
+static cudaError_t launch_kernel(const GemmArgs& g, const Plan& p, const CUtensorMap& ma, const CUtensorMap& mb,
                                  const FinishMaps& maps, cudaStream_t st) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kSharedLimit - 1024));
+    // once a kernel and device: a call of the runtime less on every launch
+    static std::atomic<uint64_t> told{0};
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
     if (e != cudaSuccess) return e;
+    const uint64_t bit = device < 64 ? 1ull << device : 0;
+    if (!(told.load(std::memory_order_acquire) & bit)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kSharedLimit - 1024));
+        if (e != cudaSuccess) return e;
+        told.fetch_or(bit, std::memory_order_release);
+    }
     kernel<<<(unsigned)std::min<int64_t>(g.items, sm_count()), kGemmThreads, p.shared, st>>>(g, ma, mb, maps);
     return cudaGetLastError();
 }
@@ -1650,23 +1668,23 @@ static int run_product(GemmArgs g, int type, Plan p, cudaStream_t st) {
     g.desc = product_desc(kTileM, p.bn, KIND == kEight ? 0 : KIND == kSplit || type == ASHB_BF16 ? 1 : 0, A_DOWN, B_DOWN);
     if constexpr (KIND != kSplit) {
         if (bulk) {
-            ASHB_CUDA_TRY((launch_kernel(layer_gemm_kernel<KIND, true, A_DOWN, B_DOWN, false>, g, p, ma, mb, maps, st)));
+            ASHB_CUDA_TRY((launch_kernel<layer_gemm_kernel<KIND, true, A_DOWN, B_DOWN, false>>(g, p, ma, mb, maps, st)));
             return ASHB_OK;
         }
     }
     if constexpr (KIND == kSplit) {
         if (bulk) {
-            ASHB_CUDA_TRY((launch_kernel(split_gemm_kernel<A_DOWN, B_DOWN>, g, p, ma, mb, maps, st)));
+            ASHB_CUDA_TRY((launch_kernel<split_gemm_kernel<A_DOWN, B_DOWN>>(g, p, ma, mb, maps, st)));
             return ASHB_OK;
         }
     }
     if constexpr (!A_DOWN) {
         if (p.b_stays) {
-            ASHB_CUDA_TRY((launch_kernel(layer_gemm_kernel<KIND, false, A_DOWN, B_DOWN, true>, g, p, ma, mb, maps, st)));
+            ASHB_CUDA_TRY((launch_kernel<layer_gemm_kernel<KIND, false, A_DOWN, B_DOWN, true>>(g, p, ma, mb, maps, st)));
             return ASHB_OK;
         }
     }
-    ASHB_CUDA_TRY((launch_kernel(layer_gemm_kernel<KIND, false, A_DOWN, B_DOWN, false>, g, p, ma, mb, maps, st)));
+    ASHB_CUDA_TRY((launch_kernel<layer_gemm_kernel<KIND, false, A_DOWN, B_DOWN, false>>(g, p, ma, mb, maps, st)));
     return ASHB_OK;
 }
 
