@@ -713,74 +713,105 @@ __device__ __forceinline__ void finish_bulk(const GemmArgs& g, const FinishMaps&
     const int quarter = threadIdx.x >> 5 & 3, n_blocks = (g.bn + 31) >> 5;
     const uint32_t block = g.f.partial || g.f.type == ASHB_F32 ? 4096u : 2048u;
     const uint32_t columns = scratch + block * g.bufs * (g.f.slope ? 2 : 1);
+    const bool fetches = FORWARD && g.f.residual != nullptr;
+    // the next place among the groups' blocks, and how many tiles on it is
+    const auto settle = [&](uint32_t& item, int& blk) {
+        int tiles = 0;
+        while (blk >= n_blocks) {
+            blk -= n_blocks;
+            item += gridDim.x;
+            ++tiles;
+        }
+        return tiles;
+    };
+    const auto fetch = [&](uint32_t to, uint32_t bar, int col, int row0) {
+        bar_expect(bar, block);
+        tma_load_3d(to, &maps.residual, col, row0, 0, bar);
+    };
     Turn slot, buf;
+    uint32_t item = blockIdx.x;
     int blk = number >> 2;
-    bool ok = true;
-    for (uint32_t item = blockIdx.x; item < g.items && ok; item += gridDim.x) {
-        const Tile t = tile_of(g, item);
-        const int row0 = t.m * kTileM + quarter * 32;
-        for (; blk < n_blocks; blk += g.groups) {
-            const int col = t.n * g.bn + blk * 32;
-            const bool inside = row0 < g.m && col < g.n;
-            const uint32_t out = scratch + block * buf.at, slope = out + block * g.bufs;
-            float row_scale = 1.0f;
-            if (inside) {
-                if (lane == 0) {      // what left from this block has been read
-                    if (g.bufs == 2) tma_wait_read<1>();
-                    else tma_wait_read<0>();
-                }
-                __syncwarp();
-                if (FORWARD) {
-                    if (g.f.residual && lane == 0) {
-                        bar_expect(arrivals + 8 * buf.at, block);
-                        tma_load_3d(out, &maps.residual, col, row0, 0, arrivals + 8 * buf.at);
-                    }
-                    const int mine = col + lane;
-                    float b = 0.0f;
-                    if (g.f.bias && mine < g.n) {
-                        if (g.f.type == ASHB_F32) b = __ldg(static_cast<const float*>(g.f.bias) + mine);
-                        else if (g.f.type == ASHB_F16) b = to_float(static_cast<const __half*>(g.f.bias)[mine]);
-                        else b = to_float(static_cast<const __nv_bfloat16*>(g.f.bias)[mine]);
-                    }
-                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(columns + 4u * lane), "f"(b) : "memory");
-                    if constexpr (KIND == kEight) {
-                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(columns + 128u + 4u * lane), "f"(mine < g.n ? __ldg(g.f.b_scales + mine) : 0.0f)
-                                     : "memory");
-                        row_scale = row0 + lane < g.m ? __ldg(g.f.a_scales + row0 + lane) : 0.0f;
-                    }
-                    __syncwarp();
-                }
+    for (int n = settle(item, blk); n > 0; --n) slot.next(g.slots);
+    Tile t{};
+    if (item < g.items) t = tile_of(g, item);
+    bool under_way = false;      // this block's residuals, fetched while the block before was worked on
+    while (item < g.items) {
+        const int row0 = t.m * kTileM + quarter * 32, col = t.n * g.bn + blk * 32;
+        const bool inside = row0 < g.m && col < g.n;
+        uint32_t next_item = item;
+        int next_blk = blk + g.groups;
+        const int tiles = settle(next_item, next_blk);
+        Tile next = t;
+        if (tiles && next_item < g.items) next = tile_of(g, next_item);
+        const uint32_t out = scratch + block * buf.at, slope = out + block * g.bufs;
+        const Turn here = buf;
+        float row_scale = 1.0f;
+        bool next_under_way = false;
+        if (inside) {
+            buf.next(g.bufs);
+            if (lane == 0 && !under_way) {      // what left from this block has been read
+                if (g.bufs == 2) tma_wait_read<1>();
+                else tma_wait_read<0>();
+                if (fetches) fetch(out, arrivals + 8 * here.at, col, row0);
             }
-            ok = bar_wait(sums_full + 8 * slot.at, slot.parity, gave_up);
-            if (FORWARD && inside && g.f.residual) ok = bar_wait(arrivals + 8 * buf.at, buf.parity, gave_up) && ok;
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) {
-                if (FORWARD && inside && g.f.residual) bar_drain(arrivals + 8 * buf.at, buf.parity);
-                break;
-            }
-            tc_fence_after();
-            if (inside) {
-                const uint32_t sums = tmem + (uint32_t)slot.at * slot_columns + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(blk * 32);
-                if (KIND == kSplit || (!FORWARD && g.f.partial) || (KIND == kEight && g.f.type == ASHB_F32))
-                    bulk_typed<KIND, FORWARD, float>(g, sums, out, slope, columns, row_scale, lane);
-                else if (g.f.type == ASHB_F16) bulk_typed<KIND, FORWARD, __half>(g, sums, out, slope, columns, row_scale, lane);
-                else bulk_typed<KIND, FORWARD, __nv_bfloat16>(g, sums, out, slope, columns, row_scale, lane);
-                tc_fence_before();
-                fence_async_shared();
+            if (fetches && g.bufs == 2 && next_item < g.items) {
+                const int next_row = next.m * kTileM + quarter * 32, next_col = next.n * g.bn + next_blk * 32;
+                next_under_way = next_row < g.m && next_col < g.n;
+                if (next_under_way && lane == 0) {
+                    tma_wait_read<0>();
+                    fetch(scratch + block * buf.at, arrivals + 8 * buf.at, next_col, next_row);
+                }
             }
             __syncwarp();
-            if (lane == 0) {
-                bar_arrive(sums_empty + 8 * slot.at);
-                if (inside) {
-                    tma_store_3d(&maps.out, col, row0, t.split, out);
-                    if (FORWARD && g.f.slope) tma_store_3d(&maps.slope, col, row0, 0, slope);
-                    tma_commit();
+            if (FORWARD) {
+                const int mine = col + lane;
+                float b = 0.0f;
+                if (g.f.bias && mine < g.n) {
+                    if (g.f.type == ASHB_F32) b = __ldg(static_cast<const float*>(g.f.bias) + mine);
+                    else if (g.f.type == ASHB_F16) b = to_float(static_cast<const __half*>(g.f.bias)[mine]);
+                    else b = to_float(static_cast<const __nv_bfloat16*>(g.f.bias)[mine]);
                 }
+                asm volatile("st.shared.f32 [%0], %1;" ::"r"(columns + 4u * lane), "f"(b) : "memory");
+                if constexpr (KIND == kEight) {
+                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(columns + 128u + 4u * lane), "f"(mine < g.n ? __ldg(g.f.b_scales + mine) : 0.0f)
+                                 : "memory");
+                    row_scale = row0 + lane < g.m ? __ldg(g.f.a_scales + row0 + lane) : 0.0f;
+                }
+                __syncwarp();
             }
-            if (inside) buf.next(g.bufs);
         }
-        blk -= n_blocks;
-        slot.next(g.slots);
+        bool ok = bar_wait(sums_full + 8 * slot.at, slot.parity, gave_up);
+        if (fetches && inside) ok = bar_wait(arrivals + 8 * here.at, here.parity, gave_up) && ok;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) {      // the copies still under way end before the CTA does
+            if (fetches && inside) bar_drain(arrivals + 8 * here.at, here.parity);
+            if (next_under_way) bar_drain(arrivals + 8 * buf.at, buf.parity);
+            break;
+        }
+        tc_fence_after();
+        if (inside) {
+            const uint32_t sums = tmem + (uint32_t)slot.at * slot_columns + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(blk * 32);
+            if (KIND == kSplit || (!FORWARD && g.f.partial) || (KIND == kEight && g.f.type == ASHB_F32))
+                bulk_typed<KIND, FORWARD, float>(g, sums, out, slope, columns, row_scale, lane);
+            else if (g.f.type == ASHB_F16) bulk_typed<KIND, FORWARD, __half>(g, sums, out, slope, columns, row_scale, lane);
+            else bulk_typed<KIND, FORWARD, __nv_bfloat16>(g, sums, out, slope, columns, row_scale, lane);
+            tc_fence_before();
+            fence_async_shared();
+        }
+        __syncwarp();
+        if (lane == 0) {
+            bar_arrive(sums_empty + 8 * slot.at);
+            if (inside) {
+                tma_store_3d(&maps.out, col, row0, t.split, out);
+                if (FORWARD && g.f.slope) tma_store_3d(&maps.slope, col, row0, 0, slope);
+                tma_commit();
+            }
+        }
+        for (int n = tiles; n > 0; --n) slot.next(g.slots);
+        item = next_item;
+        blk = next_blk;
+        t = next;
+        under_way = next_under_way;
     }
     if (lane == 0) tma_wait_read<0>();
 }
@@ -1511,12 +1542,13 @@ static void plan_shared(Plan* p, int kind, bool bulk, int64_t blocks, int block,
     const bool phases = kind == kSplit && ceil_div(p->split_blocks, kPhaseBlocks) > 1;
     p->bulk_out = p->bulk_out && !phases;
     p->places = phases && p->bn > 64 ? 2 : 1;
-    // twelve finishers and two blocks each where that leaves four stages
+    // twelve finishers and two blocks each where that leaves four stages, or three where a tile has no more than two
+    const size_t stages = (p->split_blocks <= 2 ? 3 : 4) * p->stage;
     p->groups = bulk ? 3 : 2;
     p->bufs = 2;
     const auto finish = [&] { return 4 * p->groups * finisher_bytes(*p, block, slope); };
-    if (4 * p->stage + finish() > room) p->bufs = 1;
-    if (4 * p->stage + finish() > room) p->groups = 2;
+    if (stages + finish() > room) p->groups = 2;
+    if (stages + finish() > room) p->bufs = 1;
     p->finish_bytes = (int64_t)finisher_bytes(*p, block, slope);
     p->stages = (int)std::min<size_t>(kMaxStages, (room - finish()) / p->stage);
     p->b_stays = p->b_stays && blocks <= p->stages;

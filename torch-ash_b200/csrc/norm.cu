@@ -7,7 +7,10 @@
 //   gradient, with g = dy w:  dx = dr = ds + rstd (g - s rstd^2 mean(g s)),   dw = sum over rows of dy s rstd
 //
 // Everything is memory traffic: each input is read once and each output written once, the row staying in the
-// registers of the lanes that share it between the sum of squares, the largest magnitude and the stores.  Sums are
+// registers of the lanes that share it between the sum of squares, the largest magnitude and the stores.  Accesses are 16
+// bytes.  Rows that are no multiples of that are taken through windows: the row's lanes walk the 16-byte words that hold it,
+// whose first and last it shares with its neighbours and stores value by value (12383 rows of 3230 bf16 values with gradients
+// 518 us with accesses of one value, %(window)s so).  Sums are
 // float32; s enters the statistics before it is rounded to its type, the backward pass reads it rounded.  A row has
 // 8, 32 or 256 threads by its width; rows wider than 8192 are read again for each of their passes.
 // The weight's gradient is summed by a thread over the rows of its CTA, then over the CTAs in their order by a second
@@ -34,6 +37,7 @@ struct NormGradArgs {
     void* dx;
     float* partial;    // [CTAs][width]
     int64_t rows, width;
+    int64_t period;    // rows from one to the next that begins alike in a 16-byte word
 };
 
 // Reductions over the TPR threads of a row (a CTA of 256 threads where TPR is 256; `shared` has 2 x 8 words, used in turn).
@@ -64,8 +68,44 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* shared) {
     return v;
 }
 
-// VEC values an access (one where rows or buffers are not aligned for more), NV accesses a thread.
-template <class T, int VEC, int TPR, int NV, bool QUANT>
+// VEC values of a row at p from column `col`, which may begin before the row or end behind it (WINDOW): what is not the row's is
+// zero.  `whole`: the 16 bytes are the tensor's.
+template <bool WINDOW, class T, int VEC>
+__device__ __forceinline__ void load_cols(const T* __restrict__ p, int col, int width, bool whole, float (&v)[VEC]) {
+    if (!WINDOW || whole) {
+        load_n<T, VEC>(p + col, v);
+        if (WINDOW) {
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) v[k] = (unsigned)(col + k) < (unsigned)width ? v[k] : 0.0f;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) v[k] = (unsigned)(col + k) < (unsigned)width ? to_float(p[col + k]) : 0.0f;
+    }
+}
+template <bool WINDOW, class T, int VEC>
+__device__ __forceinline__ void store_cols(T* __restrict__ p, int col, int width, const float (&v)[VEC]) {
+    if (!WINDOW || (col >= 0 && col + VEC <= width)) {
+        store_n<T, VEC>(p + col, v);
+    } else {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k)
+            if ((unsigned)(col + k) < (unsigned)width) p[col + k] = from_float<T>(v[k]);
+    }
+}
+// The weights of columns: through windows they lie askew, and come one by one, from L1.
+template <bool WINDOW, class T, int VEC>
+__device__ __forceinline__ void load_weights(const T* __restrict__ w, int col, int width, float (&v)[VEC]) {
+    if constexpr (!WINDOW) {
+        load_n<T, VEC>(w + col, v);
+    } else {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) v[k] = (unsigned)(col + k) < (unsigned)width ? to_float(__ldg(w + col + k)) : 0.0f;
+    }
+}
+
+// VEC values an access (one where rows have strides or buffers are not aligned for more), NV accesses a thread.
+template <class T, int VEC, int TPR, int NV, bool QUANT, bool WINDOW>
 __global__ void __launch_bounds__(256) norm_forward_kernel(const NormArgs a) {
     __shared__ float shared[16];
     const int sub = threadIdx.x % TPR;
@@ -74,27 +114,31 @@ __global__ void __launch_bounds__(256) norm_forward_kernel(const NormArgs a) {
     const T* x = static_cast<const T*>(a.x) + (live ? row * a.x_stride : 0);
     const T* r = a.residual ? static_cast<const T*>(a.residual) + (live ? row * a.residual_stride : 0) : nullptr;
     const T* w = static_cast<const T*>(a.weight);
+    const int width = (int)a.width;
+    const int64_t at = live ? row * a.width : 0;
+    const int skew = WINDOW ? (int)(at % VEC) : 0;                                              // columns before the row in its first word
+    const int behind = (int)min(a.rows * a.width - at, (int64_t)1 << 20);                       // first column behind the tensor
     float v[NV][VEC];
     float squares = 0.0f;
+    const auto column = [&](int j) { return (j * TPR + sub) * VEC - skew; };
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        const int64_t col = ((int64_t)j * TPR + sub) * VEC;
-        const bool in = live && col < a.width;
+        const int col = column(j);
 #pragma unroll
         for (int k = 0; k < VEC; ++k) v[j][k] = 0.0f;
-        if (in) load_n<T, VEC>(x + col, v[j]);
+        if (live && col < width) load_cols<WINDOW, T, VEC>(x, col, width, col + VEC <= behind, v[j]);
     }
     if (r != nullptr) {
-        T* s = static_cast<T*>(a.sum) + (live ? row * a.width : 0);
+        T* s = static_cast<T*>(a.sum) + at;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int64_t col = ((int64_t)j * TPR + sub) * VEC;
-            if (live && col < a.width) {
+            const int col = column(j);
+            if (live && col < width) {
                 float u[VEC];
-                load_n<T, VEC>(r + col, u);
+                load_cols<WINDOW, T, VEC>(r, col, width, col + VEC <= behind, u);
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) v[j][k] += u[k];
-                store_n<T, VEC>(s + col, v[j]);
+                store_cols<WINDOW, T, VEC>(s, col, width, v[j]);
             }
         }
     }
@@ -108,17 +152,18 @@ __global__ void __launch_bounds__(256) norm_forward_kernel(const NormArgs a) {
     uint32_t amax = 0;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        const int64_t col = ((int64_t)j * TPR + sub) * VEC;
-        if (live && col < a.width) {
+        const int col = column(j);
+        if (live && col < width) {
             float u[VEC];
-            load_n<T, VEC>(w + col, u);
+            load_weights<WINDOW, T, VEC>(w, col, width, u);
 #pragma unroll
             for (int k = 0; k < VEC; ++k) v[j][k] = v[j][k] * rstd * u[k];
             if constexpr (QUANT) {
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) amax = max(amax, magnitude_bits(v[j][k]));
+                for (int k = 0; k < VEC; ++k)      // not of columns beside the row: there a rstd of infinity makes NaN of zero
+                    if (!WINDOW || (col + k >= 0 && col + k < width)) amax = max(amax, magnitude_bits(v[j][k]));
             } else {
-                store_n<T, VEC>(static_cast<T*>(a.y) + row * a.width + col, v[j]);
+                store_cols<WINDOW, T, VEC>(static_cast<T*>(a.y) + at, col, width, v[j]);
             }
         }
     }
@@ -127,11 +172,11 @@ __global__ void __launch_bounds__(256) norm_forward_kernel(const NormArgs a) {
         if (!live) return;
         const RowScale q(amax, kFormatE4M3);
         if (sub == 0) a.scales[row] = q.scale;
-        uint8_t* codes = a.codes + row * a.width;
+        uint8_t* codes = a.codes + at;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int64_t col = ((int64_t)j * TPR + sub) * VEC;
-            if (col >= a.width) continue;
+            const int col = column(j);
+            if (col >= width) continue;
             if constexpr (VEC == 1) {
                 const float u[4] = {v[j][0], 0.0f, 0.0f, 0.0f};
                 codes[col] = (uint8_t)encode4(u, q.inverse, kFormatE4M3);
@@ -142,8 +187,14 @@ __global__ void __launch_bounds__(256) norm_forward_kernel(const NormArgs a) {
                     const float u[4] = {v[j][4 * h], v[j][4 * h + 1], v[j][4 * h + 2], v[j][4 * h + 3]};
                     c[h] = encode4(u, q.inverse, kFormatE4M3);
                 }
-                if constexpr (VEC == 8) *reinterpret_cast<uint2*>(codes + col) = make_uint2(c[0], c[1]);
-                else *reinterpret_cast<uint32_t*>(codes + col) = c[0];
+                if (!WINDOW || (col >= 0 && col + VEC <= width)) {
+                    if constexpr (VEC == 8) *reinterpret_cast<uint2*>(codes + col) = make_uint2(c[0], c[1]);
+                    else *reinterpret_cast<uint32_t*>(codes + col) = c[0];
+                } else {
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k)
+                        if (col + k >= 0 && col + k < width) codes[col + k] = (uint8_t)(c[k / 4] >> (8 * (k % 4)));
+                }
             }
         }
     }
@@ -188,43 +239,54 @@ __global__ void __launch_bounds__(256) norm_forward_long_kernel(const NormArgs a
     }
 }
 
-// Rows in turn, so that a thread keeps the weight's gradient of its columns in registers.
-template <class T, int VEC, int TPR, int NV>
-__global__ void __launch_bounds__(256) norm_backward_kernel(const NormGradArgs a) {
+// Rows in turn, so that a thread keeps the weight's gradient of its columns in registers.  Through windows the columns of a
+// thread depend on where its row begins in a 16-byte word: a group takes rows that begin alike, `period` apart.
+template <class T, int VEC, int TPR, int NV, bool WINDOW>
+__global__ void __launch_bounds__(256, NV * VEC <= 8 ? 4 : NV * VEC <= 16 ? 3 : 2) norm_backward_kernel(const NormGradArgs a) {
     __shared__ float shared[16];
     extern __shared__ float columns[];     // width: the CTA's sums
     constexpr int kGroups = 256 / TPR;
     const int sub = threadIdx.x % TPR, group = threadIdx.x / TPR;
     const T* w = static_cast<const T*>(a.weight);
+    const int64_t groups = (int64_t)gridDim.x * kGroups, me = (int64_t)blockIdx.x * kGroups + group;      // a multiple of 8
+    const int64_t start = WINDOW ? me % a.period : 0, step = WINDOW ? a.period : 1;
+    const int skew = WINDOW ? (int)(start * a.width % VEC) : 0, width = (int)a.width;
     float dw[NV][VEC];
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
         for (int k = 0; k < VEC; ++k) dw[j][k] = 0.0f;
+    const auto column = [&](int j) { return (j * TPR + sub) * VEC - skew; };
     int turn = 0;
-    for (int64_t first = (int64_t)blockIdx.x * kGroups; first < a.rows; first += (int64_t)gridDim.x * kGroups) {
-        const int64_t row = first + group;
+    // as many rounds for every group, that the lanes of a warp and the threads of a CTA stay together
+    const int64_t rounds = (a.rows + groups - 1) / groups + (WINDOW ? 1 : 0);
+    for (int64_t round = 0; round < rounds; ++round) {
+        const int64_t row = start + step * (me / step + round * (groups / step));
         const bool live = row < a.rows;
         const int64_t at = live ? row * a.width : 0;
+        const int behind = (int)min(a.rows * a.width - at, (int64_t)1 << 20);
         const float rstd = live ? a.rstd[row] : 0.0f;
-        float s[NV][VEC], g[NV][VEC];
+        // all that the row needs at once: what is added at the end would be another round trip to memory after the sum
+        float s[NV][VEC], g[NV][VEC], ds[NV][VEC];
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int64_t col = ((int64_t)j * TPR + sub) * VEC;
+            const int col = column(j);
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) s[j][k] = g[j][k] = 0.0f;
-            if (live && col < a.width) {
-                load_n<T, VEC>(static_cast<const T*>(a.s) + at + col, s[j]);
-                load_n<T, VEC>(static_cast<const T*>(a.dy) + at + col, g[j]);
+            for (int k = 0; k < VEC; ++k) s[j][k] = g[j][k] = ds[j][k] = 0.0f;
+            if (live && col < width) {
+                load_cols<WINDOW, T, VEC>(static_cast<const T*>(a.s) + at, col, width, col + VEC <= behind, s[j]);
+                load_cols<WINDOW, T, VEC>(static_cast<const T*>(a.dy) + at, col, width, col + VEC <= behind, g[j]);
+                if (a.dsum != nullptr)
+                    load_cols<WINDOW, T, VEC>(static_cast<const T*>(a.dsum) + at, col, width, col + VEC <= behind, ds[j]);
             }
         }
         float dot = 0.0f;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int64_t col = ((int64_t)j * TPR + sub) * VEC;
-            if (col < a.width) {
+            const int col = column(j);
+            if (col < width) {
                 float u[VEC];
-                load_n<T, VEC>(w + col, u);
+                load_weights<WINDOW, T, VEC>(w, col, width, u);
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) {
                     dw[j][k] = fmaf(g[j][k] * s[j][k], rstd, dw[j][k]);
@@ -239,16 +301,11 @@ __global__ void __launch_bounds__(256) norm_backward_kernel(const NormGradArgs a
         const float c = rstd * rstd * (dot / (float)a.width);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int64_t col = ((int64_t)j * TPR + sub) * VEC;
-            if (live && col < a.width) {
-                float u[VEC];
-                if (a.dsum != nullptr) load_n<T, VEC>(static_cast<const T*>(a.dsum) + at + col, u);
+            const int col = column(j);
+            if (live && col < width) {
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) {
-                    const float d = rstd * fmaf(-s[j][k], c, g[j][k]);
-                    u[k] = a.dsum != nullptr ? u[k] + d : d;
-                }
-                store_n<T, VEC>(static_cast<T*>(a.dx) + at + col, u);
+                for (int k = 0; k < VEC; ++k) ds[j][k] += rstd * fmaf(-s[j][k], c, g[j][k]);
+                store_cols<WINDOW, T, VEC>(static_cast<T*>(a.dx) + at, col, width, ds[j]);
             }
         }
     }
@@ -259,13 +316,13 @@ __global__ void __launch_bounds__(256) norm_backward_kernel(const NormGradArgs a
             for (int j = 0; j < NV; ++j)
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) {
-                    const int64_t col = ((int64_t)j * TPR + sub) * VEC + k;
-                    if (col < a.width) columns[col] = owner == 0 ? dw[j][k] : columns[col] + dw[j][k];
+                    const int col = column(j) + k;
+                    if (col >= 0 && col < width) columns[col] = owner == 0 ? dw[j][k] : columns[col] + dw[j][k];
                 }
         }
         __syncthreads();
     }
-    for (int64_t col = threadIdx.x; col < a.width; col += 256) a.partial[blockIdx.x * a.width + col] = columns[col];
+    for (int64_t col = threadIdx.x; col < width; col += 256) a.partial[blockIdx.x * a.width + col] = columns[col];
 }
 
 // Rows beyond registers: a CTA a row in turn, the CTA's sums in its row of `partial` from the start.
@@ -301,39 +358,43 @@ __global__ void __launch_bounds__(256) norm_backward_long_kernel(const NormGradA
 constexpr int64_t kLongRow = 8192;
 
 // Threads a row and accesses a thread for a width: as few threads as keep 32 values or less each, so that narrow rows
-// leave no lane idle; the largest NV of a vector width is 32 / VEC.
+// leave no lane idle; the largest NV of a vector width is 32 / VEC.  A window may be a word longer than its row.
+static int threads_of(int64_t width, int vec, bool window) {
+    const int64_t most = width + (window ? vec - 1 : 0);
+    return most <= 64 ? 8 : most <= 1024 ? 32 : 256;
+}
 template <class F>
-static void by_width(int64_t width, int vec, F&& f) {
-    const int tpr = width <= 64 ? 8 : width <= 1024 ? 32 : 256;
+static void by_width(int64_t width, int vec, bool window, F&& f) {
+    const int tpr = threads_of(width, vec, window);
     int nv = 1;
-    while ((int64_t)nv * vec * tpr < width) nv <<= 1;
+    while ((int64_t)nv * vec * tpr < width + (window ? vec - 1 : 0)) nv <<= 1;
     f(tpr, nv);
 }
 
-template <class T, int VEC, int TPR, bool QUANT>
+template <class T, int VEC, int TPR, bool QUANT, bool WINDOW>
 static void launch_forward(const NormArgs& a, int nv, cudaStream_t st) {
     const unsigned grid = (unsigned)((a.rows + 256 / TPR - 1) / (256 / TPR));
     switch (nv) {
-        case 1: norm_forward_kernel<T, VEC, TPR, 1, QUANT><<<grid, 256, 0, st>>>(a); break;
-        case 2: norm_forward_kernel<T, VEC, TPR, 2, QUANT><<<grid, 256, 0, st>>>(a); break;
-        case 4: norm_forward_kernel<T, VEC, TPR, 4, QUANT><<<grid, 256, 0, st>>>(a); break;
+        case 1: norm_forward_kernel<T, VEC, TPR, 1, QUANT, WINDOW><<<grid, 256, 0, st>>>(a); break;
+        case 2: norm_forward_kernel<T, VEC, TPR, 2, QUANT, WINDOW><<<grid, 256, 0, st>>>(a); break;
+        case 4: norm_forward_kernel<T, VEC, TPR, 4, QUANT, WINDOW><<<grid, 256, 0, st>>>(a); break;
         default:
             if constexpr (VEC <= 4) {
-                if (nv == 8) { norm_forward_kernel<T, VEC, TPR, 8, QUANT><<<grid, 256, 0, st>>>(a); break; }
+                if (nv == 8) { norm_forward_kernel<T, VEC, TPR, 8, QUANT, WINDOW><<<grid, 256, 0, st>>>(a); break; }
             }
             if constexpr (VEC == 1 && TPR >= 32) {
-                if (nv == 16) { norm_forward_kernel<T, VEC, TPR, 16, QUANT><<<grid, 256, 0, st>>>(a); break; }
-                norm_forward_kernel<T, VEC, TPR, 32, QUANT><<<grid, 256, 0, st>>>(a);
+                if (nv == 16) { norm_forward_kernel<T, VEC, TPR, 16, QUANT, WINDOW><<<grid, 256, 0, st>>>(a); break; }
+                norm_forward_kernel<T, VEC, TPR, 32, QUANT, WINDOW><<<grid, 256, 0, st>>>(a);
             }
     }
 }
 
-template <class T, int VEC, bool QUANT>
+template <class T, int VEC, bool QUANT, bool WINDOW>
 static void forward_by_width(const NormArgs& a, cudaStream_t st) {
-    by_width(a.width, VEC, [&](int tpr, int nv) {
-        if (tpr == 8) launch_forward<T, VEC, 8, QUANT>(a, nv, st);
-        else if (tpr == 32) launch_forward<T, VEC, 32, QUANT>(a, nv, st);
-        else launch_forward<T, VEC, 256, QUANT>(a, nv, st);
+    by_width(a.width, VEC, WINDOW, [&](int tpr, int nv) {
+        if (tpr == 8) launch_forward<T, VEC, 8, QUANT, WINDOW>(a, nv, st);
+        else if (tpr == 32) launch_forward<T, VEC, 32, QUANT, WINDOW>(a, nv, st);
+        else launch_forward<T, VEC, 256, QUANT, WINDOW>(a, nv, st);
     });
 }
 
@@ -347,40 +408,47 @@ static bool aligned(uintptr_t bytes, std::initializer_list<const void*> pointers
 template <class T>
 static void forward_typed(const NormArgs& a, cudaStream_t st) {
     constexpr int kVec = 16 / sizeof(T);
-    const bool wide = a.width % kVec == 0 && a.x_stride % kVec == 0 && a.residual_stride % kVec == 0 &&
-                      aligned(16, {a.x, a.residual, a.weight, a.y, a.sum}) && aligned(kVec, {a.codes});
+    const bool based = aligned(16, {a.x, a.residual, a.weight, a.y, a.sum}) && aligned(kVec, {a.codes});
+    const bool wide = based && a.width % kVec == 0 && a.x_stride % kVec == 0 && a.residual_stride % kVec == 0;
+    const bool window = based && a.width >= kVec && a.width + kVec - 1 <= kLongRow && a.x_stride == a.width &&
+                        (!a.residual || a.residual_stride == a.width);
     if (a.width > kLongRow) {
         if (a.codes) norm_forward_long_kernel<T, true><<<(unsigned)a.rows, 256, 0, st>>>(a);
         else norm_forward_long_kernel<T, false><<<(unsigned)a.rows, 256, 0, st>>>(a);
     } else if (wide) {
-        if (a.codes) forward_by_width<T, kVec, true>(a, st);
-        else forward_by_width<T, kVec, false>(a, st);
+        if (a.codes) forward_by_width<T, kVec, true, false>(a, st);
+        else forward_by_width<T, kVec, false, false>(a, st);
+    } else if (window) {
+        if (a.codes) forward_by_width<T, kVec, true, true>(a, st);
+        else forward_by_width<T, kVec, false, true>(a, st);
     } else {
-        if (a.codes) forward_by_width<T, 1, true>(a, st);
-        else forward_by_width<T, 1, false>(a, st);
+        if (a.codes) forward_by_width<T, 1, true, false>(a, st);
+        else forward_by_width<T, 1, false, false>(a, st);
     }
 }
 
 // CTAs of the backward pass: what is resident at once, and no more than there are rows for.
+// Whole multiples of eight where a CTA has one row at a time, for windows.
 static unsigned backward_ctas(int64_t rows, int64_t width) {
-    const int groups = width <= 64 ? 32 : width <= 1024 ? 8 : 1;
-    return (unsigned)std::max<int64_t>(1, std::min<int64_t>((rows + groups - 1) / groups, (int64_t)sm_count() * 4));
+    const int groups = 256 / threads_of(width, 8, true);
+    const int64_t ctas = std::max<int64_t>(1, std::min<int64_t>((rows + groups - 1) / groups, (int64_t)sm_count() * 4));
+    return (unsigned)(groups == 1 ? (ctas + 7) / 8 * 8 : ctas);
 }
 
-template <class T, int VEC, int TPR>
+template <class T, int VEC, int TPR, bool WINDOW>
 static void launch_backward(const NormGradArgs& a, int nv, unsigned grid, cudaStream_t st) {
     const size_t smem = (size_t)a.width * 4;
     switch (nv) {
-        case 1: norm_backward_kernel<T, VEC, TPR, 1><<<grid, 256, smem, st>>>(a); break;
-        case 2: norm_backward_kernel<T, VEC, TPR, 2><<<grid, 256, smem, st>>>(a); break;
-        case 4: norm_backward_kernel<T, VEC, TPR, 4><<<grid, 256, smem, st>>>(a); break;
+        case 1: norm_backward_kernel<T, VEC, TPR, 1, WINDOW><<<grid, 256, smem, st>>>(a); break;
+        case 2: norm_backward_kernel<T, VEC, TPR, 2, WINDOW><<<grid, 256, smem, st>>>(a); break;
+        case 4: norm_backward_kernel<T, VEC, TPR, 4, WINDOW><<<grid, 256, smem, st>>>(a); break;
         default:
             if constexpr (VEC <= 4) {
-                if (nv == 8) { norm_backward_kernel<T, VEC, TPR, 8><<<grid, 256, smem, st>>>(a); break; }
+                if (nv == 8) { norm_backward_kernel<T, VEC, TPR, 8, WINDOW><<<grid, 256, smem, st>>>(a); break; }
             }
             if constexpr (VEC == 1 && TPR >= 32) {
-                if (nv == 16) { norm_backward_kernel<T, VEC, TPR, 16><<<grid, 256, smem, st>>>(a); break; }
-                norm_backward_kernel<T, VEC, TPR, 32><<<grid, 256, smem, st>>>(a);
+                if (nv == 16) { norm_backward_kernel<T, VEC, TPR, 16, WINDOW><<<grid, 256, smem, st>>>(a); break; }
+                norm_backward_kernel<T, VEC, TPR, 32, WINDOW><<<grid, 256, smem, st>>>(a);
             }
     }
 }
@@ -391,17 +459,19 @@ static void backward_typed(const NormGradArgs& a, unsigned grid, void* dw, cudaS
     if (a.width > kLongRow) {
         norm_backward_long_kernel<T><<<grid, 256, 0, st>>>(a);
     } else {
-        const bool wide = a.width % kVec == 0 && aligned(16, {a.dy, a.dsum, a.s, a.weight, a.dx});
-        const auto go = [&](auto vec) {
+        const bool based = aligned(16, {a.dy, a.dsum, a.s, a.weight, a.dx});
+        const auto go = [&](auto vec, auto window) {
             constexpr int VEC = decltype(vec)::value;
-            by_width(a.width, VEC, [&](int tpr, int nv) {
-                if (tpr == 8) launch_backward<T, VEC, 8>(a, nv, grid, st);
-                else if (tpr == 32) launch_backward<T, VEC, 32>(a, nv, grid, st);
-                else launch_backward<T, VEC, 256>(a, nv, grid, st);
+            constexpr bool WINDOW = decltype(window)::value;
+            by_width(a.width, VEC, WINDOW, [&](int tpr, int nv) {
+                if (tpr == 8) launch_backward<T, VEC, 8, WINDOW>(a, nv, grid, st);
+                else if (tpr == 32) launch_backward<T, VEC, 32, WINDOW>(a, nv, grid, st);
+                else launch_backward<T, VEC, 256, WINDOW>(a, nv, grid, st);
             });
         };
-        if (wide) go(std::integral_constant<int, kVec>{});
-        else go(std::integral_constant<int, 1>{});
+        if (based && a.width % kVec == 0) go(std::integral_constant<int, kVec>{}, std::false_type{});
+        else if (based && a.width >= kVec && a.width + kVec - 1 <= kLongRow) go(std::integral_constant<int, kVec>{}, std::true_type{});
+        else go(std::integral_constant<int, 1>{}, std::false_type{});
     }
     launch_sums<T>(Sums{a.partial, grid, a.width, dw}, Sums{}, st);
 }
@@ -453,7 +523,9 @@ int ashb_rms_norm_backward(int dtype, const void* dy, const void* dsum, const vo
     ASHB_REQUIRE(dy && s && weight && rstd && dx && workspace, "null buffer");
     ASHB_REQUIRE(workspace_bytes >= ashb_rms_norm_workspace(rows, width) && aligned(4, {workspace}), "small workspace");
     ASHB_REQUIRE(aligned(value_bytes(dtype), {dy, dsum, s, weight, dx, dweight}), "buffers not aligned to their type");
-    const NormGradArgs a{dy, dsum, s, weight, rstd, dx, static_cast<float*>(workspace), rows, width};
+    int64_t period = 8;      // of rows that begin alike, whatever the type: eight values are a multiple of 16 bytes
+    while (period > 1 && width * (period / 2) % 8 == 0) period /= 2;
+    const NormGradArgs a{dy, dsum, s, weight, rstd, dx, static_cast<float*>(workspace), rows, width, period};
     const unsigned grid = backward_ctas(rows, width);
     if (dtype == ASHB_F32) backward_typed<float>(a, grid, dweight, st);
     else if (dtype == ASHB_F16) backward_typed<__half>(a, grid, dweight, st);
