@@ -814,14 +814,19 @@ int ashb_rms_norm_backward(int dtype, const void* dy_dev, const void* dsum_dev, 
 int ashb_linear_forward(int type, const void* x_dev, int64_t x_stride, const float* x_scales_dev, const void* weight_dev,
                         int64_t weight_stride, const float* weight_scales_dev, const void* bias_dev, const void* residual_dev,
                         int64_t residual_stride, int64_t rows, int64_t inputs, int64_t outputs, int activation, float omega,
-                        int out_type, void* y_dev, void* slope_dev, void* stream);
+                        int out_type, void* y_dev, void* slope_dev, void* workspace_dev, int64_t workspace_bytes, void* stream);
+/* Bytes of device scratch (256-byte aligned) that the call takes: 0 where rows of x and weight begin at multiples of 16
+ * bytes (or there are no more than four rows of x). */
+int64_t ashb_linear_forward_workspace(int type, const void* x_dev, int64_t x_stride, const void* weight_dev,
+                                      int64_t weight_stride, int64_t rows, int64_t inputs, int64_t outputs);
 
 /* Gradients of the same from dy [rows][outputs] (contiguous): dx [rows][inputs], dweight [outputs][inputs] and dbias
  * [outputs], each NULL where not wanted (the residual's is dy).  slope_kind 0: no activation, slope NULL; 1: slope holds
  * act'(z); 2: relu without a residual, slope is the output y.  Sums run in a fixed order.  _workspace: bytes of device
  * scratch (256-byte aligned). */
-int64_t ashb_linear_workspace(int type, int64_t rows, int64_t inputs, int64_t outputs, int slope_kind, int want_dweight,
-                              int want_dbias);
+int64_t ashb_linear_backward_workspace(int type, const void* dy_dev, const void* x_dev, int64_t x_stride, const void* weight_dev,
+                                       int64_t weight_stride, int64_t rows, int64_t inputs, int64_t outputs, int slope_kind,
+                                       int want_dx, int want_dweight, int want_dbias);
 int ashb_linear_backward(int type, const void* dy_dev, const void* slope_dev, int slope_kind, const void* x_dev,
                          int64_t x_stride, const void* weight_dev, int64_t weight_stride, int64_t rows, int64_t inputs,
                          int64_t outputs, void* dx_dev, void* dweight_dev, void* dbias_dev, void* workspace_dev,

@@ -118,7 +118,7 @@ def test_library_refuses_cpu_tensors_and_bad_arguments():
             call()
     lib, p = shim._lib, ctypes.c_void_p(4096)
     f = lambda *a: lib.ashb_linear_forward(*a)
-    good = [0, p, 8, None, p, 8, None, None, None, 0, 3, 8, 5, 0, 1.0, 0, p, None, None]
+    good = [0, p, 8, None, p, 8, None, None, None, 0, 3, 8, 5, 0, 1.0, 0, p, None, None, 0, None]
     for at, value in [(0, 1), (0, 9), (2, 7), (5, 7), (10, -1), (11, 0), (12, 0), (13, 5), (15, 3), (16, None), (1, None), (17, p)]:
         args = list(good)
         args[at] = value
@@ -128,6 +128,10 @@ def test_library_refuses_cpu_tensors_and_bad_arguments():
     args = list(good)
     args[0] = 8                  # e4m3 without scales
     assert f(*args) == 1
+    args = list(good)
+    args[2], args[10] = 9, 100   # rows that are no whole words, and no workspace for their copy
+    assert f(*args) == 1 and lib.ashb_linear_forward_workspace(0, p, 9, p, 8, 100, 8, 5) == 3328      # 100 rows of 32 bytes
+    assert lib.ashb_linear_forward_workspace(0, p, 8, p, 8, 100, 8, 5) == 0 == lib.ashb_linear_forward_workspace(0, p, 9, p, 8, 4, 8, 5)
     assert lib.ashb_linear_backward(0, p, None, 1, p, 8, p, 8, 3, 8, 5, p, p, p, None, 0, None) == 1
     assert lib.ashb_linear_backward(0, p, p, 1, p, 8, p, 8, 3, 8, 5, p, p, p, p, 8, None) == 1       # small workspace
     assert lib.ashb_rms_norm_forward(0, p, 4, None, 0, p, 3, 8, 1e-6, p, None, None, None, None, None) == 1

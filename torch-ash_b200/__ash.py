@@ -140,9 +140,11 @@ _lib.ashb_rms_norm_workspace.argtypes = [_i64, _i64]
 _lib.ashb_rms_norm_workspace.restype = _i64
 _lib.ashb_rms_norm_backward.argtypes = [_int] + [_vp] * 5 + [_i64, _i64, _vp, _vp, _vp, _i64, _vp]
 _lib.ashb_linear_forward.argtypes = [_int, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _int, _f32, _int,
-                                     _vp, _vp, _vp]
-_lib.ashb_linear_workspace.argtypes = [_int, _i64, _i64, _i64, _int, _int, _int]
-_lib.ashb_linear_workspace.restype = _i64
+                                     _vp, _vp, _vp, _i64, _vp]
+_lib.ashb_linear_forward_workspace.argtypes = [_int, _vp, _i64, _vp, _i64, _i64, _i64, _i64]
+_lib.ashb_linear_forward_workspace.restype = _i64
+_lib.ashb_linear_backward_workspace.argtypes = [_int, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _int, _int, _int, _int]
+_lib.ashb_linear_backward_workspace.restype = _i64
 _lib.ashb_linear_backward.argtypes = [_int, _vp, _vp, _int, _vp, _i64, _vp, _i64, _i64, _i64, _i64] + [_vp] * 4 + [_i64, _vp]
 _lib.ashb_layer_timeouts.argtypes = [_vp]
 _lib.ashb_grid_zero_rows.argtypes = [_vp, _int, _vp, _vp, _c.c_double, _vp, _int, _vp, _vp, _i64, _i64, _i64, _vp]
@@ -1711,15 +1713,20 @@ def linear_forward(x, weight, bias, activation: str, residual, omega: float, wit
     if residual is not None:
         residual, residual_stride = _rows_of(residual, "residual")
     x_scales, w_scales = (None, None) if scales is None else (_cuda(scales[0], "x.scales"), _cuda(scales[1], "weight.scales"))
-    y = torch.empty((rows, outputs), dtype=out_dtype, device=x.device)
+    kind = _VALUE_TYPES[x.dtype] if scales is None else _E4M3_ROWS
+    y = x.new_empty((rows, outputs), dtype=out_dtype)
     slope = torch.empty_like(y) if with_slope else None
     if rows:
+        at, w_at, size = x.data_ptr(), weight.data_ptr(), x.element_size()
+        workspace, nbytes = None, 0
+        if (at | w_at | x_stride * size | weight_stride * size) & 15:
+            nbytes = _lib.ashb_linear_forward_workspace(kind, at, x_stride, w_at, weight_stride, rows, inputs, outputs)
+            workspace = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         with _on(x.device):
             _check(_lib.ashb_linear_forward(
-                _E4M3_ROWS if scales is not None else _VALUE_TYPES[x.dtype], x.data_ptr(), x_stride, _ptr(x_scales),
-                weight.data_ptr(), weight_stride, _ptr(w_scales), _ptr(bias), _ptr(residual), residual_stride, rows, inputs,
-                outputs, _ACTIVATIONS[activation], omega, _VALUE_TYPES[out_dtype], y.data_ptr(), _ptr(slope),
-                _stream(x.device)))
+                kind, at, x_stride, _ptr(x_scales), w_at, weight_stride, _ptr(w_scales), _ptr(bias), _ptr(residual),
+                residual_stride, rows, inputs, outputs, _ACTIVATIONS[activation], omega, _VALUE_TYPES[out_dtype], y.data_ptr(),
+                _ptr(slope), _ptr(workspace), nbytes, _stream(x.device)))
     return y, slope
 
 
@@ -1730,13 +1737,15 @@ def linear_backward(dy, slope, slope_kind: int, x, weight, want_dx: bool, want_d
     weight, weight_stride = _rows_of(weight, "weight")
     rows, inputs = x.shape
     outputs = weight.shape[0]
-    empty = lambda *shape: torch.empty(shape, dtype=dy.dtype, device=dy.device)
+    empty = lambda *shape: dy.new_empty(shape)
     dx = empty(rows, inputs) if want_dx else None
     dw = empty(outputs, inputs) if want_dweight else None
     db = empty(outputs) if want_dbias else None
     kind = _VALUE_TYPES[dy.dtype]
     with _on(dy.device):
-        nbytes = _lib.ashb_linear_workspace(kind, rows, inputs, outputs, slope_kind, int(want_dweight), int(want_dbias))
+        nbytes = _lib.ashb_linear_backward_workspace(kind, dy.data_ptr(), x.data_ptr(), x_stride, weight.data_ptr(), weight_stride,
+                                                     rows, inputs, outputs, slope_kind, int(want_dx), int(want_dweight),
+                                                     int(want_dbias))
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=dy.device) if nbytes else None
         _check(_lib.ashb_linear_backward(kind, dy.data_ptr(), _ptr(slope), slope_kind, x.data_ptr(), x_stride,
                                          weight.data_ptr(), weight_stride, rows, inputs, outputs, _ptr(dx), _ptr(dw), _ptr(db),

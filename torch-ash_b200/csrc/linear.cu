@@ -37,14 +37,9 @@ namespace ashb {
 
 constexpr int kRowBytes = 128;            // of a tile row: 64 values of 16 bits, 128 of 8
 constexpr int kTileM = 128;
-// Warps, 16 in all (128 registers): with loads of their own seven loaders, one that issues the products and eight that finish
-// tiles; with bulk copies one loader, one for the products, two that idle, and eight or twelve that finish.
-constexpr int kGemmThreads = 512, kLoaders = 7;
-template <bool BULK>
-constexpr int kProductWarp = BULK ? 1 : kLoaders;
-template <bool BULK>
-constexpr int kFirstFinisher = BULK ? 4 : 8;
-constexpr int kPhaseBlocks = 8;           // blocks of 64 between the float32 sums of split products
+// Warps, 16 in all (128 registers): one that issues copies, one that issues products, two that idle (of float32 products six
+// that split values into parts), and eight or twelve that finish tiles.
+constexpr int kGemmThreads = 512, kFirstFinisher = 4, kFirstSplitFinisher = 8;
 constexpr int kMaxStages = 8;
 constexpr int kMaxSlots = 8;              // tiles whose sums are in tensor memory
 constexpr size_t kSharedLimit = 232448;
@@ -170,7 +165,6 @@ enum Kind { kHalf, kSplit, kEight };     // operands: 16 bits, float32 in three 
 struct Operand {
     const void* at;
     int64_t stride;      // values between rows
-    int wide;            // rows start and end at multiples of 16 bytes
 };
 
 struct Finish {          // what becomes of the sums
@@ -197,64 +191,17 @@ struct GemmArgs {
     int64_t finish_bytes;    // of shared memory, a finisher's
 };
 
-// Consecutive values of an operand that make one 16-byte word of each of its parts, at p; `left` of them exist, none if it is
-// not positive.  WIDE: all or none do, on 16-byte boundaries; the loads are predicated, so that nothing waits for them here.
-struct Eight32 { float v[8]; };
-struct Eight16 { uint4 w; };
-struct Sixteen8 { uint4 w; };
-
-template <bool WIDE>
-__device__ __forceinline__ void fetch_word(Eight32& e, const float* p, int left) {
-    if (WIDE) {
-        float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f), b = a;
-        if (left >= 4) a = __ldg(reinterpret_cast<const float4*>(p));
-        if (left >= 8) b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-        e.v[0] = a.x; e.v[1] = a.y; e.v[2] = a.z; e.v[3] = a.w;
-        e.v[4] = b.x; e.v[5] = b.y; e.v[6] = b.z; e.v[7] = b.w;
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) e.v[j] = j < left ? __ldg(p + j) : 0.0f;
-    }
-}
-template <bool WIDE>
-__device__ __forceinline__ void fetch_word(Eight16& e, const uint16_t* p, int left) {
-    e.w = make_uint4(0, 0, 0, 0);
-    if (WIDE) {
-        if (left >= 8) e.w = __ldg(reinterpret_cast<const uint4*>(p));
-    } else {
-        uint32_t h[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) h[j] = j < left ? (uint32_t)__ldg(p + j) : 0u;
-        e.w = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
-    }
-}
-template <bool WIDE>
-__device__ __forceinline__ void fetch_word(Sixteen8& e, const uint8_t* p, int left) {
-    e.w = make_uint4(0, 0, 0, 0);
-    if (WIDE) {
-        if (left >= 16) e.w = __ldg(reinterpret_cast<const uint4*>(p));
-    } else {
-        uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-            if (j < left) w[j / 4] |= (uint32_t)__ldg(p + j) << (8 * (j % 4));
-        e.w = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-}
-
 __device__ __forceinline__ void put16(uint32_t at, uint4 w) {
     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
 }
-__device__ __forceinline__ void put8(uint32_t at, uint32_t, const Eight16& e) { put16(at, e.w); }
-__device__ __forceinline__ void put8(uint32_t at, uint32_t, const Sixteen8& e) { put16(at, e.w); }
-// hi is truncated, so that the largest finite value stays finite; what follows is exact, v = hi + mid + lo.
-__device__ __forceinline__ void put8(uint32_t at, uint32_t part, const Eight32& e) {
+// Eight float32 values as a word of each of their three parts.  hi is truncated, so that the largest finite value stays finite; what follows is exact, v = hi + mid + lo.
+__device__ __forceinline__ void put_parts(uint32_t at, uint32_t part, const float (&v)[8]) {
     uint32_t h[4], m[4], l[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const uint32_t a = __float_as_uint(e.v[2 * j]), b = __float_as_uint(e.v[2 * j + 1]);
+        const uint32_t a = __float_as_uint(v[2 * j]), b = __float_as_uint(v[2 * j + 1]);
         h[j] = __byte_perm(a, b, 0x7632);
-        const float ra = e.v[2 * j] - __uint_as_float(a & 0xFFFF0000u), rb = e.v[2 * j + 1] - __uint_as_float(b & 0xFFFF0000u);
+        const float ra = v[2 * j] - __uint_as_float(a & 0xFFFF0000u), rb = v[2 * j + 1] - __uint_as_float(b & 0xFFFF0000u);
         asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(m[j]) : "f"(rb), "f"(ra));
         const float la = ra - __uint_as_float(m[j] << 16), lb = rb - __uint_as_float(m[j] & 0xFFFF0000u);
         asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(l[j]) : "f"(lb), "f"(la));
@@ -265,67 +212,13 @@ __device__ __forceinline__ void put8(uint32_t at, uint32_t part, const Eight32& 
 }
 
 template <int KIND>
-struct KindOf { using Chunk = Eight16; };
-template <>
-struct KindOf<kSplit> { using Chunk = Eight32; };
-template <>
-struct KindOf<kEight> { using Chunk = Sixteen8; };
+constexpr int kBlockK = KIND == kEight ? 128 : KIND == kHalf ? 64 : 32;       // values of a stage along k
 
-template <int KIND>
-constexpr int kBlockK = KIND == kEight ? 128 : 64;       // values of a stage along k
-template <int KIND>
-constexpr int kParts = KIND == kSplit ? 3 : 1;
-
-// Bytes of one part of an operand's tile: `extent` values across, a stage's values along k.
+// Bytes of a 16- or 8-bit operand's tile: `extent` values across, a stage's values along k.
 template <bool DOWN>
 __host__ __device__ constexpr uint32_t part_bytes(int extent) {
     return DOWN ? (uint32_t)((extent + 63) / 64) * 64u * kRowBytes : (uint32_t)extent * kRowBytes;
 }
-
-// A stage's tile of an operand by loads of the loader warps' own: CHUNKS words a thread.
-// Word `i` of a tile: along rows, row i / 8 and word i % 8; down rows, word i % 8 of row (i / 8) % 64 of box i / 512.
-template <int KIND, bool DOWN, int CHUNKS>
-struct TileFetch {
-    using Chunk = typename KindOf<KIND>::Chunk;
-    using Value = std::conditional_t<KIND == kSplit, float, std::conditional_t<KIND == kEight, uint8_t, uint16_t>>;
-    static constexpr int kValues = KIND == kEight ? 16 : 8;
-    Chunk c[CHUNKS];
-
-    // across0, k0: first value across and along k; words: 16-byte words along k that the products will read (of 8).
-    __device__ __forceinline__ void fetch(const Operand& o, int thread, int total, int64_t across0, int64_t across, int64_t k0,
-                                          int64_t k, int words) {
-        if (o.wide) fetch_as<true>(o, thread, total, across0, across, k0, k, words);
-        else fetch_as<false>(o, thread, total, across0, across, k0, k, words);
-    }
-    template <bool WIDE>
-    __device__ __forceinline__ void fetch_as(const Operand& o, int thread, int total, int64_t across0, int64_t across,
-                                             int64_t k0, int64_t k, int words) {
-        const Value* tile = static_cast<const Value*>(o.at) + (DOWN ? k0 * o.stride + across0 : across0 * o.stride + k0);
-        const int across_left = (int)min(across - across0, (int64_t)1024), k_left = (int)min(k - k0, (int64_t)1024);
-#pragma unroll
-        for (int j = 0; j < CHUNKS; ++j) {
-            const int i = thread + j * kLoaders * 32;
-            if (DOWN) {
-                const int r = (i >> 3) & 63, col = (i >> 9) * 64 + (i & 7) * 8;
-                fetch_word<WIDE>(c[j], tile + r * o.stride + col, i < total && r < k_left ? across_left - col : 0);
-            } else {
-                const int r = i >> 3, col = (i & 7) * kValues;
-                fetch_word<WIDE>(c[j], tile + r * o.stride + col,
-                                 i < total && (i & 7) < words && r < across_left ? k_left - col : 0);
-            }
-        }
-    }
-    __device__ __forceinline__ void put(uint32_t tile, uint32_t part, int thread, int total, int words) {
-#pragma unroll
-        for (int j = 0; j < CHUNKS; ++j) {
-            const int i = thread + j * kLoaders * 32;
-            if (i >= total) break;
-            const int r = i >> 3;             // tile rows of a box follow one another: 64 of 128 bytes
-            const int w = (i & 7) ^ (r & 7);
-            if (DOWN ? (r & 63) < words * 8 : (i & 7) < words) put8(tile + (uint32_t)r * kRowBytes + (uint32_t)w * 16, part, c[j]);
-        }
-    }
-};
 
 // Order of the tiles: bands of 8 rows of tiles, down the band first, so that the tiles in flight share operands in L2.
 // In 32 bits throughout: with 64-bit quotients per stage and tile the threads that issue copies and products spent more time
@@ -505,9 +398,12 @@ __device__ __forceinline__ void finish_narrow(const Finish& f, const float* bloc
         activate<ACT, SLOPE, kRounded>(f.omega, z, d);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            if (first + i >= left) break;
-            if (SLOPE) slopes[(first + i) * n] = from_float<T>(d[i]);
-            out[(first + i) * n] = from_float<T>(z[i] + r[i]);
+            if (first + i < left) {
+                if (SLOPE) *slopes = from_float<T>(d[i]);
+                *out = from_float<T>(z[i] + r[i]);
+            }
+            out += n;
+            if (SLOPE) slopes += n;
         }
     }
 }
@@ -865,21 +761,19 @@ struct GemmShared {
     int gave_up;
 };
 
-// Barriers: full[s] by the loaders (the copies' bytes, or a count of their threads), empty[s] by the products that read
-// stage s, sums_full / sums_empty of the tiles in tensor memory.  Every role walks the same items, blocks and phases.
-// STAYS (loaders with loads of their own): B is loaded once; the registers that held it hold a second tile of A under way.
-template <int KIND, bool BULK, bool A_DOWN, bool B_DOWN, bool STAYS>
+// Barriers: full[s] by the copies' bytes, empty[s] by the products that read stage s, sums_full / sums_empty of the tiles in
+// tensor memory.  Every role walks the same items and blocks.
+template <int KIND, bool A_DOWN, bool B_DOWN>
 __global__ void __launch_bounds__(kGemmThreads, 1) layer_gemm_kernel(const GemmArgs g, const __grid_constant__ CUtensorMap map_a,
                                                                      const __grid_constant__ CUtensorMap map_b,
                                                                      const __grid_constant__ FinishMaps maps) {
     extern __shared__ __align__(1024) uint8_t dynamic[];
     __shared__ GemmShared sh;
-    constexpr int kBlock = kBlockK<KIND>, kPartsOf = kParts<KIND>, kStep = KIND == kEight ? 32 : 16;
+    constexpr int kBlock = kBlockK<KIND>, kStep = KIND == kEight ? 32 : 16;
     constexpr bool kForward = !A_DOWN && !B_DOWN;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t base = (smem_of(dynamic) + 1023u) & ~1023u;
-    const uint32_t a_part = part_bytes<A_DOWN>(kTileM), b_part = part_bytes<B_DOWN>(g.bn);
-    const uint32_t a_bytes = a_part * kPartsOf, stage_bytes = a_bytes + b_part * kPartsOf;
+    const uint32_t a_bytes = part_bytes<A_DOWN>(kTileM), b_bytes = part_bytes<B_DOWN>(g.bn), stage_bytes = a_bytes + b_bytes;
     float* blocks = reinterpret_cast<float*>(dynamic + (base - smem_of(dynamic)) + (size_t)stage_bytes * g.stages);
     volatile int* gave_up = &sh.gave_up;
     const uint32_t full = smem_of(sh.full), empty = smem_of(sh.empty);
@@ -888,215 +782,117 @@ __global__ void __launch_bounds__(kGemmThreads, 1) layer_gemm_kernel(const GemmA
     if (threadIdx.x == 0) {
         sh.gave_up = 0;
         for (int s = 0; s < g.stages; ++s) {
-            bar_init(full + 8 * s, BULK ? 1 : kLoaders * 32);
+            bar_init(full + 8 * s, 1);
             bar_init(empty + 8 * s, 1);
         }
         for (int h = 0; h < g.slots; ++h) {
             bar_init(sums_full + 8 * h, 1);
-            bar_init(sums_empty + 8 * h, KIND == kSplit && !g.bulk_out ? 8 : 4 * ((g.bn + 31) >> 5));
+            bar_init(sums_empty + 8 * h, 4 * ((g.bn + 31) >> 5));
         }
         for (int i = 0; i < 24; ++i) bar_init(smem_of(sh.residual) + 8 * i, 1);
         bar_init(smem_of(&sh.drained), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == kProductWarp<BULK>) tmem_alloc(smem_of(&sh.tmem), (uint32_t)g.columns);
+    if (warp == 1) tmem_alloc(smem_of(&sh.tmem), (uint32_t)g.columns);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
-    const uint32_t slot_columns = (uint32_t)g.bn * (KIND == kSplit ? 2u : 1u);
 
-    if (warp < (BULK ? 1 : kLoaders)) {
-        if constexpr (BULK) {
-            if (threadIdx.x == 0) {
-                Turn turn;
-                int fills = 0;      // up to the number of stages
-                bool ok = true;
-                for (uint32_t item = blockIdx.x; item < g.items && ok; item += gridDim.x) {
-                    const Tile t = tile_of(g, item);
-                    int k = (int)t.k0;
-                    for (int b = 0; b < t.blocks; ++b, k += kBlock, turn.next(g.stages)) {
-                        if (!(ok = bar_wait(empty + 8 * turn.at, turn.parity ^ 1u, gave_up))) break;
-                        const bool with_b = !g.b_stays || fills < g.stages;
-                        if (fills < g.stages) ++fills;
-                        const uint32_t tile_a = base + (uint32_t)turn.at * stage_bytes, tile_b = tile_a + a_bytes;
-                        const uint32_t bar = full + 8 * turn.at;
-                        bar_expect(bar, a_part + (with_b ? b_part : 0u));
-                        if constexpr (A_DOWN) {
-                            for (int box = 0; box < kTileM / 64; ++box)
-                                tma_load_2d(tile_a + box * 64 * kRowBytes, &map_a, t.m * kTileM + box * 64, k, bar);
-                        } else {
-                            tma_load_2d(tile_a, &map_a, k, t.m * kTileM, bar);
-                        }
-                        if (with_b) {
-                            if constexpr (B_DOWN) {
-                                for (int box = 0; box * 64 < g.bn; ++box)
-                                    tma_load_2d(tile_b + box * 64 * kRowBytes, &map_b, t.n * g.bn + box * 64, k, bar);
-                            } else {
-                                tma_load_2d(tile_b, &map_b, k, t.n * g.bn, bar);
-                            }
-                        }
-                    }
-                }
-                if (!ok) {      // the copies still under way end before the CTA does
-                    for (int i = 0; i < fills; ++i) {
-                        if (turn.at == 0) turn.parity ^= 1u;
-                        turn.at = (turn.at == 0 ? g.stages : turn.at) - 1;
-                        bar_drain(full + 8 * turn.at, turn.parity);
-                    }
-                }
-            }
-        } else {
-            // words along k that the products of a stage read, of 8
-            constexpr int kStepWords = 2;
-            const auto words_of = [&](int64_t k) {
-                return (int)((min((int64_t)kBlock, g.k - k) + kStep - 1) / kStep) * kStepWords;
-            };
-            constexpr int kB = KIND == kSplit ? 5 : 10;      // 224 threads, 1024 words of A and of B (16 and 8 bits: 2048)
-            const int b_words = (int)(b_part / 16);
+    if (warp == 0) {
+        if (lane == 0) {
             Turn turn;
-            bool ok = true;
-            if constexpr (STAYS) {
-                TileFetch<KIND, A_DOWN, 5> fa[2];
-                {
-                    TileFetch<KIND, B_DOWN, kB> fb;      // a stage's block of k is the same in every round
-                    for (int s = 0; s < g.stages; ++s) {
-                        const int64_t k = (int64_t)(s % (int)g.blocks_k) * kBlock;
-                        fb.fetch(g.b, threadIdx.x, b_words, 0, g.n, k, g.k, words_of(k));
-                        fb.put(base + (uint32_t)s * stage_bytes + a_bytes, b_part, threadIdx.x, b_words, words_of(k));
-                    }
-                }
-                // tiles and blocks in one sequence: `next` is fetched one ahead
-                uint32_t item = blockIdx.x, next_item = blockIdx.x;
-                int b = 0, next_b = 0;
-                const auto fetch = [&](TileFetch<KIND, A_DOWN, 5>& f) {
-                    if (next_item >= g.items) return;
-                    const int64_t k = (int64_t)next_b * kBlock;
-                    f.fetch(g.a, threadIdx.x, 1024, (int64_t)next_item * kTileM, g.m, k, g.k, words_of(k));
-                    if (++next_b == (int)g.blocks_k) {
-                        next_b = 0;
-                        next_item += gridDim.x;
-                    }
-                };
-                const auto put = [&](TileFetch<KIND, A_DOWN, 5>& f) {
-                    if (!(ok = bar_wait(empty + 8 * turn.at, turn.parity ^ 1u, gave_up))) return;
-                    f.put(base + (uint32_t)turn.at * stage_bytes, a_part, threadIdx.x, 1024, words_of((int64_t)b * kBlock));
-                    fence_async_shared();
-                    bar_arrive(full + 8 * turn.at);
-                    turn.next(g.stages);
-                    if (++b == (int)g.blocks_k) {
-                        b = 0;
-                        item += gridDim.x;
-                    }
-                };
-                fetch(fa[0]);
-                while (item < g.items && ok) {
-                    fetch(fa[1]);
-                    put(fa[0]);
-                    if (item >= g.items || !ok) break;
-                    fetch(fa[0]);
-                    put(fa[1]);
-                }
-            } else {
-                for (uint32_t item = blockIdx.x; item < g.items && ok; item += gridDim.x) {
-                    const Tile t = tile_of(g, item);
-                    int64_t k = t.k0;
-                    for (int b = 0; b < t.blocks; ++b, k += kBlock, turn.next(g.stages)) {
-                        const uint32_t tile_a = base + (uint32_t)turn.at * stage_bytes, tile_b = tile_a + a_bytes;
-                        const int words = words_of(k);
-                        TileFetch<KIND, A_DOWN, 5> fa;
-                        TileFetch<KIND, B_DOWN, kB> fb;
-                        fa.fetch(g.a, threadIdx.x, 1024, (int64_t)t.m * kTileM, g.m, k, g.k, words);
-                        fb.fetch(g.b, threadIdx.x, b_words, (int64_t)t.n * g.bn, g.n, k, g.k, words);
-                        if (!(ok = bar_wait(empty + 8 * turn.at, turn.parity ^ 1u, gave_up))) break;
-                        fa.put(tile_a, a_part, threadIdx.x, 1024, words);
-                        fb.put(tile_b, b_part, threadIdx.x, b_words, words);
-                        fence_async_shared();
-                        bar_arrive(full + 8 * turn.at);
-                    }
-                }
-            }
-        }
-    } else if (warp == kProductWarp<BULK>) {
-        {
-            const uint32_t mine = elected();
-            Turn turn, slot;
+            int fills = 0;      // up to the number of stages
             bool ok = true;
             for (uint32_t item = blockIdx.x; item < g.items && ok; item += gridDim.x) {
                 const Tile t = tile_of(g, item);
-                int left = (int)min((int64_t)t.blocks * kBlock, g.k - t.k0);      // values along k
-                for (int b0 = 0; b0 < t.blocks && ok; slot.next(g.slots)) {
-                    const int b1 = KIND == kSplit ? min(t.blocks, b0 + kPhaseBlocks) : t.blocks;
-                    const uint32_t sums = tmem + (uint32_t)slot.at * slot_columns;
-                    if (!(ok = bar_wait(sums_empty + 8 * slot.at, slot.parity ^ 1u, gave_up))) break;
-                    tc_fence_after();
-                    bool add = false;
-                    for (; b0 < b1; ++b0, left -= kBlock, turn.next(g.stages)) {
-                        if (!(ok = bar_wait(full + 8 * turn.at, turn.parity, gave_up))) break;
-                        tc_fence_after();
-                        const int steps = (min(kBlock, left) + kStep - 1) / kStep;
-                        const uint32_t tile_a = base + (uint32_t)turn.at * stage_bytes;
-                        // a step along k: 32 bytes along rows, 16 rows down them
-                        constexpr uint64_t a_step = (A_DOWN ? 16 * kRowBytes : 32) >> 4, b_step = (B_DOWN ? 16 * kRowBytes : 32) >> 4;
-                        uint64_t a = tile_desc(tile_a, 64 * kRowBytes), b = tile_desc(tile_a + a_bytes, 64 * kRowBytes);
-                        if constexpr (KIND == kSplit) {
-                            const uint64_t ap = a_part >> 4, bp = b_part >> 4;
-                            const uint32_t small = sums + (uint32_t)g.bn;
-                            for (int i = 0; i < steps; ++i, a += a_step, b += b_step) {
-                                product<false>(mine, sums, a, b, g.desc, add);
-                                product<false>(mine, small, a + 2 * ap, b, g.desc, add);
-                                product<false>(mine, small, a, b + 2 * bp, g.desc, true);
-                                product<false>(mine, small, a + ap, b + bp, g.desc, true);
-                                product<false>(mine, small, a + ap, b, g.desc, true);
-                                product<false>(mine, small, a, b + bp, g.desc, true);
-                                add = true;
-                            }
-                        } else {
-                            for (int i = 0; i < steps; ++i, a += a_step, b += b_step) {
-                                product<KIND == kEight>(mine, sums, a, b, g.desc, add);
-                                add = true;
-                            }
-                        }
-                        products_done(mine, empty + 8 * turn.at);
+                int k = (int)t.k0;
+                for (int b = 0; b < t.blocks; ++b, k += kBlock, turn.next(g.stages)) {
+                    if (!(ok = bar_wait(empty + 8 * turn.at, turn.parity ^ 1u, gave_up))) break;
+                    const bool with_b = !g.b_stays || fills < g.stages;
+                    if (fills < g.stages) ++fills;
+                    const uint32_t tile_a = base + (uint32_t)turn.at * stage_bytes, tile_b = tile_a + a_bytes;
+                    const uint32_t bar = full + 8 * turn.at;
+                    bar_expect(bar, a_bytes + (with_b ? b_bytes : 0u));
+                    if constexpr (A_DOWN) {
+                        for (int box = 0; box < kTileM / 64; ++box)
+                            tma_load_2d(tile_a + box * 64 * kRowBytes, &map_a, t.m * kTileM + box * 64, k, bar);
+                    } else {
+                        tma_load_2d(tile_a, &map_a, k, t.m * kTileM, bar);
                     }
-                    if (ok) products_done(mine, sums_full + 8 * slot.at);
+                    if (with_b) {
+                        if constexpr (B_DOWN) {
+                            for (int box = 0; box * 64 < g.bn; ++box)
+                                tma_load_2d(tile_b + box * 64 * kRowBytes, &map_b, t.n * g.bn + box * 64, k, bar);
+                        } else {
+                            tma_load_2d(tile_b, &map_b, k, t.n * g.bn, bar);
+                        }
+                    }
                 }
             }
-            if (!ok) {      // tensor memory is not given back under products still running
-                products_done(mine, smem_of(&sh.drained));
-                bar_drain(smem_of(&sh.drained), 0);
-                if (mine) atomicAdd(&g_layer_timeouts, 1u);
+            if (!ok) {      // the copies still under way end before the CTA does
+                for (int i = 0; i < fills; ++i) {
+                    if (turn.at == 0) turn.parity ^= 1u;
+                    turn.at = (turn.at == 0 ? g.stages : turn.at) - 1;
+                    bar_drain(full + 8 * turn.at, turn.parity);
+                }
             }
         }
-    } else if (warp >= kFirstFinisher<BULK> && warp < kFirstFinisher<BULK> + 4 * g.groups) {
-        // lanes of tensor memory that the warp may read, and its group: the blocks of 32 columns go to the groups in turn
-        const int quarter = warp & 3, which = (warp - kFirstFinisher<BULK>) >> 2;
-        if (g.bulk_out) {
-            const int number = warp - kFirstFinisher<BULK>;
-            finish_bulk<KIND, kForward>(g, maps, number, lane, tmem, slot_columns, sums_full, sums_empty,
-                                        smem_of(blocks) + (uint32_t)(number * g.finish_bytes), smem_of(sh.residual) + 16 * number, gave_up);
-        }
-        float* block = blocks + (size_t)(warp - kFirstFinisher<BULK>) * 32 * 32 * g.places;
-        const int n_blocks = (g.bn + 31) >> 5;
-        Turn slot;
-        typename AheadOf<KIND>::type ahead;
-        int blk = which;
-        for (uint32_t item = blockIdx.x; item < g.items && !g.bulk_out; item += gridDim.x) {
+    } else if (warp == 1) {
+        const uint32_t mine = elected();
+        Turn turn, slot;
+        bool ok = true;
+        for (uint32_t item = blockIdx.x; item < g.items && ok; item += gridDim.x, slot.next(g.slots)) {
             const Tile t = tile_of(g, item);
-            const int64_t row0 = (int64_t)t.m * kTileM + quarter * 32, col0 = (int64_t)t.n * g.bn;
+            int left = (int)min((int64_t)t.blocks * kBlock, g.k - t.k0);      // values along k
+            const uint32_t sums = tmem + (uint32_t)(slot.at * g.bn);
+            if (!(ok = bar_wait(sums_empty + 8 * slot.at, slot.parity ^ 1u, gave_up))) break;
+            tc_fence_after();
+            bool add = false;
+            for (int b = 0; b < t.blocks; ++b, left -= kBlock, turn.next(g.stages)) {
+                if (!(ok = bar_wait(full + 8 * turn.at, turn.parity, gave_up))) break;
+                tc_fence_after();
+                const int steps = (min(kBlock, left) + kStep - 1) / kStep;
+                const uint32_t tile_a = base + (uint32_t)turn.at * stage_bytes;
+                // a step along k: 32 bytes along rows, 16 rows down them
+                constexpr uint64_t a_step = (A_DOWN ? 16 * kRowBytes : 32) >> 4, b_step = (B_DOWN ? 16 * kRowBytes : 32) >> 4;
+                uint64_t at = tile_desc(tile_a, 64 * kRowBytes), bt = tile_desc(tile_a + a_bytes, 64 * kRowBytes);
+                for (int i = 0; i < steps; ++i, at += a_step, bt += b_step) {
+                    product<KIND == kEight>(mine, sums, at, bt, g.desc, add);
+                    add = true;
+                }
+                products_done(mine, empty + 8 * turn.at);
+            }
+            if (ok) products_done(mine, sums_full + 8 * slot.at);
+        }
+        if (!ok) {      // tensor memory is not given back under products still running
+            products_done(mine, smem_of(&sh.drained));
+            bar_drain(smem_of(&sh.drained), 0);
+            if (mine) atomicAdd(&g_layer_timeouts, 1u);
+        }
+    } else if (warp >= kFirstFinisher && warp < kFirstFinisher + 4 * g.groups) {
+        const int number = warp - kFirstFinisher;
+        if (g.bulk_out) {
+            finish_bulk<KIND, kForward>(g, maps, number, lane, tmem, (uint32_t)g.bn, sums_full, sums_empty,
+                                        smem_of(blocks) + (uint32_t)(number * g.finish_bytes), smem_of(sh.residual) + 16 * number, gave_up);
+        } else {
+            // lanes of tensor memory that the warp may read; the blocks of 32 columns go to the groups in turn
+            const int quarter = warp & 3, n_blocks = (g.bn + 31) >> 5;
+            float* block = blocks + (size_t)number * 1024;
+            Turn slot;
+            Ahead<__nv_bfloat16> ahead;
+            int blk = number >> 2;
             bool ok = true;
-            if constexpr (KIND == kSplit) {
-                if (!finish_split<kForward>(g, t, kPhaseBlocks, slot, tmem, sums_full, sums_empty, gave_up, block, quarter, which,
-                                            lane))
-                    break;
-            } else {
-                for (; blk < n_blocks && ok; blk += g.groups) {
+            for (uint32_t item = blockIdx.x; item < g.items && ok; item += gridDim.x, blk -= n_blocks, slot.next(g.slots)) {
+                const Tile t = tile_of(g, item);
+                const int64_t row0 = (int64_t)t.m * kTileM + quarter * 32, col0 = (int64_t)t.n * g.bn;
+                for (; blk < n_blocks; blk += g.groups) {
                     if (kForward) ahead.fetch(g.f, lane, row0, col0 + blk * 32, g.m, g.n);
                     ok = __all_sync(0xffffffffu, bar_wait(sums_full + 8 * slot.at, slot.parity, gave_up));
                     if (!ok) break;
                     tc_fence_after();
                     float r[32];
-                    tmem_load32(tmem + (uint32_t)slot.at * slot_columns + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(blk * 32), r);
+                    tmem_load32(tmem + (uint32_t)(slot.at * g.bn) + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(blk * 32), r);
                     put_block(block, lane, r);
                     tc_fence_before();
                     __syncwarp();
@@ -1104,9 +900,6 @@ __global__ void __launch_bounds__(kGemmThreads, 1) layer_gemm_kernel(const GemmA
                     finish<KIND, kForward>(g, block, ahead, lane, row0, col0 + blk * 32, t.split);
                     __syncwarp();
                 }
-                if (!ok) break;
-                blk -= n_blocks;
-                slot.next(g.slots);
             }
         }
     }
@@ -1114,11 +907,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1) layer_gemm_kernel(const GemmA
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == kProductWarp<BULK>) tmem_free(tmem, (uint32_t)g.columns);
+    if (warp == 1) tmem_free(tmem, (uint32_t)g.columns);
 }
 
 // ---- split products from bulk copies ---------------------------------------------------------------------------------------
-// The product kernel of float32 operands whose rows are multiples of 16 bytes.  The copies bring values as they are into a ring
+// The product kernel of float32 operands.  The copies bring values as they are into a ring
 // of their own, 32 along k a stage, so that several tiles are under way without a register; six warps split them into the
 // parts' tiles by a short loop.  Splitting on the way from registers instead took 40 registers for a tile under way and a loop
 // so long that it and the finishers' did not fit the instruction cache together (1M rows 64 -> 64: 145 us, %(none)s this way).
@@ -1154,9 +947,7 @@ __device__ __forceinline__ void split_tile(uint32_t raw, uint32_t parts, int ext
         const int r = i >> 2, c = i & 3;
         const uint32_t row = raw + (uint32_t)r * 128u;      // rows of boxes follow one another too
         const float4 a = get16(row + (uint32_t)(((2 * c) ^ (r & 7)) << 4)), b = get16(row + (uint32_t)(((2 * c + 1) ^ (r & 7)) << 4));
-        Eight32 e;
-        e.v[0] = a.x; e.v[1] = a.y; e.v[2] = a.z; e.v[3] = a.w;
-        e.v[4] = b.x; e.v[5] = b.y; e.v[6] = b.z; e.v[7] = b.w;
+        const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
         uint32_t to;
         if (DOWN) {
             const int box = r >> 5, k = r & 31, word = (box & 1) * 4 + c;
@@ -1164,7 +955,7 @@ __device__ __forceinline__ void split_tile(uint32_t raw, uint32_t parts, int ext
         } else {
             to = parts + (uint32_t)r * 64u + (uint32_t)((c ^ ((r >> 1) & 3)) << 4);
         }
-        put8(to, part, e);
+        put_parts(to, part, v);
     }
 }
 
@@ -1331,7 +1122,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) split_gemm_kernel(const GemmA
             }
         }
     } else {
-        const int quarter = warp & 3, which = (warp - 8) >> 2;
+        const int quarter = warp & 3, which = (warp - kFirstSplitFinisher) >> 2;
         if (g.bulk_out)
             finish_bulk<kSplit, !A_DOWN && !B_DOWN>(g, maps, warp - 8, lane, tmem, 2u * g.bn, sums_full, sums_empty,
                                                     smem_of(blocks) + (uint32_t)((warp - 8) * g.finish_bytes),
@@ -1352,6 +1143,52 @@ __global__ void __launch_bounds__(kGemmThreads, 1) split_gemm_kernel(const GemmA
     if (warp == 1) tmem_free(tmem, (uint32_t)g.columns);
 }
 
+// ---- rows of whole words ------------------------------------------------------------------------------------------------
+// Operands whose rows do not begin at multiples of 16 bytes are copied to where they do: bulk copies take no others.  Two
+// operands a launch; a thread gathers a word.  Reading such rows by loads of the product kernel's own instead was slower at
+// every size (1M rows 63 -> 63 of bfloat16 162 us against %(pad)s; 500 rows 4001 -> 301 134 us, a round trip to memory for every
+// stage along k, against %(pad2)s).
+struct Padding {
+    const void* from;
+    void* to;
+    int64_t rows, cols, stride, words;      // words: of a row where it goes
+    int lanes;                              // of a row: the power of two that covers its words, 32 at most
+    uint32_t units;                         // of work of a CTA: `lanes` words of as many rows as it has lanes for, four times
+    unsigned blocks;
+};
+constexpr int kPadRows = 4;      // of a thread under way
+template <class V>
+__global__ void __launch_bounds__(256) pad_kernel(const Padding first, const Padding second) {
+    constexpr int kValues = 16 / sizeof(V);
+    const bool is_first = blockIdx.x < first.blocks;
+    const Padding& p = is_first ? first : second;
+    const int lanes = p.lanes, sub = threadIdx.x & (lanes - 1), groups = 256 / lanes;
+    // in turn: the next `lanes` words of the same rows, then the next rows
+    const uint32_t pieces = (uint32_t)((p.words + lanes - 1) / lanes);
+    for (uint32_t unit = is_first ? blockIdx.x : blockIdx.x - first.blocks; unit < p.units; unit += p.blocks) {
+        const uint32_t rows = unit / pieces;
+        const int64_t row0 = (int64_t)rows * groups * kPadRows + threadIdx.x / lanes;
+        const int64_t word = (int64_t)(unit - rows * pieces) * lanes + sub, col = word * kValues;
+        const int left = (int)max(min(p.cols - col, (int64_t)kValues), (int64_t)0);
+        uint4 w[kPadRows];
+#pragma unroll
+        for (int i = 0; i < kPadRows; ++i) {
+            const int64_t row = row0 + i * groups;
+            const V* from = static_cast<const V*>(p.from) + row * p.stride + col;
+            V v[kValues];
+#pragma unroll
+            for (int k = 0; k < kValues; ++k) v[k] = row < p.rows && k < left ? __ldg(from + k) : (V)0;
+            uint32_t u[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int k = 0; k < kValues; ++k) u[k * (int)sizeof(V) / 4] |= (uint32_t)v[k] << (8 * (k * (int)sizeof(V) % 4));
+            w[i] = make_uint4(u[0], u[1], u[2], u[3]);
+        }
+#pragma unroll
+        for (int i = 0; i < kPadRows; ++i)
+            if (row0 + i * groups < p.rows && word < p.words) static_cast<uint4*>(p.to)[(row0 + i * groups) * p.words + word] = w[i];
+    }
+}
+
 // ---- few rows ------------------------------------------------------------------------------------------------------
 // Up to kFewRows rows: the weights are all there is to read, so a warp takes one output at a time, 16 bytes a lane and
 // load, and keeps a float32 sum per row of x.  A 128-row tile would load as much and pad the rest; from five rows on the
@@ -1368,7 +1205,7 @@ struct E4M3 { uint8_t code; };
 __device__ __forceinline__ float to_float(E4M3 c) { return __half2float(__half(__nv_cvt_fp8_to_halfraw(c.code, __NV_E4M3))); }
 
 template <class T, class OUT, bool ROUNDED>
-__global__ void __launch_bounds__(256) few_rows_kernel(const GemmArgs g) {
+__global__ void __launch_bounds__(256) few_rows_kernel(const GemmArgs g, bool wide) {
     constexpr int kVec = 16 / sizeof(T);
     const int lane = threadIdx.x & 31;
     const T* x = static_cast<const T*>(g.a.at);
@@ -1376,7 +1213,7 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const GemmArgs g) {
     for (int64_t n = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); n < g.n; n += (int64_t)gridDim.x * 8) {
         const T* w = static_cast<const T*>(g.b.at) + n * g.b.stride;
         float sum[kFewRows] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (g.a.wide && g.b.wide) {
+        if (wide) {
 #pragma unroll 4
             for (int64_t k = lane * kVec; k < g.k; k += 32 * kVec) {
                 float wv[kVec];
@@ -1432,7 +1269,7 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const GemmArgs g) {
 template <class T, int VEC>
 __global__ void __launch_bounds__(256) slope_kernel(const T* __restrict__ dy, const T* __restrict__ slope, int kind,
                                                     int64_t rows, int64_t n, int lanes, T* __restrict__ dz,
-                                                    float* __restrict__ partial) {
+                                                    int64_t dz_stride, float* __restrict__ partial) {
     __shared__ float sums[256 * VEC];
     const int sub = threadIdx.x & (lanes - 1), group = threadIdx.x / lanes, groups = 256 / lanes;
     const int64_t col = ((int64_t)blockIdx.x * lanes + sub) * VEC;
@@ -1448,7 +1285,7 @@ __global__ void __launch_bounds__(256) slope_kernel(const T* __restrict__ dy, co
                 load_n<T, VEC>(slope + r * n + col, s);
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) g[j] = kind == 1 ? g[j] * s[j] : s[j] > 0.0f ? g[j] : 0.0f;
-                store_n<T, VEC>(dz + r * n + col, g);
+                if (dz != nullptr) store_n<T, VEC>(dz + r * dz_stride + col, g);
             }
 #pragma unroll
             for (int j = 0; j < VEC; ++j) total[j] += g[j];
@@ -1488,7 +1325,7 @@ static double cycles(int kind, int bn, int64_t blocks, int64_t items, int sms) {
 }
 
 static Plan plan_product(int kind, bool a_down, bool b_down, int64_t m, int64_t n, int64_t k, bool may_split) {
-    const int block = kind == kEight ? 128 : 64, parts = kind == kSplit ? 3 : 1, sms = sm_count();
+    const int block = kind == kEight ? 128 : 64, sms = sm_count();
     const int widest = kind == kSplit ? 128 : 256;
     Plan best{};
     double least = 0.0;
@@ -1518,16 +1355,18 @@ static Plan plan_product(int kind, bool a_down, bool b_down, int64_t m, int64_t 
             }
         }
     }
-    best.stage = (size_t)parts * ((a_down ? part_bytes<true>(kTileM) : part_bytes<false>(kTileM)) +
-                                  (b_down ? part_bytes<true>(best.bn) : part_bytes<false>(best.bn)));
+    best.stage = (a_down ? part_bytes<true>(kTileM) : part_bytes<false>(kTileM)) +
+                 (b_down ? part_bytes<true>(best.bn) : part_bytes<false>(best.bn));
     best.b_stays = !a_down && best.tiles_n == 1 && best.splits == 1;      // if the stages hold all of it
-    const int columns = best.bn * (kind == kSplit ? 2 : 1);
-    // as many tiles' sums as tensor memory holds: with two, a narrow tile waits for the round trip of one through the
-    // products, a barrier, the way out and a barrier back (1.5k cycles)
-    best.slots = std::min(kMaxSlots, 512 / columns);
-    best.columns = 32;
-    while (best.columns < columns * best.slots) best.columns <<= 1;
     return best;
+}
+
+// As many tiles' sums as tensor memory holds: with two, a narrow tile waits for the round trip of one through the products, a
+// barrier, the way out and a barrier back (1.5k cycles).
+static void plan_slots(Plan* p, int columns) {
+    p->slots = std::min(kMaxSlots, 512 / columns);
+    p->columns = 32;
+    while (p->columns < columns * p->slots) p->columns <<= 1;
 }
 
 // A finisher's shared memory: blocks that leave by bulk copies, and their columns' biases and scales, or a block (two, where
@@ -1536,15 +1375,14 @@ static size_t finisher_bytes(const Plan& p, int block, bool slope) {
     return p.bulk_out ? (size_t)(block * p.bufs * (slope ? 2 : 1) + 1024) : (size_t)4096 * p.places;
 }
 
-// Stages and finishers once it is known how operands are loaded and results stored.  block: bytes of one that leaves by bulk copies.
-static void plan_shared(Plan* p, int kind, bool bulk, int64_t blocks, int block, bool slope) {
+// Stages and finishers once it is known how results are stored.  block: bytes of one that leaves by bulk copies.
+static void plan_shared(Plan* p, int64_t blocks, int block, bool slope) {
     const size_t room = kSharedLimit - 2048;
-    const bool phases = kind == kSplit && ceil_div(p->split_blocks, kPhaseBlocks) > 1;
-    p->bulk_out = p->bulk_out && !phases;
-    p->places = phases && p->bn > 64 ? 2 : 1;
+    plan_slots(p, p->bn);
+    p->places = 1;
     // twelve finishers and two blocks each where that leaves four stages, or three where a tile has no more than two
     const size_t stages = (p->split_blocks <= 2 ? 3 : 4) * p->stage;
-    p->groups = bulk ? 3 : 2;
+    p->groups = 3;
     p->bufs = 2;
     const auto finish = [&] { return 4 * p->groups * finisher_bytes(*p, block, slope); };
     if (stages + finish() > room) p->groups = 2;
@@ -1560,6 +1398,7 @@ static void plan_shared(Plan* p, int kind, bool bulk, int64_t blocks, int block,
 // The same of split_gemm_kernel.  Blocks are half as long as the plan counts them.
 static void plan_split(Plan* p, bool a_down, bool b_down, int64_t k, bool slope) {
     const int64_t blocks = ceil_div(k, kSplitBlock);
+    plan_slots(p, 2 * p->bn);
     p->split_blocks *= 2;
     const bool phases = p->split_blocks > kSplitPhase;
     p->bulk_out = p->bulk_out && !phases;
@@ -1660,22 +1499,58 @@ static cudaError_t launch_kernel(const GemmArgs& g, const Plan& p, const CUtenso
     return cudaGetLastError();
 }
 
+// ---- operands ----------------------------------------------------------------------------------------------------------
+static size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
+
+static int operand_bytes(int type) { return type == ASHB_E4M3_ROWS ? 1 : value_bytes(type); }
+
+// Values between rows that begin at multiples of 16 bytes.
+static int64_t whole_stride(int type, int64_t cols) {
+    const int64_t values = 16 / operand_bytes(type);
+    return ceil_div(cols, values) * values;
+}
+static bool is_whole(int type, const void* at, int64_t stride) {
+    return ((uintptr_t)at & 15) == 0 && stride * operand_bytes(type) % 16 == 0;
+}
+// Bytes of the copy that an operand needs, 0 if it is taken as it is.
+static size_t copy_bytes(int type, const void* at, int64_t stride, int64_t rows, int64_t cols) {
+    return is_whole(type, at, stride) ? 0 : padded((size_t)(rows * whole_stride(type, cols)) * operand_bytes(type));
+}
+// The operand where `to` has its copy if it needs one; the copy itself is left in *p for launch_padding.
+static Operand placed(int type, const void* at, int64_t stride, int64_t rows, int64_t cols, char* to, Padding* p) {
+    if (is_whole(type, at, stride)) return Operand{at, stride};
+    const int64_t whole = whole_stride(type, cols);
+    *p = Padding{at, to, rows, cols, stride, whole * operand_bytes(type) / 16, 1, 0, 0};
+    while (p->lanes < 32 && p->lanes < p->words) p->lanes <<= 1;
+    p->units = (uint32_t)(ceil_div(rows, 256 / p->lanes * kPadRows) * ceil_div(p->words, p->lanes));
+    p->blocks = (unsigned)std::min<int64_t>(p->units, (int64_t)sm_count() * 16);
+    return Operand{to, whole};
+}
+static void launch_padding(int type, const Padding& first, const Padding& second, cudaStream_t st) {
+    const unsigned blocks = first.blocks + second.blocks;
+    if (blocks == 0) return;
+    switch (operand_bytes(type)) {
+        case 1: pad_kernel<uint8_t><<<blocks, 256, 0, st>>>(first, second); break;
+        case 2: pad_kernel<uint16_t><<<blocks, 256, 0, st>>>(first, second); break;
+        default: pad_kernel<uint32_t><<<blocks, 256, 0, st>>>(first, second);
+    }
+}
+
+// Operands' rows begin at multiples of 16 bytes.
 template <int KIND, bool A_DOWN, bool B_DOWN>
 static int run_product(GemmArgs g, int type, Plan p, cudaStream_t st) {
-    constexpr int kBytes = KIND == kEight ? 1 : KIND == kSplit ? 4 : 2;
-    // rows start at multiples of 16 bytes; for loads of their own they end there too
-    const auto starts = [&](const Operand& o) { return ((uintptr_t)o.at & 15) == 0 && o.stride * kBytes % 16 == 0; };
-    g.a.wide = starts(g.a) && (A_DOWN ? g.m : g.k) * kBytes % 16 == 0;
-    g.b.wide = starts(g.b) && (B_DOWN ? g.n : g.k) * kBytes % 16 == 0;
     CUtensorMap ma{}, mb{};
     const int down = KIND == kSplit ? kSplitBlock : 64;      // rows of a box that k runs down
-    const bool bulk = starts(g.a) && starts(g.b) &&
-                      operand_map(&ma, KIND, type, g.a, A_DOWN ? g.k : g.m, A_DOWN ? g.m : g.k, A_DOWN ? down : kTileM) &&
-                      operand_map(&mb, KIND, type, g.b, B_DOWN ? g.k : g.n, B_DOWN ? g.n : g.k, B_DOWN ? down : p.bn);
+    if (!operand_map(&ma, KIND, type, g.a, A_DOWN ? g.k : g.m, A_DOWN ? g.m : g.k, A_DOWN ? down : kTileM) ||
+        !operand_map(&mb, KIND, type, g.b, B_DOWN ? g.k : g.n, B_DOWN ? g.n : g.k, B_DOWN ? down : p.bn)) {
+        set_error("no tensor map of a product's operands");
+        return ASHB_ERR_CUDA;
+    }
     FinishMaps maps{};
     p.bulk_out = finish_maps(&maps, g, p.splits);
-    if (KIND == kSplit && bulk) plan_split(&p, A_DOWN, B_DOWN, g.k, g.f.slope != nullptr);
-    else plan_shared(&p, KIND, bulk, ceil_div(g.k, kBlockK<KIND>), g.f.partial || g.f.type == ASHB_F32 ? 4096 : 2048, g.f.slope != nullptr);
+    constexpr int64_t kBlock = kBlockK<KIND>;
+    if (KIND == kSplit) plan_split(&p, A_DOWN, B_DOWN, g.k, g.f.slope != nullptr);
+    else plan_shared(&p, ceil_div(g.k, kBlock), g.f.partial || g.f.type == ASHB_F32 ? 4096 : 2048, g.f.slope != nullptr);
     g.bulk_out = p.bulk_out;
     g.bufs = p.bufs;
     g.finish_bytes = p.finish_bytes;
@@ -1687,36 +1562,18 @@ static int run_product(GemmArgs g, int type, Plan p, cudaStream_t st) {
     g.raws = p.raws;
     g.b_stays = p.b_stays;
     g.columns = p.columns;
-    const int64_t block = KIND == kEight ? 128 : KIND == kSplit && bulk ? kSplitBlock : 64;
     ASHB_REQUIRE(p.tiles_m * p.tiles_n * p.splits < (int64_t)1 << 31, "a product of %lld x %lld values", (long long)g.m, (long long)g.n);
     g.tiles_m = (uint32_t)p.tiles_m;
     g.tiles_n = (uint32_t)p.tiles_n;
     g.tiles = g.tiles_m * g.tiles_n;
     g.splits = (uint32_t)p.splits;
     g.items = g.tiles * g.splits;
-    g.blocks_k = (uint32_t)ceil_div(g.k, block);
+    g.blocks_k = (uint32_t)ceil_div(g.k, kBlock);
     g.split_blocks = (uint32_t)p.split_blocks;
-    g.block_k = (uint32_t)block;
+    g.block_k = (uint32_t)kBlock;
     g.desc = product_desc(kTileM, p.bn, KIND == kEight ? 0 : KIND == kSplit || type == ASHB_BF16 ? 1 : 0, A_DOWN, B_DOWN);
-    if constexpr (KIND != kSplit) {
-        if (bulk) {
-            ASHB_CUDA_TRY((launch_kernel<layer_gemm_kernel<KIND, true, A_DOWN, B_DOWN, false>>(g, p, ma, mb, maps, st)));
-            return ASHB_OK;
-        }
-    }
-    if constexpr (KIND == kSplit) {
-        if (bulk) {
-            ASHB_CUDA_TRY((launch_kernel<split_gemm_kernel<A_DOWN, B_DOWN>>(g, p, ma, mb, maps, st)));
-            return ASHB_OK;
-        }
-    }
-    if constexpr (!A_DOWN) {
-        if (p.b_stays) {
-            ASHB_CUDA_TRY((launch_kernel<layer_gemm_kernel<KIND, false, A_DOWN, B_DOWN, true>>(g, p, ma, mb, maps, st)));
-            return ASHB_OK;
-        }
-    }
-    ASHB_CUDA_TRY((launch_kernel<layer_gemm_kernel<KIND, false, A_DOWN, B_DOWN, false>>(g, p, ma, mb, maps, st)));
+    if constexpr (KIND == kSplit) ASHB_CUDA_TRY((launch_kernel<split_gemm_kernel<A_DOWN, B_DOWN>>(g, p, ma, mb, maps, st)));
+    else ASHB_CUDA_TRY((launch_kernel<layer_gemm_kernel<KIND, A_DOWN, B_DOWN>>(g, p, ma, mb, maps, st)));
     return ASHB_OK;
 }
 
@@ -1726,13 +1583,13 @@ static int run_typed(const GemmArgs& g, int type, const Plan& p, cudaStream_t st
                             : run_product<kHalf, A_DOWN, B_DOWN>(g, type, p, st);
 }
 
-static int kind_of(int type) { return type == ASHB_F32 ? kSplit : type == ASHB_E4M3_ROWS ? kEight : kHalf; }
-
 template <class T, class OUT>
-static void launch_few(const GemmArgs& g, cudaStream_t st) {
+static void launch_few(const GemmArgs& g, bool wide, cudaStream_t st) {
     const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(g.n, 8), (int64_t)sm_count() * 8);
-    few_rows_kernel<T, OUT, sizeof(OUT) == 2><<<grid, 256, 0, st>>>(g);
+    few_rows_kernel<T, OUT, sizeof(OUT) == 2><<<grid, 256, 0, st>>>(g, wide);
 }
+
+static int kind_of(int type) { return type == ASHB_F32 ? kSplit : type == ASHB_E4M3_ROWS ? kEight : kHalf; }
 
 struct SlopePlan {
     int vec, lanes;
@@ -1755,27 +1612,37 @@ static int64_t slope_rows(int type, int64_t rows, int64_t n) {
 
 template <class T>
 static void launch_slope(const SlopePlan& p, const void* dy, const void* slope, int kind, int64_t rows, int64_t n, void* dz,
-                         float* partial, cudaStream_t st) {
+                         int64_t dz_stride, float* partial, cudaStream_t st) {
     const dim3 grid(p.across, p.down);
     const T *g = static_cast<const T*>(dy), *s = static_cast<const T*>(slope);
-    if (p.vec > 1) slope_kernel<T, 16 / sizeof(T)><<<grid, 256, 0, st>>>(g, s, kind, rows, n, p.lanes, static_cast<T*>(dz), partial);
-    else slope_kernel<T, 1><<<grid, 256, 0, st>>>(g, s, kind, rows, n, p.lanes, static_cast<T*>(dz), partial);
+    if (p.vec > 1) slope_kernel<T, 16 / sizeof(T)><<<grid, 256, 0, st>>>(g, s, kind, rows, n, p.lanes, static_cast<T*>(dz), dz_stride, partial);
+    else slope_kernel<T, 1><<<grid, 256, 0, st>>>(g, s, kind, rows, n, p.lanes, static_cast<T*>(dz), dz_stride, partial);
 }
 
-static size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
-
+// What the backward pass needs: dz where it differs from dy or dy's rows are no whole words, copies of x and the weights that
+// are none, partial sums of the bias's and the weights' gradients.
 struct BackwardPlan {
-    size_t dz, bias, weight, total;      // offsets into the workspace
+    size_t dz, x, weight, sums_b, sums_w, total;      // offsets into the workspace
+    bool makes_dz;
+    int64_t dz_stride;
     Plan pw;
 };
-static BackwardPlan plan_backward(int type, int64_t rows, int64_t inputs, int64_t outputs, int kind, bool want_w, bool want_b) {
+static BackwardPlan plan_backward(int type, const void* dy, const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
+                                  int64_t rows, int64_t inputs, int64_t outputs, int kind, bool want_x, bool want_w, bool want_b) {
     BackwardPlan b{};
     size_t at = 0;
+    const bool products = want_x || want_w;
+    b.makes_dz = products && (kind != 0 || !is_whole(type, dy, outputs));
+    b.dz_stride = b.makes_dz ? whole_stride(type, outputs) : outputs;
     b.dz = at;
-    if (kind != 0) at += padded((size_t)(rows * outputs) * value_bytes(type));
-    b.bias = at;
-    if (want_b) at += padded((size_t)(slope_rows(type, rows, outputs) * outputs) * sizeof(float));
+    if (b.makes_dz) at += padded((size_t)(rows * b.dz_stride) * value_bytes(type));
+    b.x = at;
+    if (want_w) at += copy_bytes(type, x, x_stride, rows, inputs);
     b.weight = at;
+    if (want_x) at += copy_bytes(type, weight, weight_stride, outputs, inputs);
+    b.sums_b = at;
+    if (want_b) at += padded((size_t)(slope_rows(type, rows, outputs) * outputs) * sizeof(float));
+    b.sums_w = at;
     if (want_w) {
         b.pw = plan_product(kind_of(type), true, true, outputs, inputs, rows, true);
         if (b.pw.splits > 1) at += padded((size_t)(b.pw.splits * outputs * inputs) * sizeof(float));
@@ -1800,7 +1667,7 @@ extern "C" {
 int ashb_linear_forward(int type, const void* x, int64_t x_stride, const float* x_scales, const void* weight,
                         int64_t weight_stride, const float* weight_scales, const void* bias, const void* residual,
                         int64_t residual_stride, int64_t rows, int64_t inputs, int64_t outputs, int activation, float omega,
-                        int out_type, void* y, void* slope, void* stream) {
+                        int out_type, void* y, void* slope, void* workspace, int64_t workspace_bytes, void* stream) {
     const bool eight = type == ASHB_E4M3_ROWS;
     ASHB_REQUIRE(is_value_type(type) || eight, "operand type %d", type);
     ASHB_REQUIRE(is_value_type(out_type) && (eight || out_type == type), "output type %d", out_type);
@@ -1811,8 +1678,8 @@ int ashb_linear_forward(int type, const void* x, int64_t x_stride, const float* 
     ASHB_REQUIRE((x_stride >= inputs || rows == 1) && weight_stride >= inputs, "rows overlap");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     GemmArgs g{};
-    g.a = Operand{x, x_stride, 0};
-    g.b = Operand{weight, weight_stride, 0};
+    g.a = Operand{x, x_stride};
+    g.b = Operand{weight, weight_stride};
     g.m = rows;
     g.n = outputs;
     g.k = inputs;
@@ -1832,31 +1699,45 @@ int ashb_linear_forward(int type, const void* x, int64_t x_stride, const float* 
              (((uintptr_t)y | (uintptr_t)slope | (uintptr_t)bias | (uintptr_t)residual) & (four - 1)) == 0 &&
              ((uintptr_t)f.b_scales & 15) == 0;
     if (rows <= kFewRows) {
-        const int bytes = eight ? 1 : value_bytes(type);
-        const auto wide = [&](const Operand& o) {
-            return ((uintptr_t)o.at & 15) == 0 && o.stride * bytes % 16 == 0 && inputs * bytes % 16 == 0;
-        };
-        g.a.wide = wide(g.a);
-        g.b.wide = wide(g.b);
-        if (type == ASHB_F32) launch_few<float, float>(g, st);
-        else if (type == ASHB_F16) launch_few<__half, __half>(g, st);
-        else if (type == ASHB_BF16) launch_few<__nv_bfloat16, __nv_bfloat16>(g, st);
-        else if (out_type == ASHB_F32) launch_few<E4M3, float>(g, st);
-        else if (out_type == ASHB_F16) launch_few<E4M3, __half>(g, st);
-        else launch_few<E4M3, __nv_bfloat16>(g, st);
+        const bool wide = is_whole(type, x, rows == 1 ? 0 : x_stride) && is_whole(type, weight, weight_stride) &&
+                          inputs * operand_bytes(type) % 16 == 0;
+        if (type == ASHB_F32) launch_few<float, float>(g, wide, st);
+        else if (type == ASHB_F16) launch_few<__half, __half>(g, wide, st);
+        else if (type == ASHB_BF16) launch_few<__nv_bfloat16, __nv_bfloat16>(g, wide, st);
+        else if (out_type == ASHB_F32) launch_few<E4M3, float>(g, wide, st);
+        else if (out_type == ASHB_F16) launch_few<E4M3, __half>(g, wide, st);
+        else launch_few<E4M3, __nv_bfloat16>(g, wide, st);
         ASHB_LAUNCH_CHECK();
         return ASHB_OK;
     }
     const Plan p = plan_product(kind_of(type), false, false, rows, outputs, inputs, false);
+    const size_t copy_x = copy_bytes(type, x, x_stride, rows, inputs);
+    const size_t copies = copy_x + copy_bytes(type, weight, weight_stride, outputs, inputs);
+    ASHB_REQUIRE(copies == 0 || (workspace && ((uintptr_t)workspace & 255) == 0 && workspace_bytes >= (int64_t)copies),
+                 "null, unaligned or small workspace");
     ASHB_REQUIRE(!slope || (!eight && activation != kNone), "a slope is of an activation, of operands that are not quantised");
+    Padding px{}, pw{};
+    char* ws = static_cast<char*>(workspace);
+    g.a = placed(type, x, x_stride, rows, inputs, ws, &px);
+    g.b = placed(type, weight, weight_stride, outputs, inputs, ws + copy_x, &pw);
+    launch_padding(type, px, pw, st);
     if (eight) return run_product<kEight, false, false>(g, type, p, st);
     return run_typed<false, false>(g, type, p, st);
 }
 
-int64_t ashb_linear_workspace(int type, int64_t rows, int64_t inputs, int64_t outputs, int slope_kind, int want_dweight,
-                              int want_dbias) {
+int64_t ashb_linear_forward_workspace(int type, const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
+                                      int64_t rows, int64_t inputs, int64_t outputs) {
+    if ((!is_value_type(type) && type != ASHB_E4M3_ROWS) || check_sizes(rows, inputs, outputs) != ASHB_OK || rows <= kFewRows) return 0;
+    return (int64_t)(copy_bytes(type, x, x_stride, rows, inputs) + copy_bytes(type, weight, weight_stride, outputs, inputs));
+}
+
+int64_t ashb_linear_backward_workspace(int type, const void* dy, const void* x, int64_t x_stride, const void* weight,
+                                       int64_t weight_stride, int64_t rows, int64_t inputs, int64_t outputs, int slope_kind,
+                                       int want_dx, int want_dweight, int want_dbias) {
     if (!is_value_type(type) || check_sizes(rows, inputs, outputs) != ASHB_OK || rows == 0) return 0;
-    return (int64_t)plan_backward(type, rows, inputs, outputs, slope_kind, want_dweight != 0, want_dbias != 0).total;
+    return (int64_t)plan_backward(type, dy, x, x_stride, weight, weight_stride, rows, inputs, outputs, slope_kind, want_dx != 0,
+                                  want_dweight != 0, want_dbias != 0)
+            .total;
 }
 
 int ashb_linear_backward(int type, const void* dy, const void* slope, int slope_kind, const void* x, int64_t x_stride,
@@ -1876,20 +1757,31 @@ int ashb_linear_backward(int type, const void* dy, const void* slope, int slope_
                  "null buffer, or a slope that the slope kind has no use for");
     ASHB_REQUIRE(!dx || weight_stride >= inputs, "rows overlap");
     ASHB_REQUIRE(!dweight || x_stride >= inputs || rows == 1, "rows overlap");
-    const BackwardPlan bp = plan_backward(type, rows, inputs, outputs, slope_kind, dweight != nullptr, dbias != nullptr);
+    const BackwardPlan bp = plan_backward(type, dy, x, x_stride, weight, weight_stride, rows, inputs, outputs, slope_kind,
+                                          dx != nullptr, dweight != nullptr, dbias != nullptr);
     ASHB_REQUIRE(bp.total == 0 || (workspace && ((uintptr_t)workspace & 255) == 0 && workspace_bytes >= (int64_t)bp.total),
                  "null, unaligned or small workspace");
     char* ws = static_cast<char*>(workspace);
-    const void* dz = slope_kind != 0 ? ws + bp.dz : dy;
-    float* pb = dbias ? reinterpret_cast<float*>(ws + bp.bias) : nullptr;
+    float* pb = dbias ? reinterpret_cast<float*>(ws + bp.sums_b) : nullptr;
+    void* made = bp.makes_dz ? ws + bp.dz : nullptr;
+    const Operand dz{made ? made : dy, bp.dz_stride};
+    Padding px{}, pweight{}, pdy{};
+    const Operand ox = dweight ? placed(type, x, x_stride, rows, inputs, ws + bp.x, &px) : Operand{};
+    const Operand ow = dx ? placed(type, weight, weight_stride, outputs, inputs, ws + bp.weight, &pweight) : Operand{};
+    launch_padding(type, px, pweight, st);
+    if (made && slope_kind == 0) {
+        placed(type, dy, outputs, rows, outputs, ws + bp.dz, &pdy);
+        launch_padding(type, pdy, Padding{}, st);
+    }
+    ASHB_LAUNCH_CHECK();
     int64_t count_b = 0;
-    if (slope_kind != 0 || dbias) {
+    if ((made && slope_kind != 0) || dbias) {
         const bool wide = outputs * (int64_t)e % 16 == 0 && (((uintptr_t)dy | (uintptr_t)slope) & 15) == 0;
         const SlopePlan sp = plan_slope(type, rows, outputs, wide);
         count_b = sp.down;
-        if (type == ASHB_F32) launch_slope<float>(sp, dy, slope, slope_kind, rows, outputs, ws + bp.dz, pb, st);
-        else if (type == ASHB_F16) launch_slope<__half>(sp, dy, slope, slope_kind, rows, outputs, ws + bp.dz, pb, st);
-        else launch_slope<__nv_bfloat16>(sp, dy, slope, slope_kind, rows, outputs, ws + bp.dz, pb, st);
+        if (type == ASHB_F32) launch_slope<float>(sp, dy, slope, slope_kind, rows, outputs, made, bp.dz_stride, pb, st);
+        else if (type == ASHB_F16) launch_slope<__half>(sp, dy, slope, slope_kind, rows, outputs, made, bp.dz_stride, pb, st);
+        else launch_slope<__nv_bfloat16>(sp, dy, slope, slope_kind, rows, outputs, made, bp.dz_stride, pb, st);
         ASHB_LAUNCH_CHECK();
     }
     const auto finish_to = [&](void* out, int64_t n) {
@@ -1902,8 +1794,8 @@ int ashb_linear_backward(int type, const void* dy, const void* slope, int slope_
     };
     if (dx) {
         GemmArgs g{};
-        g.a = Operand{dz, outputs, 0};
-        g.b = Operand{weight, weight_stride, 0};
+        g.a = dz;
+        g.b = ow;
         g.f = finish_to(dx, inputs);
         g.m = rows;
         g.n = inputs;
@@ -1914,14 +1806,14 @@ int ashb_linear_backward(int type, const void* dy, const void* slope, int slope_
     const float* pw = nullptr;
     if (dweight) {
         GemmArgs g{};
-        g.a = Operand{dz, outputs, 0};
-        g.b = Operand{x, x_stride, 0};
+        g.a = dz;
+        g.b = ox;
         g.f = finish_to(dweight, inputs);
         g.m = outputs;
         g.n = inputs;
         g.k = rows;
         if (bp.pw.splits > 1) {
-            g.f.partial = reinterpret_cast<float*>(ws + bp.weight);
+            g.f.partial = reinterpret_cast<float*>(ws + bp.sums_w);
             pw = g.f.partial;
         }
         if (int rc = run_typed<true, true>(g, type, bp.pw, st)) return rc;
