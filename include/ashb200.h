@@ -815,8 +815,8 @@ int ashb_linear_forward(int type, const void* x_dev, int64_t x_stride, const flo
                         int64_t weight_stride, const float* weight_scales_dev, const void* bias_dev, const void* residual_dev,
                         int64_t residual_stride, int64_t rows, int64_t inputs, int64_t outputs, int activation, float omega,
                         int out_type, void* y_dev, void* slope_dev, void* workspace_dev, int64_t workspace_bytes, void* stream);
-/* Bytes of device scratch (256-byte aligned) that the call takes: 0 where rows of x and weight begin at multiples of 16
- * bytes (or there are no more than four rows of x). */
+/* Bytes of device scratch (256-byte aligned) that the call takes: copies of x and weight where their rows do not begin at
+ * multiples of 16 bytes, partial sums where the layer is small; often 0, always with four rows of x or less. */
 int64_t ashb_linear_forward_workspace(int type, const void* x_dev, int64_t x_stride, const void* weight_dev,
                                       int64_t weight_stride, int64_t rows, int64_t inputs, int64_t outputs);
 

@@ -40,10 +40,11 @@ def activation(z, name, omega):
 def sum_steps(k, dtype):
     """Steps by which a sum of k products may be off, relative to the magnitudes: 16-bit products are exact and are
     accumulated 16 (or, 8 bits, 32) at a time; float32 ones lose 2 steps to what is left out of them and are accumulated
-    over 512 before a rounded addition of two sums each."""
+    over 512 before a rounded addition of two sums each.  Where there are few tiles the sums are split into parts of 256
+    products or more, whose additions are rounded too."""
     if dtype == torch.float32:
-        return min(math.ceil(k / 16), 32) + math.ceil(k / 512) + 4
-    return math.ceil(k / 16) + 4
+        return min(math.ceil(k / 16), 32) + math.ceil(k / 512) + math.ceil(k / 256) + 4
+    return math.ceil(k / 16) + math.ceil(k / 256) + 4
 
 
 def linear(x, w, b, name, r, omega):

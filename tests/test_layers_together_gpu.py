@@ -318,6 +318,22 @@ def test_networks():
     assert bool(grid.embeddings.grad.any()) and bool(p.grad.any())
 
 
+def test_tangents_and_transforms_are_refused():
+    import ash
+    import torch.autograd.forward_ad as fwd
+
+    x, w = torch.randn(9, 8, device=DEV), torch.randn(5, 8, device=DEV)
+    with fwd.dual_level():
+        d = fwd.make_dual(x, torch.ones_like(x))
+        for call in (lambda: ash.fused_linear(d, w), lambda: ash.rms_norm(d, w[0]), lambda: ash.rms_norm(d, w[0], quantize=True),
+                     lambda: ash.fused_linear(d, w.clone().requires_grad_(True))):
+            with pytest.raises(RuntimeError):
+                call()
+        assert torch.equal(ash.fused_linear(x, w), ash.fused_linear(x, w))      # none among the tensors
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda t: ash.fused_linear(t, w))(x[None])
+
+
 def test_no_wait_ran_out():
     import __ash
 

@@ -11,7 +11,9 @@ ACTS = ["none", "relu", "silu", "gelu", "sin"]
 
 # rows, inputs, outputs: few rows, edges of tiles and stages, sizes that are no multiples of anything, one of everything
 SIZES = [(1, 256, 256), (4, 100, 33), (3, 1, 1), (5, 64, 64), (8, 16, 16), (128, 64, 128), (129, 65, 130), (127, 8, 40),
-         (1000, 35, 131), (257, 520, 96), (300, 1100, 264), (2000, 128, 8), (640, 192, 256), (1, 5000, 3), (33, 24, 520)]
+         (1000, 35, 131), (257, 520, 96), (300, 1100, 264), (2000, 128, 8), (640, 192, 256), (1, 5000, 3), (33, 24, 520),
+         # sums split over several SMs, whole and odd; more tiles than SMs with sums of several phases
+         (64, 2048, 40), (65, 3001, 33), (19000, 1100, 128), (19100, 1028, 130), (150, 40, 4001)]
 
 
 def make(m, k, n, dtype, seed, bias=True, residual=True, scale=1.0):
@@ -55,6 +57,80 @@ def test_gradients(i, dtype):
         for name, got in zip(names, grads):
             assert got.dtype == dtype
             lb.assert_within(got, *want[name], f"grad {name} of {act} {(m, k, n)}")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("what", ["x", "weight", "bias", "residual", "x weight", "bias residual"])
+def test_only_some_gradients(dtype, what):
+    import ash
+
+    for m, k, n in ((200, 63, 40), (70, 64, 64)):
+        for act in ("none", "relu", "gelu"):
+            x, w, b, r = make(m, k, n, dtype, 5, residual=act != "relu" or "residual" in what)
+            t = {"x": x, "weight": w, "bias": b, "residual": r}
+            for name in what.split():
+                t[name].requires_grad_(True)
+            y = ash.fused_linear(x, w, b, activation=act, residual=r)
+            dy = make(m, 1, n, dtype, 6)[3]
+            grads = torch.autograd.grad(y, [t[name] for name in what.split()], dy)
+            d = [None if v is None else v.detach() for v in (x, w, b, r)]
+            want = lb.backward(*d[:3], act, d[3], 1.0, dy, dtype)
+            for name, got in zip(what.split(), grads):
+                lb.assert_within(got, *want[name], f"{name} of {act}")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_values_at_the_edges_of_the_range(dtype):
+    """Zeros, the largest and the smallest values, infinities and NaN: each stays in its row."""
+    import ash
+
+    k, n = 64, 48
+    x, w, b, _ = make(300, k, n, dtype, 3, residual=False)
+    big = torch.finfo(dtype).max
+    x[1] = 0
+    x[2] = 0
+    x[2, 3] = big
+    x[4] = 0
+    x[4, 5] = torch.finfo(dtype).smallest_normal
+    x[6, 7], x[8, 9] = float("inf"), float("nan")
+    w[:, 3] = torch.where(w[:, 3] < 0, -0.5, 0.5).to(dtype)
+    y = ash.fused_linear(x, w, b)
+    assert torch.equal(y[1], b) and bool(y[8].isnan().all()) and not bool(torch.isfinite(y[6]).any())
+    rest = torch.ones(300, dtype=torch.bool, device=DEV)
+    rest[[6, 8]] = False
+    assert bool(torch.isfinite(y[rest]).all())
+    want = (x[2, 3].double() * w[:, 3].double() + b.double())
+    assert (y[2].double() - want).abs().max() <= 2 * lb.half(dtype) * big
+    for act in ("relu", "silu", "gelu", "sin"):
+        z = ash.fused_linear(x, w, b, activation=act)
+        assert bool(z[8].isnan().all()) and bool(torch.isfinite(z[0]).all() & torch.isfinite(z[9:]).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_long_phases(dtype):
+    """Sines of phases up to 2^17 by the kernel's own reduction, beyond it by the library's."""
+    import ash
+
+    x = torch.linspace(-1, 1, 4001, device=DEV)[:, None].to(dtype)
+    w = torch.ones(8, 1, device=DEV, dtype=dtype)
+    for omega in (1.0, 30.0, 1000.0, 1e5, 1.3e5, 1e7):
+        y = ash.fused_linear(x, w, activation="sin", omega=omega)
+        phase = (x.float() * omega).to(lb.D)               # the phase is a float32 product
+        bound = 2.0**-20 + lb.half(dtype) if dtype != torch.float32 else 6 * lb.STEP
+        assert (y.to(lb.D) - torch.sin(phase)).abs().max() <= bound, omega
+
+
+def test_same_bits_again():
+    import ash
+
+    for dtype, (m, k, n) in ((torch.float32, (5000, 100, 60)), (torch.bfloat16, (65, 3001, 33)), (torch.float32, (64, 2048, 40))):
+        x, w, b, r = make(m, k, n, dtype, 11)
+        leaves = [t.requires_grad_(True) for t in (x, w, b, r)]
+        runs = []
+        for _ in range(3):
+            y = ash.fused_linear(x, w, b, "gelu", r)
+            runs.append([y.detach(), *torch.autograd.grad(y, leaves, torch.ones_like(y))])
+        assert all(torch.equal(p, q) for other in runs[1:] for p, q in zip(runs[0], other))
 
 
 def test_no_wait_ran_out():

@@ -8,7 +8,8 @@ pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda:0")
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
 SIZES = [(1, 1), (3, 2), (7, 8), (1000, 16), (65, 33), (33, 64), (257, 65), (20, 128), (9, 1000), (5, 1024), (6, 1025),
-         (3, 4096), (2, 5001), (4, 8192), (3, 8193), (2, 20000), (0, 64), (5000, 40)]
+         (3, 4096), (2, 5001), (4, 8192), (3, 8193), (2, 20000), (0, 64), (5000, 40),
+         (700, 60), (1500, 9), (900, 127), (1300, 1019), (70, 1022), (40, 3230), (650, 8189), (9, 8185), (12, 7)]
 EPS = 1e-6
 
 

@@ -1717,12 +1717,10 @@ def linear_forward(x, weight, bias, activation: str, residual, omega: float, wit
     y = x.new_empty((rows, outputs), dtype=out_dtype)
     slope = torch.empty_like(y) if with_slope else None
     if rows:
-        at, w_at, size = x.data_ptr(), weight.data_ptr(), x.element_size()
-        workspace, nbytes = None, 0
-        if (at | w_at | x_stride * size | weight_stride * size) & 15:
+        at, w_at = x.data_ptr(), weight.data_ptr()
+        with _on(x.device):
             nbytes = _lib.ashb_linear_forward_workspace(kind, at, x_stride, w_at, weight_stride, rows, inputs, outputs)
             workspace = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-        with _on(x.device):
             _check(_lib.ashb_linear_forward(
                 kind, at, x_stride, _ptr(x_scales), w_at, weight_stride, _ptr(w_scales), _ptr(bias), _ptr(residual),
                 residual_stride, rows, inputs, outputs, _ACTIVATIONS[activation], omega, _VALUE_TYPES[out_dtype], y.data_ptr(),

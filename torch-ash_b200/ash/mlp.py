@@ -62,6 +62,17 @@ def _recorded(*tensors) -> bool:
     return False
 
 
+_transforms_open = getattr(backend, "transforms_open", lambda: False)
+
+
+def _refuse_tangents(*tensors) -> None:
+    """Forward-mode derivatives are not computed: rather than dropped without a word they are refused."""
+    if _transforms_open():
+        for t in tensors:
+            if t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("forward-mode derivatives of dense layers and norms are not implemented")
+
+
 # ------------------------------------------------------------------------------------------------ dense layer
 def _slope(z: torch.Tensor, activation: str, omega: float) -> torch.Tensor:
     """act'(z) by elementwise operations that autograd records."""
@@ -144,6 +155,7 @@ def fused_linear(x: Union[torch.Tensor, QuantizedRows], weight: Union[torch.Tens
     if _recorded(x, weight, bias, residual):
         y = _FusedLinear.apply(x2, weight, bias, r2, activation, float(omega))
     else:
+        _refuse_tangents(x, weight, bias, residual)
         y = backend.linear_forward(x2, weight, bias, activation, r2, float(omega), False)[0]
     return y if x.dim() == 2 else y.reshape(shape)
 
@@ -227,12 +239,14 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
     if quantize:
         if _recorded(x, weight, residual):
             raise RuntimeError("a quantised norm has no gradient: call it under torch.no_grad()")
+        _refuse_tangents(x, weight, residual)
         _, codes, scales, s, _ = backend.rms_norm_forward(x2, weight, r2, float(eps), True, False)
         y = QuantizedRows(codes.reshape(x.shape), scales.reshape(x.shape[:-1]))
         return y if residual is None else (y, s.reshape(x.shape))
     if _recorded(x, weight, residual):
         got = _RMSNorm.apply(x2, weight, r2, float(eps))
     else:
+        _refuse_tangents(x, weight, residual)
         y, _, _, s, _ = backend.rms_norm_forward(x2, weight, r2, float(eps), False, False)
         got = y if residual is None else (y, s)
     if residual is None:

@@ -10,7 +10,7 @@
 // registers of the lanes that share it between the sum of squares, the largest magnitude and the stores.  Accesses are 16
 // bytes.  Rows that are no multiples of that are taken through windows: the row's lanes walk the 16-byte words that hold it,
 // whose first and last it shares with its neighbours and stores value by value (12383 rows of 3230 bf16 values with gradients
-// 518 us with accesses of one value, %(window)s so).  Sums are
+// 518 us with accesses of one value, 309 so).  Sums are
 // float32; s enters the statistics before it is rounded to its type, the backward pass reads it rounded.  A row has
 // 8, 32 or 256 threads by its width; rows wider than 8192 are read again for each of their passes.
 // The weight's gradient is summed by a thread over the rows of its CTA, then over the CTAs in their order by a second
