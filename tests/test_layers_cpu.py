@@ -133,7 +133,7 @@ def test_library_refuses_cpu_tensors_and_bad_arguments():
     assert f(*args) == 1 and lib.ashb_linear_forward_workspace(0, p, 9, p, 8, 100, 8, 5) == 3328      # 100 rows of 32 bytes
     assert lib.ashb_linear_forward_workspace(0, p, 8, p, 8, 100, 8, 5) == 0 == lib.ashb_linear_forward_workspace(0, p, 9, p, 8, 4, 8, 5)
     assert lib.ashb_linear_backward(0, p, None, 1, p, 8, p, 8, 3, 8, 5, p, p, p, None, 0, None) == 1
-    assert lib.ashb_linear_backward(0, p, p, 1, p, 8, p, 8, 3, 8, 5, p, p, p, p, 8, None) == 1       # small workspace
+    assert lib.ashb_linear_backward(0, p, p, 1, p, 8, p, 8, 3000, 8, 5, p, p, p, p, 8, None) == 1       # small workspace
     assert lib.ashb_rms_norm_forward(0, p, 4, None, 0, p, 3, 8, 1e-6, p, None, None, None, None, None) == 1
     assert lib.ashb_rms_norm_forward(0, p, 8, None, 0, p, 3, 8, 1e-6, p, p, p, None, None, None) == 1
     assert lib.ashb_rms_norm_forward(0, p, 8, p, 8, p, 3, 8, 1e-6, p, None, None, None, None, None) == 1

@@ -19,7 +19,8 @@ def gen(seed):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("m,k,n", [(1, 64, 64), (3, 100, 7), (4, 256, 33), (5, 16, 16), (130, 128, 64), (129, 130, 131),
-                                   (257, 1040, 264), (64, 3, 5), (1000, 144, 48)])
+                                   (257, 1040, 264), (64, 3, 5), (1000, 144, 48),
+                                   (64, 4096, 40), (65, 5001, 33), (30, 2500, 130)])       # sums split over several SMs
 def test_quantised_product(m, k, n, dtype):
     import ash
 
@@ -34,8 +35,8 @@ def test_quantised_product(m, k, n, dtype):
         z, mag = xd @ wd.T, xd.abs() @ wd.abs().T
         if b is not None:
             z, mag = z + b.to(lb.D), mag + b.to(lb.D).abs()
-        # sums of codes 32 at a time, the two scales' product and the bias: rounded operations of float32
-        ez = (k / 32 + 8) * lb.STEP * mag + lb.TINY
+        # sums of codes 32 at a time, parts of 512 or more joined, the two scales' product and the bias: rounded operations
+        ez = (k / 32 + k / 512 + 8) * lb.STEP * mag + lb.TINY
         omega = 2.0 if act == "sin" else 1.0
         a, _, l1, _ = lb.activation(z, act, omega)
         y = a if r is None else a + r.to(lb.D)

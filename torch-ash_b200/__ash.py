@@ -1650,6 +1650,8 @@ def read_rows(codes: torch.Tensor, scales: torch.Tensor, indices, dtype: torch.d
 
 def _rows_of(t: torch.Tensor, name: str):
     """(2-D view or copy whose rows are contiguous, its row stride)."""
+    if t.is_cuda and t.dim() == 2 and t.is_contiguous():
+        return t, t.shape[1]
     if not t.is_cuda:
         raise RuntimeError(f"{name} must be a CUDA tensor (there is no CPU implementation), got {t.device}")
     width = t.shape[-1]
@@ -1672,17 +1674,22 @@ def rms_norm_forward(x, weight, residual, eps: float, quantize: bool, with_rstd:
     if residual is not None:
         residual, residual_stride = _rows_of(residual, "residual")
     rows, width = x.shape
-    empty = lambda *shape, dtype=x.dtype: torch.empty(shape, dtype=dtype, device=x.device)
-    y = None if quantize else empty(rows, width)
-    codes = empty(rows, width, dtype=torch.float8_e4m3fn) if quantize else None
-    scales = empty(rows, dtype=torch.float32) if quantize else None
-    total = empty(rows, width) if residual is not None else None
-    rstd = empty(rows, dtype=torch.float32) if with_rstd else None
+    device = x.device
+    y = codes = scales = None
+    if quantize:
+        codes = x.new_empty((rows, width), dtype=torch.float8_e4m3fn)
+        scales = x.new_empty((rows,), dtype=torch.float32)
+    else:
+        y = x.new_empty((rows, width))
+    total = x.new_empty((rows, width)) if residual is not None else None
+    rstd = x.new_empty((rows,), dtype=torch.float32) if with_rstd else None
     if rows:
-        with _on(x.device):
-            _check(_lib.ashb_rms_norm_forward(_VALUE_TYPES[x.dtype], x.data_ptr(), x_stride, _ptr(residual), residual_stride,
-                                              weight.data_ptr(), rows, width, eps, _ptr(y), _ptr(codes), _ptr(scales),
-                                              _ptr(total), _ptr(rstd), _stream(x.device)))
+        with _on(device):
+            rc = _lib.ashb_rms_norm_forward(_VALUE_TYPES[x.dtype], x.data_ptr(), x_stride, _ptr(residual), residual_stride,
+                                            weight.data_ptr(), rows, width, eps, _ptr(y), _ptr(codes), _ptr(scales),
+                                            _ptr(total), _ptr(rstd), _stream(device))
+        if rc:
+            _check(rc)
     return y, codes, scales, total, rstd
 
 
@@ -1705,26 +1712,38 @@ def linear_forward(x, weight, bias, activation: str, residual, omega: float, wit
     """``(y, slope or None)``, 2-D; ``scales``: (of x's rows, of weight's rows) where both are e4m3 codes."""
     x, x_stride = _rows_of(x, "x")
     weight, weight_stride = _rows_of(weight, "weight")
-    out_dtype = out_dtype or x.dtype
     rows, inputs = x.shape
-    outputs = weight.shape[0]
-    bias = None if bias is None else _cuda(bias, "bias")
-    residual_stride = 0
+    outputs, device = weight.shape[0], x.device
+    residual_stride, bias_at, residual_at, x_scales, w_scales = 0, None, None, None, None
+    if bias is not None:
+        bias = _cuda(bias, "bias")
+        bias_at = bias.data_ptr()
     if residual is not None:
         residual, residual_stride = _rows_of(residual, "residual")
-    x_scales, w_scales = (None, None) if scales is None else (_cuda(scales[0], "x.scales"), _cuda(scales[1], "weight.scales"))
-    kind = _VALUE_TYPES[x.dtype] if scales is None else _E4M3_ROWS
-    y = x.new_empty((rows, outputs), dtype=out_dtype)
+        residual_at = residual.data_ptr()
+    if scales is None:
+        kind = out_kind = _VALUE_TYPES[x.dtype]
+        y = x.new_empty((rows, outputs))
+    else:
+        kind, out_kind = _E4M3_ROWS, _VALUE_TYPES[out_dtype]
+        y = x.new_empty((rows, outputs), dtype=out_dtype)
+        x_scales, w_scales = _cuda(scales[0], "x.scales"), _cuda(scales[1], "weight.scales")
     slope = torch.empty_like(y) if with_slope else None
-    if rows:
-        at, w_at = x.data_ptr(), weight.data_ptr()
-        with _on(x.device):
+    if rows == 0:
+        return y, slope
+    at, w_at, workspace, nbytes = x.data_ptr(), weight.data_ptr(), None, 0
+    with _on(device):
+        if rows > 4:      # up to four rows take no workspace
             nbytes = _lib.ashb_linear_forward_workspace(kind, at, x_stride, w_at, weight_stride, rows, inputs, outputs)
-            workspace = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-            _check(_lib.ashb_linear_forward(
-                kind, at, x_stride, _ptr(x_scales), w_at, weight_stride, _ptr(w_scales), _ptr(bias), _ptr(residual),
-                residual_stride, rows, inputs, outputs, _ACTIVATIONS[activation], omega, _VALUE_TYPES[out_dtype], y.data_ptr(),
-                _ptr(slope), _ptr(workspace), nbytes, _stream(x.device)))
+            if nbytes:
+                workspace = x.new_empty(nbytes, dtype=torch.uint8)
+        rc = _lib.ashb_linear_forward(
+            kind, at, x_stride, _ptr(x_scales), w_at, weight_stride, _ptr(w_scales), bias_at, residual_at, residual_stride,
+            rows, inputs, outputs, _ACTIVATIONS[activation], omega, out_kind, y.data_ptr(),
+            None if slope is None else slope.data_ptr(), None if workspace is None else workspace.data_ptr(), nbytes,
+            _stream(device))
+    if rc:
+        _check(rc)
     return y, slope
 
 

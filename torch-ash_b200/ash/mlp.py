@@ -141,23 +141,28 @@ def fused_linear(x: Union[torch.Tensor, QuantizedRows], weight: Union[torch.Tens
             raise ValueError("x and weight must both be QuantizedRows or both be tensors")
         return _quantized_linear(x, weight, bias, activation, residual, omega, dtype or torch.bfloat16)
     _check_value(x, "x")
-    if dtype is not None and dtype != x.dtype:
-        raise ValueError(f"dtype is for QuantizedRows: the result of {x.dtype} rows is {x.dtype}")
+    kept = x.dtype
+    if dtype is not None and dtype != kept:
+        raise ValueError(f"dtype is for QuantizedRows: the result of {kept} rows is {kept}")
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[-1] or weight.numel() == 0:
         raise ValueError(f"x (..., inputs) and weight (outputs, inputs) are wanted, got {tuple(x.shape)} and "
                          f"{tuple(weight.shape)}")
-    shape = (*x.shape[:-1], weight.shape[0])
-    _check_like(weight, "weight", weight.shape, x, x.dtype)
-    _check_like(bias, "bias", weight.shape[:1], x, x.dtype)
-    _check_like(residual, "residual", shape, x, x.dtype)
-    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    r2 = residual if residual is None or residual.dim() == 2 else residual.reshape(-1, shape[-1])
+    outputs, flat = weight.shape[0], x.dim() == 2
+    shape = (*x.shape[:-1], outputs)
+    if weight.dtype is not kept or weight.device != x.device:
+        _check_like(weight, "weight", weight.shape, x, kept)
+    if bias is not None:
+        _check_like(bias, "bias", (outputs,), x, kept)
+    if residual is not None:
+        _check_like(residual, "residual", shape, x, kept)
+    x2 = x if flat else x.reshape(-1, x.shape[-1])
+    r2 = residual if residual is None or flat else residual.reshape(-1, outputs)
     if _recorded(x, weight, bias, residual):
         y = _FusedLinear.apply(x2, weight, bias, r2, activation, float(omega))
     else:
         _refuse_tangents(x, weight, bias, residual)
         y = backend.linear_forward(x2, weight, bias, activation, r2, float(omega), False)[0]
-    return y if x.dim() == 2 else y.reshape(shape)
+    return y if flat else y.reshape(shape)
 
 
 def _quantized_linear(x, weight, bias, activation, residual, omega, dtype):
@@ -249,6 +254,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
         _refuse_tangents(x, weight, residual)
         y, _, _, s, _ = backend.rms_norm_forward(x2, weight, r2, float(eps), False, False)
         got = y if residual is None else (y, s)
+    if x.dim() == 2:
+        return got
     if residual is None:
         return got.reshape(x.shape)
     return got[0].reshape(x.shape), got[1].reshape(x.shape)

@@ -411,12 +411,13 @@ __device__ __forceinline__ void finish_narrow(const Finish& f, const float* bloc
     }
 }
 
-__device__ __forceinline__ void finish_partial(float* partial, const float* block, int lane, int64_t row0, int64_t col0, int64_t m,
-                                               int64_t n) {
+__device__ __forceinline__ void finish_partial(const Finish& f, float* partial, const float* block, int lane, int64_t row0, int64_t col0,
+                                               int64_t m, int64_t n) {
     const int64_t col = col0 + lane;
     if (col >= n) return;
     partial += row0 * n + col;
     const int left = (int)min((int64_t)32, m - row0);
+    const float sb = f.b_scales ? f.b_scales[col] : 1.0f;
 #pragma unroll
     for (int first = 0; first < 32; first += 8) {
         float z[8];
@@ -424,6 +425,7 @@ __device__ __forceinline__ void finish_partial(float* partial, const float* bloc
         for (int i = 0; i < 8; ++i) {
             const int in = first + i;
             z[i] = block[in * 32 + (((lane >> 2) ^ (in & 7)) << 2) + (lane & 3)];
+            if (f.b_scales) z[i] *= f.a_scales[row0 + min(in, left - 1)] * sb;
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -478,7 +480,7 @@ template <int KIND, bool FORWARD>
 __device__ __forceinline__ void finish(const GemmArgs& g, const float* block, typename AheadOf<KIND>::type& r, int lane,
                                        int64_t row0, int64_t col0, int split) {
     if (g.f.partial) {
-        finish_partial(g.f.partial + split * g.m * g.n, block, lane, row0, col0, g.m, g.n);
+        finish_partial(g.f, g.f.partial + split * g.m * g.n, block, lane, row0, col0, g.m, g.n);
         return;
     }
     if constexpr (KIND == kSplit) {
@@ -1333,6 +1335,102 @@ __global__ void __launch_bounds__(256) slope_kernel(const T* __restrict__ dy, co
     }
 }
 
+// ---- gradients of a small layer ------------------------------------------------------------------------------------------
+// All gradients in one launch, for layers whose backward pass is launches and little else: a CTA has a 32 x 32 tile of dx or of
+// dW and walks the summed dimension 32 at a time, both operands as float32 in shared memory, dz made on the way (and not
+// rounded); the tiles of dW at the first inputs sum the columns of dz too.  A call takes 15 us of the host where four or five
+// launches and their maps take 30.  The GPU needs about 2.7 us for 32 of a sum: 22 us for 250 x 256 x 256 against 24 of the tensor
+// cores' kernels, but 38 for sums of 500, so these are the limits.
+constexpr int64_t kSmallLayer = (int64_t)1 << 24, kSmallSum = 256;
+
+struct SmallGrads {
+    const void *dy, *slope, *x, *weight;
+    void *dx, *dw, *db;
+    int64_t x_stride, weight_stride;
+    int rows, inputs, outputs, kind;
+    int dx_tiles;      // the first blocks', then dW's
+};
+
+template <class T>
+__global__ void __launch_bounds__(256) small_grads_kernel(const SmallGrads s) {
+    // left by the summed index, so that a thread's four values are one read that all lanes share
+    __shared__ __align__(16) float left[32][36];
+    __shared__ float right[32][33];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const bool is_dx = (int)blockIdx.x < s.dx_tiles;
+    const int tile = is_dx ? blockIdx.x : blockIdx.x - s.dx_tiles, across = (s.inputs + 31) / 32;
+    const int first = tile / across * 32, k0 = tile % across * 32;      // rows of x, or outputs; inputs
+    const int length = is_dx ? s.outputs : s.rows;
+    const T *dy = static_cast<const T*>(s.dy), *slope = static_cast<const T*>(s.slope);
+    const T* other = static_cast<const T*>(is_dx ? s.weight : s.dw ? s.x : nullptr);
+    const int64_t stride = is_dx ? s.weight_stride : s.x_stride;
+    const bool sums = !is_dx && k0 == 0 && s.db != nullptr;
+    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, total = 0.0f, a[4], b[4];
+    // dz of a row and output, and the other operand: rows of 32, the next ones fetched while these are multiplied
+    const auto fetch = [&](int at) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = ty + 8 * i;
+            const int row = is_dx ? first + r : at + r, out = is_dx ? at + tx : first + tx;
+            a[i] = b[i] = 0.0f;
+            if (row < s.rows && out < s.outputs) {
+                const int64_t e = (int64_t)row * s.outputs + out;
+                a[i] = to_float(dy[e]);
+                if (s.kind == 1) a[i] *= to_float(slope[e]);
+                else if (s.kind == 2) a[i] = to_float(slope[e]) > 0.0f ? a[i] : 0.0f;
+            }
+            if (other != nullptr && at + r < length && k0 + tx < s.inputs) b[i] = to_float(other[(at + r) * stride + k0 + tx]);
+        }
+    };
+    fetch(0);
+    for (int at = 0; at < length; at += 32) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (is_dx) left[tx][ty + 8 * i] = a[i];
+            else left[ty + 8 * i][tx] = a[i];
+            right[ty + 8 * i][tx] = b[i];
+        }
+        __syncthreads();
+        if (at + 32 < length) fetch(at + 32);
+#pragma unroll 8
+        for (int j = 0; j < 32; ++j) {
+            const float r = right[j][tx];
+            const float4 l = *reinterpret_cast<const float4*>(&left[j][4 * ty]);
+            acc[0] = fmaf(l.x, r, acc[0]);
+            acc[1] = fmaf(l.y, r, acc[1]);
+            acc[2] = fmaf(l.z, r, acc[2]);
+            acc[3] = fmaf(l.w, r, acc[3]);
+        }
+        if (sums && ty == 0) {
+#pragma unroll 8
+            for (int j = 0; j < 32; ++j) total += left[j][tx];
+        }
+        __syncthreads();
+    }
+    T* out = static_cast<T*>(is_dx ? s.dx : s.dw);
+    const int most = is_dx ? s.rows : s.outputs;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (out != nullptr && first + 4 * ty + i < most && k0 + tx < s.inputs)
+            out[(int64_t)(first + 4 * ty + i) * s.inputs + k0 + tx] = from_float<T>(acc[i]);
+    if (sums && ty == 0 && first + tx < s.outputs) static_cast<T*>(s.db)[first + tx] = from_float<T>(total);
+}
+
+static bool is_small_layer(int64_t rows, int64_t inputs, int64_t outputs) {
+    return rows <= kSmallSum && outputs <= kSmallSum && inputs <= kSmallLayer && rows * outputs * inputs <= kSmallLayer;
+}
+static void launch_small_grads(int type, SmallGrads s, cudaStream_t st) {
+    const int across = (s.inputs + 31) / 32;
+    s.dx_tiles = s.dx ? (s.rows + 31) / 32 * across : 0;
+    // dW's tiles, or those of the first inputs alone where only the columns' sums are wanted: they come first in a row of tiles
+    const int dw_tiles = s.dw || s.db ? (s.outputs + 31) / 32 * across : 0;
+    const unsigned blocks = (unsigned)(s.dx_tiles + dw_tiles);
+    if (blocks == 0) return;
+    if (type == ASHB_F32) small_grads_kernel<float><<<blocks, 256, 0, st>>>(s);
+    else if (type == ASHB_F16) small_grads_kernel<__half><<<blocks, 256, 0, st>>>(s);
+    else small_grads_kernel<__nv_bfloat16><<<blocks, 256, 0, st>>>(s);
+}
+
 // ---- plans --------------------------------------------------------------------------------------------------------------
 static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
@@ -1797,7 +1895,8 @@ int64_t ashb_linear_forward_workspace(int type, const void* x, int64_t x_stride,
 int64_t ashb_linear_backward_workspace(int type, const void* dy, const void* x, int64_t x_stride, const void* weight,
                                        int64_t weight_stride, int64_t rows, int64_t inputs, int64_t outputs, int slope_kind,
                                        int want_dx, int want_dweight, int want_dbias) {
-    if (!is_value_type(type) || check_sizes(rows, inputs, outputs) != ASHB_OK || rows == 0) return 0;
+    if (!is_value_type(type) || check_sizes(rows, inputs, outputs) != ASHB_OK || rows == 0 || is_small_layer(rows, inputs, outputs))
+        return 0;
     return (int64_t)plan_backward(type, dy, x, x_stride, weight, weight_stride, rows, inputs, outputs, slope_kind, want_dx != 0,
                                   want_dweight != 0, want_dbias != 0)
             .total;
@@ -1820,6 +1919,12 @@ int ashb_linear_backward(int type, const void* dy, const void* slope, int slope_
                  "null buffer, or a slope that the slope kind has no use for");
     ASHB_REQUIRE(!dx || weight_stride >= inputs, "rows overlap");
     ASHB_REQUIRE(!dweight || x_stride >= inputs || rows == 1, "rows overlap");
+    if (is_small_layer(rows, inputs, outputs)) {
+        launch_small_grads(type, SmallGrads{dy, slope, x, weight, dx, dweight, dbias, x_stride, weight_stride, (int)rows, (int)inputs,
+                                            (int)outputs, slope_kind, 0}, st);
+        ASHB_LAUNCH_CHECK();
+        return ASHB_OK;
+    }
     const BackwardPlan bp = plan_backward(type, dy, x, x_stride, weight, weight_stride, rows, inputs, outputs, slope_kind,
                                           dx != nullptr, dweight != nullptr, dbias != nullptr);
     ASHB_REQUIRE(bp.total == 0 || (workspace && ((uintptr_t)workspace & 255) == 0 && workspace_bytes >= (int64_t)bp.total),
