@@ -792,7 +792,7 @@ int ashb_rms_norm_forward(int dtype, const void* x_dev, int64_t x_stride, const 
                           float* scales_dev, void* sum_dev, float* rstd_dev, void* stream);
 
 /* Its gradient: dx (which is the residual's too) and dweight, from dy, the gradient dsum of `sum` (NULL: none), s (x, or
- * `sum`), and rstd.  The weight's gradient is summed in a fixed order.  _workspace: bytes of device scratch. */
+ * `sum`), and rstd.  The weight's gradient is summed in a fixed order.  _workspace: bytes of device scratch (16-byte aligned). */
 int64_t ashb_rms_norm_workspace(int64_t rows, int64_t width);
 int ashb_rms_norm_backward(int dtype, const void* dy_dev, const void* dsum_dev, const void* s_dev, const void* weight_dev,
                            const float* rstd_dev, int64_t rows, int64_t width, void* dx_dev, void* dweight_dev,

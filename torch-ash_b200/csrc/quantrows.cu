@@ -7,10 +7,10 @@
 // they have quadruples of values (32 at most), four rows of a group under way.  In one launch the registers of the
 // second part leave an SM one CTA for the first, whose chains of dependent accesses want many (1M keys with 32 values:
 // 331 us against 47 and 48).
-// Reading takes one: a CTA looks 256 keys up and notes their rows and scales in shared memory, then its threads walk the
-// 256 rows of output as one run of quadruples, four of a thread under way, so that stores are contiguous whatever the width.
-// Eight CTAs an SM with four under way read 4M keys' rows of 64 int8 values, half of them misses, in 297 us (4.3 TB/s); six with
-// eight, 303 us; lanes of a group per row, 336 us.
+// Reading takes one: a CTA looks 128 keys up and notes their rows and scales in shared memory, then its threads walk the
+// 128 rows of output as one run of quadruples, four of a thread under way, so that stores are contiguous whatever the width.
+// Sixteen CTAs an SM read 4M keys' rows of 64 int8 values, half of them misses, in 291 us (4.4 TB/s); eight of 256 keys, 297 us;
+// six with eight quadruples under way, 303 us; lanes of a group per row, 336 us.
 #include <algorithm>
 #include <cstring>
 
@@ -29,7 +29,7 @@ struct RowTable {
     int format;          // 0: copied as bytes
     int dtype;           // of the values
     int wide;            // quadruples are aligned on both sides
-    int long_rows;       // reading: a run of 256 rows has too many places for 32 bits
+    int long_rows;       // reading: a CTA's run has too many places for 32 bits
     uint32_t reciprocal; // reading: of a row's steps, for a place's row in a run (0: one step a row)
 };
 struct RowTables {
@@ -126,20 +126,20 @@ __global__ void __launch_bounds__(256, 5) quantize_rows_kernel(int64_t n, const 
 }
 
 // ---- reading rows ------------------------------------------------------------------------------------------------------
-// The rows of 256 keys or numbers: rows[i] of the codes (negative: zeros) to row first + i of the values, i < have.
+// The rows of kReaders keys or numbers: rows[i] of the codes (negative: zeros) to row first + i of the values, i < have.
 // UNIT values a step of a thread: four, or one where rows are not multiples of four or not aligned.
-constexpr int kReadsAhead = 4;
+constexpr int kReadsAhead = 4, kReaders = 128;
 template <class T, int UNIT>
 __device__ __forceinline__ void read_run(const RowTable& t, int64_t first, int have, const int* rows, const float* scales) {
     const uint8_t* codes = static_cast<const uint8_t*>(t.src);
     T* out = static_cast<T*>(t.dst) + first * t.width;
     const uint32_t per_row = (uint32_t)t.width / UNIT, total = per_row * (uint32_t)have;
-    for (uint32_t e0 = threadIdx.x; e0 < total; e0 += 256 * kReadsAhead) {
+    for (uint32_t e0 = threadIdx.x; e0 < total; e0 += kReaders * kReadsAhead) {
         uint32_t w[kReadsAhead];
         float scale[kReadsAhead];
 #pragma unroll
         for (int i = 0; i < kReadsAhead; ++i) {
-            const uint32_t e = e0 + 256 * i;
+            const uint32_t e = e0 + kReaders * i;
             w[i] = 0;
             scale[i] = 0.0f;
             if (e >= total) continue;
@@ -152,7 +152,7 @@ __device__ __forceinline__ void read_run(const RowTable& t, int64_t first, int h
         }
 #pragma unroll
         for (int i = 0; i < kReadsAhead; ++i) {
-            const uint32_t e = e0 + 256 * i;
+            const uint32_t e = e0 + kReaders * i;
             if (e >= total) continue;
             float v[4];
             decode4(w[i], scale[i], t.format, v);
@@ -162,13 +162,13 @@ __device__ __forceinline__ void read_run(const RowTable& t, int64_t first, int h
     }
 }
 
-// Rows too wide for 32-bit positions in a run of 256: a row at a time.
+// Rows too wide for 32-bit positions in a CTA's run: a row at a time.
 template <class T>
 __device__ __noinline__ void read_long(const RowTable& t, int64_t first, int have, const int* rows, const float* scales) {
     const uint8_t* codes = static_cast<const uint8_t*>(t.src);
     T* out = static_cast<T*>(t.dst);
     for (int r = 0; r < have; ++r)
-        for (int64_t c = threadIdx.x; c < t.width; c += 256) {
+        for (int64_t c = threadIdx.x; c < t.width; c += kReaders) {
             float v[4];
             decode4(rows[r] >= 0 ? (uint32_t)codes[rows[r] * t.width + c] : 0u, scales[r], t.format, v);
             out[(first + r) * t.width + c] = from_float<T>(v[0]);
@@ -184,9 +184,9 @@ __device__ __forceinline__ void read_typed(const RowTable& t, int64_t first, int
 
 // All of the CTA: the row of this thread's key is `mine` (negative: none).
 __device__ __forceinline__ void read_rows_of(const RowTables& tables, int64_t first, int64_t n, int mine) {
-    __shared__ int rows[256];
-    __shared__ float scales[256];
-    const int have = (int)min((int64_t)256, n - first);
+    __shared__ int rows[kReaders];
+    __shared__ float scales[kReaders];
+    const int have = (int)min((int64_t)kReaders, n - first);
     rows[threadIdx.x] = mine;
     for (int j = 0; j < tables.n; ++j) {
         const RowTable& t = tables.t[j];
@@ -233,10 +233,10 @@ __global__ void __launch_bounds__(256) insert_rows_kernel(Table t, const int32_t
 }
 
 template <class Table, int DIM, bool FILTER>
-__global__ void __launch_bounds__(256, 8) find_rows_kernel(Table t, const int32_t* __restrict__ keys, int64_t n,
+__global__ void __launch_bounds__(kReaders, 2048 / kReaders) find_rows_kernel(Table t, const int32_t* __restrict__ keys, int64_t n,
                                                         int64_t* __restrict__ indices, uint8_t* __restrict__ masks,
                                                         const __grid_constant__ RowTables tables) {
-    const int64_t first = (int64_t)blockIdx.x * 256, i = first + threadIdx.x;
+    const int64_t first = (int64_t)blockIdx.x * kReaders, i = first + threadIdx.x;
     int found = -1;
     if (i < n) {
         int k0, k1, k2, k3;
@@ -263,9 +263,9 @@ __global__ void __launch_bounds__(256, 8) find_rows_kernel(Table t, const int32_
 
 // ---- rows in order, or by number -------------------------------------------------------------------------------
 // A number outside 0 .. n_rows - 1 reads zeros.
-__global__ void __launch_bounds__(256, 8) read_rows_kernel(int64_t n, const int64_t* __restrict__ numbers, int64_t n_rows,
+__global__ void __launch_bounds__(kReaders, 2048 / kReaders) read_rows_kernel(int64_t n, const int64_t* __restrict__ numbers, int64_t n_rows,
                                                         const __grid_constant__ RowTables tables) {
-    const int64_t first = (int64_t)blockIdx.x * 256, i = first + threadIdx.x;
+    const int64_t first = (int64_t)blockIdx.x * kReaders, i = first + threadIdx.x;
     const int64_t row = i < n ? (numbers ? numbers[i] : i) : -1;
     read_rows_of(tables, first, n, row >= 0 && row < n_rows ? (int)row : -1);
 }
@@ -310,7 +310,7 @@ static int check_table(const ashb_row_table* in, bool reading, bool may_copy, Ro
     const uintptr_t values = (uintptr_t)(reading ? in->dst : in->src), codes = (uintptr_t)(reading ? in->src : in->dst);
     ASHB_REQUIRE((values & (value_bytes(in->dtype) - 1)) == 0, "row table: values not aligned to their type");
     out->wide = in->width % 4 == 0 && (values & (4 * value_bytes(in->dtype) - 1)) == 0 && (codes & 3) == 0;
-    // e * ceil(2^32 / steps) >> 32 is e / steps while e * steps < 2^32, e being below 256 * steps
+    // e * ceil(2^32 / steps) >> 32 is e / steps while e * steps < 2^32, e being below 256 * steps (kReaders is no more)
     const int64_t steps = out->wide ? in->width / 4 : in->width;
     out->long_rows = steps >= 4096;
     out->reciprocal = steps == 1 || out->long_rows ? 0u : (uint32_t)(((1ull << 32) + (uint64_t)steps - 1) / (uint64_t)steps);
@@ -328,7 +328,7 @@ static int check_tables(int n, const ashb_row_table* in, bool reading, bool may_
 }
 
 static int tile_count(int64_t n, unsigned* grid) {
-    ASHB_REQUIRE(n >= 0 && (n + 255) / 256 <= 0x7FFFFFFF, "%lld rows", (long long)n);
+    ASHB_REQUIRE(n >= 0 && n / kReaders < 0x7FFFFFFF, "%lld rows", (long long)n);
     *grid = (unsigned)((n + 255) / 256);
     return ASHB_OK;
 }
@@ -379,16 +379,17 @@ int ashb_map_find_rows(ashb_map* m, const int32_t* keys, int64_t n, int64_t* ind
     const Table16 t = table16_of(m);
     // as find: tables beyond L2 ask the occupancy bits first
     const bool filter = m->occupied != nullptr && m->n_slots * m->slot_bytes >= (size_t)64 << 20;
+    const unsigned readers = (unsigned)((n + kReaders - 1) / kReaders);
 #define ASHB_FIND_ROWS(DIM)                                                                                              \
-    if (filter) find_rows_kernel<Table16, DIM, true><<<grid, 256, 0, st>>>(t, keys, n, indices, masks, v);                \
-    else find_rows_kernel<Table16, DIM, false><<<grid, 256, 0, st>>>(t, keys, n, indices, masks, v)
+    if (filter) find_rows_kernel<Table16, DIM, true><<<readers, kReaders, 0, st>>>(t, keys, n, indices, masks, v);                \
+    else find_rows_kernel<Table16, DIM, false><<<readers, kReaders, 0, st>>>(t, keys, n, indices, masks, v)
     switch (m->key_dim) {
         case 1: ASHB_FIND_ROWS(1); break;
         case 2: ASHB_FIND_ROWS(2); break;
         case 3: ASHB_FIND_ROWS(3); break;
         default: {
             const Table32 t4{static_cast<Slot32*>(m->slots), (uint32_t)(m->n_slots - 1), m->status};
-            find_rows_kernel<Table32, 4, false><<<grid, 256, 0, st>>>(t4, keys, n, indices, masks, v);
+            find_rows_kernel<Table32, 4, false><<<readers, kReaders, 0, st>>>(t4, keys, n, indices, masks, v);
         }
     }
 #undef ASHB_FIND_ROWS
@@ -415,7 +416,7 @@ int ashb_read_rows(int64_t n, const int64_t* numbers, int64_t n_rows, const ashb
     ASHB_REQUIRE(numbers != nullptr || n <= n_rows, "more rows than the table has");
     RowTables t;
     if (int rc = check_tables(1, table, true, false, &t)) return rc;
-    read_rows_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(n, numbers, n_rows, t);
+    read_rows_kernel<<<(unsigned)((n + kReaders - 1) / kReaders), kReaders, 0, static_cast<cudaStream_t>(stream)>>>(n, numbers, n_rows, t);
     ASHB_LAUNCH_CHECK();
     return ASHB_OK;
 }
