@@ -148,6 +148,17 @@ def test_second_order(act):
         assert (p.to(lb.D) - q).abs().max() <= 2.0**-15 * max(1.0, q.abs().max().item())
 
 
+@pytest.mark.parametrize("act", ["none", "silu"])
+def test_second_order_without_rows(act):
+    import ash
+
+    x, w, b = torch.empty(0, 6, device=DEV), torch.ones(9, 6, device=DEV), torch.ones(9, device=DEV)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    grads = torch.autograd.grad(ash.fused_linear(x, w, b, act).sum(), leaves, create_graph=True)
+    assert [tuple(t.shape) for t in grads] == [(0, 6), (9, 6), (9,)]
+    assert not grads[1].any() and not grads[2].any()
+
+
 def test_streams_and_graph():
     """On a stream of its own, two at once, and captured: the same bits."""
     import ash

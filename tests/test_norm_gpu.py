@@ -168,6 +168,40 @@ def test_differences_and_second_order():
     assert abs(numeric - (second * u).sum().item()) < 2e-2 * max(1.0, abs(numeric))
 
 
+@pytest.mark.parametrize("made", ["same", "scaled", "normed"])
+def test_second_order_with_a_residual_made_from_x(made):
+    """What reaches x by way of the residual counts once, whether the backward pass is recorded or not, and the gradient of
+    the recorded one is that of the formula in 64 bits."""
+    import ash
+
+    g = torch.Generator(device=DEV).manual_seed(11)
+    x, dy, ds, v = (torch.randn(5, 24, generator=g, device=DEV) for _ in range(4))
+    w = 1 + torch.randn(24, generator=g, device=DEV) / 5
+
+    def formula(x, w, residual=None):
+        s = x if residual is None else x + residual
+        y = s * torch.rsqrt((s * s).mean(1, keepdim=True) + 1e-6) * w
+        return y if residual is None else (y, s)
+
+    def grads(norm, x, w, dy, ds, create):
+        r = {"same": lambda: x, "scaled": lambda: x * 1.5, "normed": lambda: norm(x, w) * 0.5}[made]()
+        return torch.autograd.grad(norm(x, w, residual=r), [x, w], [dy, ds], create_graph=create)
+
+    leaves = [x.requires_grad_(True), w.requires_grad_(True)]
+    exact = [t.detach().to(lb.D).requires_grad_(True) for t in leaves]
+    want = grads(formula, *exact, dy.to(lb.D), ds.to(lb.D), True)
+    for create in (False, True):
+        got = grads(ash.rms_norm, *leaves, dy, ds, create)
+        for a, b in zip(got, want):
+            # a few dozen float32 steps of values of order ten: 2^-24 x 2^8
+            assert (a.to(lb.D) - b).abs().max() <= 2.0**-16 * max(1.0, b.abs().max().item())
+    second = torch.autograd.grad((got[0] * v).sum() + got[1].square().sum(), leaves)
+    exact2 = torch.autograd.grad((want[0] * v.to(lb.D)).sum() + want[1].square().sum(), exact)
+    for a, b in zip(second, exact2):
+        # twice as many steps, of products of two such values: 2^-24 x 2^10
+        assert (a.to(lb.D) - b).abs().max() <= 2.0**-14 * max(1.0, b.abs().max().item())
+
+
 def test_only_the_sum_is_used():
     import ash
 

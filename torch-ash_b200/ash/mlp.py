@@ -11,6 +11,10 @@ is rounded once.  float32 layers are as exact as float32 sums (their factors are
 bfloat16 parts), except that an infinity among x or W makes NaN of what it touches.  Both functions are differentiable
 any number of times: a backward pass that is itself recorded (``create_graph=True``) is composed of the same functions and
 elementwise ones.
+
+A training step may be captured in a CUDA graph under the conditions that torch puts on any: run it a few times on a side
+stream first, and let the outputs of those runs go before the capture, since autograd otherwise meets the leaves'
+accumulation on the stream that they were made for and the capture fails.
 """
 import math
 from typing import List, Optional, Tuple, Union
@@ -115,7 +119,8 @@ class _FusedLinear(torch.autograd.Function):
                 z = fused_linear(x, weight, bias)
                 dz = (grad.float() * _slope(z.float(), ctx.activation, ctx.omega)).to(grad.dtype)
             dx = fused_linear(dz, weight.t()) if want_x else None
-            dw = fused_linear(dz.t(), x.t()) if want_w else None
+            # without rows there is no product to take
+            dw = (fused_linear(dz.t(), x.t()) if x.shape[0] else torch.zeros_like(weight)) if want_w else None
             db = dz.float().sum(0).to(dz.dtype) if want_b else None
         elif want_x or want_w or want_b:
             dx, dw, db = backend.linear_backward(grad, slope, ctx.kind, x, weight, want_x, want_w, want_b)
@@ -208,20 +213,22 @@ class _RMSNorm(torch.autograd.Function):
         if dy is None:
             return ds, None, ds if ctx.has_residual else None, None
         if torch.is_grad_enabled():
-            inputs = [t for t in (x, weight, residual) if t is not None and t.requires_grad]
-            y, s = _composed_norm(x, weight, residual, ctx.eps)
-            outs, grads = ([y], [dy]) if ds is None else ([y, s], [dy, ds])
-            got = iter(torch.autograd.grad(outs, inputs, grads, create_graph=True, allow_unused=True))
-            return (*[next(got) if t is not None and t.requires_grad else None for t in (x, weight, residual)], None)
+            dx, dw = _composed_norm_gradients(x, weight, residual, ctx.eps, dy, ds)
+            return dx, dw, dx if ctx.has_residual else None, None
         dx, dw = backend.rms_norm_backward(dy, ds, x if total is None else total, weight, rstd)
         return dx, dw, dx if ctx.has_residual else None, None
 
 
-def _composed_norm(x, weight, residual, eps):
-    """The same by elementwise operations that autograd records."""
-    s = x.float() if residual is None else x.float() + residual.float()
-    y = s * torch.rsqrt((s * s).mean(1, keepdim=True) + eps) * weight.float()
-    return y.to(x.dtype), s.to(x.dtype)
+def _composed_norm_gradients(x, weight, residual, eps, dy, ds):
+    """The gradients of x (and the residual) and of the weight, by elementwise operations that autograd records.  Written out:
+    asking autograd for those of a composed norm would count what reaches x by way of a residual made from it twice."""
+    s, g = x.float() if residual is None else x.float() + residual.float(), dy.float()
+    rstd = torch.rsqrt((s * s).mean(1, keepdim=True) + eps)
+    n, gw = s * rstd, g * weight.float()
+    dx = rstd * (gw - n * (gw * n).mean(1, keepdim=True))
+    if ds is not None:
+        dx = dx + ds.float()
+    return dx.to(x.dtype), (g * n).sum(0).to(weight.dtype)
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, eps: float = 1e-6,
