@@ -237,7 +237,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
     weight``.  Returns y, with a residual ``(y, s)``.
 
     ``quantize``: y comes as ``QuantizedRows`` in e4m3, the operand of ``fused_linear``; that form is for serving and has no
-    gradient.  A row of zeros gives zeros; a row that holds an infinity or a NaN gives NaN.
+    gradient.  A row of zeros gives zeros (with an eps of 0 NaN, 0/0); a row that holds an infinity or a NaN gives NaN.
     """
     _check_value(x, "x")
     if x.dim() < 1 or x.shape[-1] < 1:
