@@ -60,6 +60,32 @@ def test_gradients(i, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [1, 2, 3, 4, 5])
+def test_few_outputs(n, dtype):
+    """Heads: rows that are and are not whole 16-byte words, from one value on, the last group of lanes half empty, columns
+    of wider rows, and both sides of the widest rows that have a kernel of their own."""
+    import ash
+
+    for i, (m, k) in enumerate(((5, 1), (33, 3), (1000, 16), (257, 64), (4099, 63), (50, 162), (301, 65), (20001, 8), (7, 64))):
+        for j, act in enumerate(ACTS):
+            omega = 2.0 if act == "sin" else 1.0
+            x, w, b, r = make(m, k, n, dtype, 300 + 7 * i + j, bias=(i + j) % 3 != 0, residual=(i + j) % 2 == 0)
+            if i % 2:      # columns of wider tables, which begin anywhere
+                x, w = (torch.cat([t[:, :1], t, t[:, :j]], 1)[:, 1:1 + k] for t in (x, w))
+            leaves = [t.requires_grad_(True) for t in (x, w)]
+            got = ash.fused_linear(x, w, b, activation=act, residual=r, omega=omega)
+            with torch.no_grad():
+                y, z, a, d, ez, l1, l2 = lb.linear(x, w, b, act, r, omega)
+                bound = lb.forward_bound(y, z, a, ez, l1, act, r, omega, dtype)
+                for one in (got, ash.fused_linear(x, w, b, activation=act, residual=r, omega=omega)):
+                    lb.assert_within(one, y, bound, f"{act} {(m, k, n)}")
+            dy = make(m, 1, n, dtype, i)[3]
+            want = lb.backward(x.detach(), w.detach(), b, act, r, omega, dy, dtype)
+            for name, grad in zip(("x", "weight"), torch.autograd.grad(got, leaves, dy)):
+                lb.assert_within(grad, *want[name], f"grad {name} of {act} {(m, k, n)}")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("what", ["x", "weight", "bias", "residual", "x weight", "bias residual"])
 def test_only_some_gradients(dtype, what):
     import ash

@@ -1294,6 +1294,90 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const GemmArgs g, bool wi
     }
 }
 
+// ---- few outputs ---------------------------------------------------------------------------------------------------
+// Heads of one to three outputs (a distance, a colour) on narrow rows, and of four where rows are no whole 16-byte words: their
+// tiles are nearly empty, and leave value by value.  Four lanes have a row, and two rows at a time, which share the weights that
+// they fetch from L1; with more lanes a row's shuffles and its way out cost more than its products.  The four sums of a row are
+// joined by halves: lanes give two away and keep two, then one, and end with an output each.
+// A million rows of 64 into one output: float32 64 us (tiles 156), bf16 43 (87); 16 into three 36 (140) and 39 (85); 100k rows of
+// 63 into three 23 (38, a copy to whole rows included) and 19 (28).  Bf16 rows of 64 into four gain nothing (59 against 52), nor do
+// wider rows, where four lanes are too few and more do too much beside (162 into four 182 against 152).
+constexpr int kFewOutputs = 4, kNarrowRow = 64, kRowLanes = 4;
+
+template <class T, bool ROUNDED>
+__global__ void __launch_bounds__(256) few_outputs_kernel(const GemmArgs g, bool wide) {
+    constexpr int kVec = 16 / sizeof(T), kRows = 2, lanes = kRowLanes;
+    const int sub = threadIdx.x & (lanes - 1), outputs = (int)g.n;
+    const int64_t groups = (int64_t)gridDim.x * (256 / lanes), me = (int64_t)blockIdx.x * (256 / lanes) + threadIdx.x / lanes;
+    const int64_t rounds = (g.m + groups * kRows - 1) / (groups * kRows);      // of all lanes alike, for the shuffles
+    const T* weights = static_cast<const T*>(g.b.at);
+    const bool upper = sub & 2, second = sub & 1;
+    const int n = sub;                                                         // this lane's output
+    for (int64_t round = 0; round < rounds; ++round) {
+        const int64_t row0 = (round * groups + me) * kRows;
+        const T* x[kRows];
+        float sum[kRows][kFewOutputs];
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            x[i] = static_cast<const T*>(g.a.at) + min(row0 + i, g.m - 1) * g.a.stride;
+#pragma unroll
+            for (int r = 0; r < kFewOutputs; ++r) sum[i][r] = 0.0f;
+        }
+        if (wide) {
+#pragma unroll 2
+            for (int64_t k = sub * kVec; k < g.k; k += lanes * kVec) {
+                float xv[kRows][kVec];
+#pragma unroll
+                for (int i = 0; i < kRows; ++i) words_to_floats<T>(__ldg(reinterpret_cast<const uint4*>(x[i] + k)), xv[i]);
+#pragma unroll
+                for (int r = 0; r < kFewOutputs; ++r) {
+                    if (r >= outputs) break;
+                    float wv[kVec];
+                    words_to_floats<T>(__ldg(reinterpret_cast<const uint4*>(weights + r * g.b.stride + k)), wv);
+#pragma unroll
+                    for (int i = 0; i < kRows; ++i)
+#pragma unroll
+                        for (int j = 0; j < kVec; ++j) sum[i][r] = fmaf(wv[j], xv[i][j], sum[i][r]);
+                }
+            }
+        } else {
+#pragma unroll 4
+            for (int64_t k = sub; k < g.k; k += lanes) {
+                float xv[kRows];
+#pragma unroll
+                for (int i = 0; i < kRows; ++i) xv[i] = to_float(x[i][k]);
+#pragma unroll
+                for (int r = 0; r < kFewOutputs; ++r) {
+                    if (r >= outputs) break;
+                    const float wv = to_float(weights[r * g.b.stride + k]);
+#pragma unroll
+                    for (int i = 0; i < kRows; ++i) sum[i][r] = fmaf(wv, xv[i], sum[i][r]);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            float (&s)[kFewOutputs] = sum[i];
+            const float a = (upper ? s[2] : s[0]) + __shfl_xor_sync(0xffffffffu, upper ? s[0] : s[2], 2);
+            const float b = (upper ? s[3] : s[1]) + __shfl_xor_sync(0xffffffffu, upper ? s[1] : s[3], 2);
+            const float v = (second ? b : a) + __shfl_xor_sync(0xffffffffu, second ? a : b, 1);
+            if (row0 + i >= g.m || n >= outputs) continue;
+            const Finish& f = g.f;
+            float z[1] = {v}, d[1] = {1.0f};
+            if (f.bias) z[0] += to_float(static_cast<const T*>(f.bias)[n]);
+            const float r = f.residual ? to_float(static_cast<const T*>(f.residual)[(row0 + i) * f.residual_stride + n]) : 0.0f;
+            const int64_t at = (row0 + i) * outputs + n;
+            by_activation(f.activation, [&](auto act) {
+                constexpr int ACT = decltype(act)::value;
+                if (f.slope) activate<ACT, true, ROUNDED>(f.omega, z, d);
+                else activate<ACT, false, ROUNDED>(f.omega, z, d);
+            });
+            if (f.slope) static_cast<T*>(f.slope)[at] = from_float<T>(d[0]);
+            static_cast<T*>(f.out)[at] = from_float<T>(z[0] + r);
+        }
+    }
+}
+
 // ---- dz and its column sums -------------------------------------------------------------------------------------------
 // dz = dy * slope (slope kind 1) or dy where the output is positive (kind 2: relu without a residual); column sums of it
 // (kind 0: of dy) over the rows of a CTA go to partial[CTA][outputs].  A row has as many lanes as it has accesses, 32 at
@@ -1640,6 +1724,17 @@ static int64_t whole_stride(int type, int64_t cols) {
 static bool is_whole(int type, const void* at, int64_t stride) {
     return ((uintptr_t)at & 15) == 0 && stride * operand_bytes(type) % 16 == 0;
 }
+
+static bool takes_few_outputs(int type, const void* x, int64_t x_stride, int64_t inputs, int64_t outputs) {
+    return type != ASHB_E4M3_ROWS && outputs <= kFewOutputs && inputs <= kNarrowRow &&
+           (outputs < kFewOutputs || !is_whole(type, x, x_stride));
+}
+
+template <class T>
+static void launch_few_outputs(const GemmArgs& g, bool wide, cudaStream_t st) {
+    const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(g.m, 2 * (256 / kRowLanes)), (int64_t)sm_count() * 8);
+    few_outputs_kernel<T, sizeof(T) == 2><<<grid, 256, 0, st>>>(g, wide);
+}
 // Bytes of the copy that an operand needs, 0 if it is taken as it is.
 static size_t copy_bytes(int type, const void* at, int64_t stride, int64_t rows, int64_t cols) {
     return is_whole(type, at, stride) ? 0 : padded((size_t)(rows * whole_stride(type, cols)) * operand_bytes(type));
@@ -1858,6 +1953,15 @@ int ashb_linear_forward(int type, const void* x, int64_t x_stride, const float* 
         ASHB_LAUNCH_CHECK();
         return ASHB_OK;
     }
+    if (takes_few_outputs(type, x, x_stride, inputs, outputs)) {
+        const bool wide = is_whole(type, x, x_stride) && is_whole(type, weight, outputs == 1 ? 0 : weight_stride) &&
+                          inputs * operand_bytes(type) % 16 == 0;
+        if (type == ASHB_F32) launch_few_outputs<float>(g, wide, st);
+        else if (type == ASHB_F16) launch_few_outputs<__half>(g, wide, st);
+        else launch_few_outputs<__nv_bfloat16>(g, wide, st);
+        ASHB_LAUNCH_CHECK();
+        return ASHB_OK;
+    }
     const ForwardPlan fp = plan_forward(type, x, x_stride, weight, weight_stride, rows, inputs, outputs);
     ASHB_REQUIRE(fp.total == 0 || (workspace && ((uintptr_t)workspace & 255) == 0 && workspace_bytes >= (int64_t)fp.total),
                  "null, unaligned or small workspace");
@@ -1888,7 +1992,9 @@ int ashb_linear_forward(int type, const void* x, int64_t x_stride, const float* 
 
 int64_t ashb_linear_forward_workspace(int type, const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
                                       int64_t rows, int64_t inputs, int64_t outputs) {
-    if ((!is_value_type(type) && type != ASHB_E4M3_ROWS) || check_sizes(rows, inputs, outputs) != ASHB_OK || rows <= kFewRows) return 0;
+    if ((!is_value_type(type) && type != ASHB_E4M3_ROWS) || check_sizes(rows, inputs, outputs) != ASHB_OK || rows <= kFewRows ||
+        takes_few_outputs(type, x, x_stride, inputs, outputs))
+        return 0;
     return (int64_t)plan_forward(type, x, x_stride, weight, weight_stride, rows, inputs, outputs).total;
 }
 
