@@ -85,7 +85,7 @@ def test_map_formats_refuse():
                           ("int8", {"a": 1, "a_scale": 1}), ("int8", 0)]:
         with pytest.raises(ValueError):
             _value_formats(formats, dims)
-    if not torch.cuda.is_available():       # the checker's stand-in of the native module has no rows in 8 bits
+    if not torch.cuda.is_available():       # a stand-in of the native module has no rows in 8 bits
         with pytest.raises(RuntimeError):
             ash.HashMap(3, 4, 10, "cpu", value_formats="int8")
 

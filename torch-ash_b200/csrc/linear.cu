@@ -1296,11 +1296,11 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const GemmArgs g, bool wi
 
 // ---- few outputs ---------------------------------------------------------------------------------------------------
 // Heads of one to three outputs (a distance, a colour) on narrow rows, and of four in float32 or where rows are no whole 16-byte
-// words: their tiles are nearly empty, and but for four leave value by value.  Four lanes have a row, and two rows at a time, which share the weights that
-// they fetch from L1; with more lanes a row's shuffles and its way out cost more than its products.  The four sums of a row are
+// words: their tiles are nearly empty, and but for four leave value by value.  Four lanes have a row, and two rows at a time,
+// which share the weights that they fetch from L1; with more lanes a row's shuffles and its way out cost more than its products.  The four sums of a row are
 // joined by halves: lanes give two away and keep two, then one, and end with an output each.
-// A million rows of 64 into one output: float32 64 us (tiles 156), bf16 43 (87); into four float32 68 (100); 16 into three 36 (140) and 39 (85); 100k rows of
-// 63 into three 23 (38, a copy to whole rows included) and 19 (28).  Bf16 rows of 64 into four gain nothing (59 against 52), nor do
+// A million rows of 64 into one output: float32 64 us (tiles 156), bf16 43 (87); into four float32 68 (100);
+// 16 into three 36 (140) and 39 (85); 100k rows of 63 into three 23 (38, a copy to whole rows included) and 19 (28).  Bf16 rows of 64 into four gain nothing (59 against 52), nor do
 // wider rows, where four lanes are too few and more do too much beside (162 into four 182 against 152).
 constexpr int kFewOutputs = 4, kNarrowRow = 64, kRowLanes = 4;
 
