@@ -148,22 +148,15 @@ def _distinct_keys(n, dim, g):
     return torch.stack(columns, 1).int() - edge // 2
 
 
-_package = None
-
-
 def _ash():
-    """The package, found and imported once: a program that uses it does not look it up on every pass."""
-    global _package
-    if _package is None:
-        at = os.path.abspath("torch-ash_b200")
-        if at not in sys.path:
-            sys.path.insert(0, at)
-        import ash
-        import ash.mlp
-        import ash.quant
+    at = os.path.abspath("torch-ash_b200")
+    if at not in sys.path:
+        sys.path.insert(0, at)
+    import ash
+    import ash.mlp
+    import ash.quant
 
-        _package = ash
-    return _package
+    return ash
 
 
 def prepare(case, seed):
