@@ -163,3 +163,84 @@ def test_no_wait_ran_out():
     import __ash
 
     assert __ash.layer_timeouts(DEV) == 0
+
+def recorded_case(act, dtype, m, k, n, seed, scale):
+    """Operands, and in 64 bits z, its error as a sum of exact products in float32, act' and act''."""
+    omega = 30.0 if act == "sin" else 1.0
+    x, w, b, _ = make(m, k, n, dtype, seed, residual=False, scale=scale)
+    z = (x.to(lb.D) @ w.to(lb.D).T + b.to(lb.D)).requires_grad_(True)
+    _, d, _, l2 = lb.activation(z, act, omega)
+    d2, = torch.autograd.grad(d.sum(), z) if d.requires_grad else (torch.zeros_like(z),)
+    ez = lb.linear(x.float(), w.float(), b.float(), act, None, omega)[4]
+    return x, w, b, omega, z.detach(), ez, d.detach(), d2, l2
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("act", ["relu", "silu", "gelu", "sin"])
+def test_recorded_gradients(act, dtype):
+    """With create_graph the gradients keep the bounds that they have without: the slope is of the float32 sum, whatever
+    the layer's type.  A sine of frequency 30 on positions, as a network's first layer has it, and layers of the usual scale."""
+    import ash
+
+    for m, k, n, scale in ((300, 3, 40, 0.58), (70, 64, 33, 1.0), (4, 64, 48, 1.0)):
+        x, w, b, omega, *_ = recorded_case(act, dtype, m, k, n, 21, scale)
+        leaves = [t.requires_grad_(True) for t in (x, w, b)]
+        for r in (None, make(m, 1, n, dtype, 23)[3]):
+            dy = make(m, 1, n, dtype, 22)[3]
+            want = lb.backward(x.detach(), w.detach(), b.detach(), act, None, omega, dy, dtype)
+            for create in (False, True):
+                y = ash.fused_linear(x, w, b, act, r, omega)
+                grads = torch.autograd.grad(y, leaves, dy, create_graph=create)
+                for name, got in zip(("x", "weight", "bias"), grads):
+                    lb.assert_within(got.detach(), *want[name], f"grad {name} of {act} {(m, k, n)} recorded {create}")
+
+
+def test_recorded_sums_beyond_float16():
+    """A float16 layer whose sums leave the type's range: the slope is that of the sum, where a rounded one would be NaN."""
+    import ash
+
+    x = torch.full((20, 64), 200.0, device=DEV, dtype=torch.float16)
+    w = torch.full((8, 64), 10.0, device=DEV, dtype=torch.float16)
+    w[::2] *= -1
+    for act in ("silu", "gelu"):
+        leaves = [x.clone().requires_grad_(True), w.clone().requires_grad_(True)]
+        y = ash.fused_linear(*leaves, activation=act)
+        gx, = torch.autograd.grad(y, leaves[0], torch.ones_like(y), create_graph=True)
+        assert torch.equal(gx, torch.full_like(gx, 40.0))      # four outputs with a slope of one, four with none
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("act", ["silu", "gelu", "sin"])
+def test_second_order_of_any_type(act, dtype):
+    """The gradient of sum(v dx) by x and W, v constant, against the formula at bounds that follow its steps."""
+    import ash
+
+    half, own = lb.half(dtype), 32 * lb.STEP
+    for m, k, n, scale in ((300, 3, 40, 0.58), (70, 64, 33, 1.0)):
+        x, w, b, omega, z, ez, d, d2, l2 = recorded_case(act, dtype, m, k, n, 31, scale)
+        g, v = make(m, 1, n, dtype, 32)[3], make(m, 1, k, dtype, 33)[3]
+        leaves = [t.clone().requires_grad_(True) for t in (x, w)]
+        y = ash.fused_linear(*leaves, b, act, omega=omega)
+        gx, = torch.autograd.grad(y, leaves[0], g, create_graph=True)
+        got = torch.autograd.grad((gx * v).sum(), leaves)
+        x, w, g, v = (t.to(lb.D) for t in (x, w, g, v))
+        scale1, scale2 = (omega, omega**2) if act == "sin" else (1.0, 1.0)
+        phase = omega * z.abs() * lb.STEP if act == "sin" else 0.0
+        # act' and act'' by float32 operations of terms up to 1 + z^2, of a sum off by ez; |act'''| is below 2 for these two
+        e1 = l2 * ez + scale1 * (own * (1 + z.abs()) + phase)
+        e2 = (omega**3 if act == "sin" else 2.0) * ez + scale2 * (own * (1 + z * z) + phase)
+        dz, back = g * d, v @ w.T
+        edz = g.abs() * e1 + half * dz.abs() * (1 + half) + lb.smallest(dtype)
+        eback = (lb.sum_steps(k, dtype) + 1) * lb.STEP * (v.abs() @ w.abs().T)      # what comes back to dz, rounded to the type
+        eback = eback * (1 + half) + half * back.abs() + lb.smallest(dtype)
+        gz = g * d2 * back
+        egz = g.abs() * (d2.abs() * eback + e2 * (back.abs() + eback)) + 4 * lb.STEP * gz.abs()
+        final = lambda e, t: e * (1 + half) + half * t.abs() + lb.smallest(dtype)
+        want = gz @ w
+        e = egz @ w.abs() + (lb.sum_steps(n, torch.float32) + 1) * lb.STEP * ((gz.abs() + egz) @ w.abs())
+        lb.assert_within(got[0], want, final(e, want), f"x of {act}")
+        # W is reached by way of z and of the product with dz: two results of the layer's type, and their sum
+        a, c = gz.T @ x, dz.T @ v
+        ea = final(egz.T @ x.abs() + (lb.sum_steps(m, torch.float32) + 16) * lb.STEP * ((gz.abs() + egz).T @ x.abs()), a)
+        ec = final(edz.T @ v.abs() + (lb.sum_steps(m, dtype) + 16) * lb.STEP * ((dz.abs() + edz).T @ v.abs()), c)
+        lb.assert_within(got[1], a + c, final(ea + ec, a + c), f"weight of {act}")
