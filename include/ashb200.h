@@ -35,6 +35,7 @@ extern "C" {
 #define ASHB_ERR_INVALID 1   /* bad argument (dimension, size, null pointer, dtype code) */
 #define ASHB_ERR_CUDA 2      /* a CUDA runtime call failed */
 #define ASHB_ERR_UNSUPPORTED 3
+#define ASHB_ERR_TIMEOUT 4   /* a bounded wait inside an earlier launch ran out: its results are incomplete */
 
 /* Bits of the device-side status word returned by ashb_map_status(). */
 #define ASHB_STATUS_CAPACITY 1u   /* an insert needed more than `capacity` indices; the key was dropped */
@@ -832,10 +833,16 @@ int ashb_linear_backward(int type, const void* dy_dev, const void* slope_dev, in
                          int64_t outputs, void* dx_dev, void* dweight_dev, void* dbias_dev, void* workspace_dev,
                          int64_t workspace_bytes, void* stream);
 
-/* How many waits inside the layer kernels ran out on the current device (0 in a healthy run).  Synchronises. */
+/* In how many CTAs of the layer kernels a wait ran out on the current device since this was last asked (0 in a healthy
+ * run); what such a launch returned is incomplete.  Waits for the device.  The calls above look without waiting: the first
+ * one after it is known, with arguments that are otherwise good, launches nothing and returns ASHB_ERR_TIMEOUT, once. */
 int ashb_layer_timeouts(unsigned int* out);
 
 /* ---------------------------------------------------------------- runtime knobs */
+
+/* Polls that a wait inside the layer kernels may take, up to a microsecond each (negative: the default, 2^22).  For tests of
+ * what a wait that runs out leads to; 0 makes every wait run out that is not over when it begins. */
+int ashb_set_layer_wait_limit(int polls);
 
 /* Selects how ashb_query_backward_forward and ashb_grid_query_backward scatter the embedding
  * gradient: 0 = one vector reduction per lane and corner (default), 1 = lanes of a warp that add to

@@ -147,3 +147,19 @@ def test_library_refuses_cpu_tensors_and_bad_arguments():
     t = shim._RowTable(4096, 4096, 4096, 8, 1, 0)
     assert lib.ashb_read_rows(5, None, 4, ctypes.byref(t), None) == 1
     assert lib.ashb_map_insert_rows(None, p, 3, 0, None, p, None) == 1 and lib.ashb_map_find_rows(None, p, 3, p, p, 0, None, None) == 1
+
+
+def test_waits_that_ran_out_raise(monkeypatch):
+    """check_waits of a stand-in that counts, and the library's knob."""
+    import ash
+
+    asked = []
+    for count in (0, 3):
+        monkeypatch.setattr(ash.mlp, "backend", type("Counts", (), {"layer_timeouts": staticmethod(lambda d: asked.append(d) or count)}))
+        for device in (1, "cuda:1", torch.device("cuda", 1)):
+            if count:
+                with pytest.raises(RuntimeError, match="3 thread blocks on cuda:1"):
+                    ash.mlp.check_waits(device)
+            else:
+                assert ash.mlp.check_waits(device) is None
+    assert asked == [torch.device("cuda", 1)] * 6

@@ -147,6 +147,7 @@ _lib.ashb_linear_backward_workspace.argtypes = [_int, _vp, _vp, _i64, _vp, _i64,
 _lib.ashb_linear_backward_workspace.restype = _i64
 _lib.ashb_linear_backward.argtypes = [_int, _vp, _vp, _int, _vp, _i64, _vp, _i64, _i64, _i64, _i64] + [_vp] * 4 + [_i64, _vp]
 _lib.ashb_layer_timeouts.argtypes = [_vp]
+_lib.ashb_set_layer_wait_limit.argtypes = [_int]
 _lib.ashb_grid_zero_rows.argtypes = [_vp, _int, _vp, _vp, _c.c_double, _vp, _int, _vp, _vp, _i64, _i64, _i64, _vp]
 
 STATUS_CAPACITY, STATUS_PROBE, STATUS_SPIN, STATUS_DUPLICATE = 1, 2, 4, 8
@@ -1771,8 +1772,13 @@ def linear_backward(dy, slope, slope_kind: int, x, weight, want_dx: bool, want_d
 
 
 def layer_timeouts(device) -> int:
-    """How many waits inside the layer kernels ran out on ``device`` (0 in a healthy run)."""
+    """In how many CTAs of the layer kernels a wait ran out on ``device`` since this was last asked (0 in a healthy run)."""
     out = _c.c_uint()
     with torch.cuda.device(device):
         _check(_lib.ashb_layer_timeouts(_c.byref(out)))
     return int(out.value)
+
+
+def set_layer_wait_limit(polls: int) -> None:
+    """Polls that a wait inside the layer kernels may take, negative: the default.  For tests of waits that run out."""
+    _check(_lib.ashb_set_layer_wait_limit(polls))

@@ -170,6 +170,19 @@ def fused_linear(x: Union[torch.Tensor, QuantizedRows], weight: Union[torch.Tens
     return y if flat else y.reshape(shape)
 
 
+def check_waits(device: Union[None, int, str, torch.device] = None) -> None:
+    """Wait for ``device`` (the current one) and raise ``RuntimeError`` if a layer's kernel gave up on a wait there since this was
+    last asked: what that layer returned is incomplete.  The waits inside the kernels are bounded, by seconds where they
+    take microseconds, so that a launch always ends.  Layers called later raise the same without waiting; for work
+    that no call follows, or that a replayed CUDA graph does, ask here."""
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device("cuda", device) \
+        if isinstance(device, int) else torch.device(device)
+    count = backend.layer_timeouts(device)
+    if count:
+        raise RuntimeError(f"waits inside the kernels of dense layers ran out in {count} thread blocks on {device}: what those layers "
+                           "returned is incomplete")
+
+
 def _quantized_linear(x, weight, bias, activation, residual, omega, dtype):
     x.check("x")
     weight.check("weight")

@@ -49,7 +49,15 @@ constexpr size_t kSharedLimit = 232448;
 
 enum Activation { kNone = ASHB_ACT_NONE, kRelu = ASHB_ACT_RELU, kSilu = ASHB_ACT_SILU, kGelu = ASHB_ACT_GELU, kSin = ASHB_ACT_SIN };
 
+// CTAs in which a wait ran out.  What they had left to write is not written, so the host has to learn of it: by this count, for
+// which it waits, and by a word of its own memory, which the next call looks at.
 __device__ unsigned int g_layer_timeouts = 0;
+
+__device__ __noinline__ void tell_timeout(unsigned int* told) {
+    atomicAdd(&g_layer_timeouts, 1u);
+    if (told) *static_cast<volatile unsigned int*>(told) = 1u;
+    __threadfence_system();
+}
 
 // ---- activations -----------------------------------------------------------------------------------------------------
 // Short and without branches, so that a block's 32 values a lane are straight code.  ROUNDED: the results are rounded to 16
@@ -192,6 +200,8 @@ struct GemmArgs {
     int raws;      // split_gemm_kernel: stages of values as they came
     int bulk_out, bufs;      // finishing by bulk copies, from this many blocks in turn
     int64_t finish_bytes;    // of shared memory, a finisher's
+    int polls;               // of a wait
+    unsigned int* told;      // the host's word for waits that ran out (may be null)
 };
 
 __device__ __forceinline__ void put16(uint32_t at, uint4 w) {
@@ -610,7 +620,7 @@ __device__ __forceinline__ void bulk_typed(const GemmArgs& g, uint32_t sums, uin
 template <int KIND, bool FORWARD>
 __device__ __forceinline__ void finish_bulk(const GemmArgs& g, const FinishMaps& maps, int number, int lane, uint32_t tmem,
                                             uint32_t slot_columns, uint32_t sums_full, uint32_t sums_empty, uint32_t scratch,
-                                            uint32_t arrivals, volatile int* gave_up) {
+                                            uint32_t arrivals, const Waits& waits) {
     const int quarter = threadIdx.x >> 5 & 3, n_blocks = (g.bn + 31) >> 5;
     const uint32_t block = g.f.partial || g.f.type == ASHB_F32 ? 4096u : 2048u;
     const uint32_t columns = scratch + block * g.bufs * (g.f.slope ? 2 : 1);
@@ -681,8 +691,8 @@ __device__ __forceinline__ void finish_bulk(const GemmArgs& g, const FinishMaps&
                 __syncwarp();
             }
         }
-        bool ok = bar_wait(sums_full + 8 * slot.at, slot.parity, gave_up);
-        if (fetches && inside) ok = bar_wait(arrivals + 8 * here.at, here.parity, gave_up) && ok;
+        bool ok = bar_wait(sums_full + 8 * slot.at, slot.parity, waits);
+        if (fetches && inside) ok = bar_wait(arrivals + 8 * here.at, here.parity, waits) && ok;
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) {      // the copies still under way end before the CTA does
             if (fetches && inside) bar_drain(arrivals + 8 * here.at, here.parity);
@@ -723,7 +733,7 @@ __device__ __forceinline__ void finish_bulk(const GemmArgs& g, const FinishMaps&
 // there are several phases).  False: a wait gave up.
 template <bool FORWARD>
 __device__ __forceinline__ bool finish_split(const GemmArgs& g, const Tile& t, int phase_blocks, Turn& slot, uint32_t tmem,
-                                             uint32_t sums_full, uint32_t sums_empty, volatile int* gave_up, float* block,
+                                             uint32_t sums_full, uint32_t sums_empty, const Waits& waits, float* block,
                                              int quarter, int which, int lane) {
     const int n_blocks = (g.bn + 31) >> 5;
     const int64_t row0 = (int64_t)t.m * kTileM + quarter * 32, col0 = (int64_t)t.n * g.bn;
@@ -732,7 +742,7 @@ __device__ __forceinline__ bool finish_split(const GemmArgs& g, const Tile& t, i
 #pragma unroll 1
     for (int b0 = 0; b0 < t.blocks; b0 += phase_blocks, slot.next(g.slots)) {
         const bool last = b0 + phase_blocks >= t.blocks;
-        if (!__all_sync(0xffffffffu, bar_wait(sums_full + 8 * slot.at, slot.parity, gave_up))) return false;
+        if (!__all_sync(0xffffffffu, bar_wait(sums_full + 8 * slot.at, slot.parity, waits))) return false;
         tc_fence_after();
         const uint32_t at = tmem + (uint32_t)(slot.at * 2 * g.bn) + ((uint32_t)(quarter * 32) << 16);
 #pragma unroll 1
@@ -781,7 +791,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) layer_gemm_kernel(const GemmA
     const uint32_t base = (smem_of(dynamic) + 1023u) & ~1023u;
     const uint32_t a_bytes = part_bytes<A_DOWN>(kTileM), b_bytes = part_bytes<B_DOWN>(g.bn), stage_bytes = a_bytes + b_bytes;
     float* blocks = reinterpret_cast<float*>(dynamic + (base - smem_of(dynamic)) + (size_t)stage_bytes * g.stages);
-    volatile int* gave_up = &sh.gave_up;
+    const Waits waits{&sh.gave_up, g.polls};
     const uint32_t full = smem_of(sh.full), empty = smem_of(sh.empty);
     const uint32_t sums_full = smem_of(sh.sums_full), sums_empty = smem_of(sh.sums_empty);
 
@@ -814,7 +824,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) layer_gemm_kernel(const GemmA
                 const Tile t = tile_of(g, item);
                 int k = (int)t.k0;
                 for (int b = 0; b < t.blocks; ++b, k += kBlock, turn.next(g.stages)) {
-                    if (!(ok = bar_wait(empty + 8 * turn.at, turn.parity ^ 1u, gave_up))) break;
+                    if (!(ok = bar_wait(empty + 8 * turn.at, turn.parity ^ 1u, waits))) break;
                     const bool with_b = !g.b_stays || fills < g.stages;
                     if (fills < g.stages) ++fills;
                     const uint32_t tile_a = base + (uint32_t)turn.at * stage_bytes, tile_b = tile_a + a_bytes;
@@ -836,12 +846,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1) layer_gemm_kernel(const GemmA
                     }
                 }
             }
-            if (!ok) {      // the copies still under way end before the CTA does
-                for (int i = 0; i < fills; ++i) {
-                    if (turn.at == 0) turn.parity ^= 1u;
-                    turn.at = (turn.at == 0 ? g.stages : turn.at) - 1;
-                    bar_drain(full + 8 * turn.at, turn.parity);
-                }
+            // The copies still under way end before the CTA does: those that it has products for have ended by then, the
+            // others where a wait ran out in whatever role.
+            for (; fills > 0; --fills) {
+                if (turn.at == 0) turn.parity ^= 1u;
+                turn.at = (turn.at == 0 ? g.stages : turn.at) - 1;
+                bar_drain(full + 8 * turn.at, turn.parity);
             }
         }
     } else if (warp == 1) {
@@ -852,11 +862,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1) layer_gemm_kernel(const GemmA
             const Tile t = tile_of(g, item);
             int left = (int)min((int64_t)t.blocks * kBlock, g.k - t.k0);      // values along k
             const uint32_t sums = tmem + (uint32_t)(slot.at * g.bn);
-            if (!(ok = bar_wait(sums_empty + 8 * slot.at, slot.parity ^ 1u, gave_up))) break;
+            if (!(ok = bar_wait(sums_empty + 8 * slot.at, slot.parity ^ 1u, waits))) break;
             tc_fence_after();
             bool add = false;
             for (int b = 0; b < t.blocks; ++b, left -= kBlock, turn.next(g.stages)) {
-                if (!(ok = bar_wait(full + 8 * turn.at, turn.parity, gave_up))) break;
+                if (!(ok = bar_wait(full + 8 * turn.at, turn.parity, waits))) break;
                 tc_fence_after();
                 const int steps = (min(kBlock, left) + kStep - 1) / kStep;
                 const uint32_t tile_a = base + (uint32_t)turn.at * stage_bytes;
@@ -871,16 +881,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1) layer_gemm_kernel(const GemmA
             }
             if (ok) products_done(mine, sums_full + 8 * slot.at);
         }
-        if (!ok) {      // tensor memory is not given back under products still running
-            products_done(mine, smem_of(&sh.drained));
-            bar_drain(smem_of(&sh.drained), 0);
-            if (mine) atomicAdd(&g_layer_timeouts, 1u);
-        }
+        // Tensor memory is not given back, nor shared memory left, under products still running: finishers that gave up have not
+        // waited for them.
+        products_done(mine, smem_of(&sh.drained));
+        bar_drain(smem_of(&sh.drained), 0);
     } else if (warp >= kFirstFinisher && warp < kFirstFinisher + 4 * g.groups) {
         const int number = warp - kFirstFinisher;
         if (g.bulk_out) {
             finish_bulk<KIND, kForward>(g, maps, number, lane, tmem, (uint32_t)g.bn, sums_full, sums_empty,
-                                        smem_of(blocks) + (uint32_t)(number * g.finish_bytes), smem_of(sh.residual) + 16 * number, gave_up);
+                                        smem_of(blocks) + (uint32_t)(number * g.finish_bytes), smem_of(sh.residual) + 16 * number, waits);
         } else {
             // lanes of tensor memory that the warp may read; the blocks of 32 columns go to the groups in turn
             const int quarter = warp & 3, n_blocks = (g.bn + 31) >> 5;
@@ -894,7 +903,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) layer_gemm_kernel(const GemmA
                 const int64_t row0 = (int64_t)t.m * kTileM + quarter * 32, col0 = (int64_t)t.n * g.bn;
                 for (; blk < n_blocks; blk += g.groups) {
                     if (kForward) ahead.fetch(g.f, lane, row0, col0 + blk * 32, g.m, g.n);
-                    ok = __all_sync(0xffffffffu, bar_wait(sums_full + 8 * slot.at, slot.parity, gave_up));
+                    ok = __all_sync(0xffffffffu, bar_wait(sums_full + 8 * slot.at, slot.parity, waits));
                     if (!ok) break;
                     tc_fence_after();
                     float r[32];
@@ -914,6 +923,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) layer_gemm_kernel(const GemmA
     __syncthreads();
     tc_fence_after();
     if (warp == 1) tmem_free(tmem, (uint32_t)g.columns);
+    if (threadIdx.x == 0 && *waits.gave_up) tell_timeout(g.told);
 }
 
 // ---- split products from bulk copies ---------------------------------------------------------------------------------------
@@ -979,7 +989,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) split_gemm_kernel(const GemmA
     const uint32_t raw_bytes = raw_a + (g.b_stays ? 0u : raw_b), stage_bytes = 3 * (a_part + (g.b_stays ? 0u : b_part));
     const uint32_t raws = base, stages = raws + raw_bytes * g.raws, all_b = stages + stage_bytes * g.stages;
     float* blocks = reinterpret_cast<float*>(dynamic + (all_b - smem_of(dynamic)) + (g.b_stays ? (size_t)3 * b_part * g.blocks_k : 0));
-    volatile int* gave_up = &sh.gave_up;
+    const Waits waits{&sh.gave_up, g.polls};
     const uint32_t raw_full = smem_of(sh.raw_full), raw_empty = smem_of(sh.raw_empty), full = smem_of(sh.full),
                    empty = smem_of(sh.empty), sums_full = smem_of(sh.sums_full), sums_empty = smem_of(sh.sums_empty);
 
@@ -1013,7 +1023,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) split_gemm_kernel(const GemmA
             int fills = 0;      // up to the ring's size
             bool ok = true;
             const auto room = [&](uint32_t bytes) {
-                if (!(ok = bar_wait(raw_empty + 8 * raw.at, raw.parity ^ 1u, gave_up))) return false;
+                if (!(ok = bar_wait(raw_empty + 8 * raw.at, raw.parity ^ 1u, waits))) return false;
                 bar_expect(raw_full + 8 * raw.at, bytes);
                 fills = min(fills + 1, g.raws);
                 return true;
@@ -1043,12 +1053,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1) split_gemm_kernel(const GemmA
                     raw.next(g.raws);
                 }
             }
-            if (!ok) {      // the copies still under way end before the CTA does
-                for (int i = 0; i < fills; ++i) {
-                    if (raw.at == 0) raw.parity ^= 1u;
-                    raw.at = (raw.at == 0 ? g.raws : raw.at) - 1;
-                    bar_drain(raw_full + 8 * raw.at, raw.parity);
-                }
+            for (; fills > 0; --fills) {      // the copies still under way end before the CTA does
+                if (raw.at == 0) raw.parity ^= 1u;
+                raw.at = (raw.at == 0 ? g.raws : raw.at) - 1;
+                bar_drain(raw_full + 8 * raw.at, raw.parity);
             }
         }
     } else if (warp == 1) {
@@ -1065,10 +1073,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1) split_gemm_kernel(const GemmA
                 for (int b0 = 0; b0 < t.blocks && ok; slot.next(g.slots)) {
                     const int b1 = min(t.blocks, b0 + kSplitPhase);
                     const uint32_t sums = tmem + (uint32_t)(slot.at * 2 * g.bn), small = sums + (uint32_t)g.bn;
-                    if (!(ok = bar_wait(sums_empty + 8 * slot.at, slot.parity ^ 1u, gave_up))) break;
+                    if (!(ok = bar_wait(sums_empty + 8 * slot.at, slot.parity ^ 1u, waits))) break;
                     bool add = false;
                     for (; b0 < b1; ++b0, left -= kSplitBlock, turn.next(g.stages)) {
-                        if (!(ok = bar_wait(full + 8 * turn.at, turn.parity, gave_up))) break;
+                        if (!(ok = bar_wait(full + 8 * turn.at, turn.parity, waits))) break;
                         tc_fence_after();
                         const uint32_t at = stages + (uint32_t)turn.at * stage_bytes;
                         const uint32_t at_b = g.b_stays ? all_b + (uint32_t)b0 * 3u * b_part : at + 3 * a_part;
@@ -1088,11 +1096,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) split_gemm_kernel(const GemmA
                     if (ok) products_done(mine, sums_full + 8 * slot.at);
                 }
             }
-            if (!ok) {
-                products_done(mine, smem_of(&sh.drained));
-                bar_drain(smem_of(&sh.drained), 0);
-                if (mine) atomicAdd(&g_layer_timeouts, 1u);
-            }
+            products_done(mine, smem_of(&sh.drained));      // as in layer_gemm_kernel
+            bar_drain(smem_of(&sh.drained), 0);
         }
     } else if (warp < 2 + kSplitters) {
         const int thread = threadIdx.x - 64;
@@ -1105,7 +1110,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) split_gemm_kernel(const GemmA
         };
         if (g.b_stays)
             for (int b = 0; b < (int)g.blocks_k && ok; ++b) {
-                ok = __all_sync(0xffffffffu, bar_wait(raw_full + 8 * raw.at, raw.parity, gave_up));
+                ok = __all_sync(0xffffffffu, bar_wait(raw_full + 8 * raw.at, raw.parity, waits));
                 if (!ok) break;
                 split_tile<B_DOWN>(raws + raw.at * raw_bytes, all_b + (uint32_t)b * 3u * b_part, g.bn, thread);
                 tell(raw_empty + 8 * raw.at);
@@ -1114,8 +1119,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) split_gemm_kernel(const GemmA
         for (uint32_t item = blockIdx.x; item < g.items && ok; item += gridDim.x) {
             const Tile t = tile_of(g, item);
             for (int b = 0; b < t.blocks && ok; ++b) {
-                ok = __all_sync(0xffffffffu, bar_wait(empty + 8 * turn.at, turn.parity ^ 1u, gave_up) &&
-                                                     bar_wait(raw_full + 8 * raw.at, raw.parity, gave_up));
+                ok = __all_sync(0xffffffffu, bar_wait(empty + 8 * turn.at, turn.parity ^ 1u, waits) &&
+                                                     bar_wait(raw_full + 8 * raw.at, raw.parity, waits));
                 if (!ok) break;
                 const uint32_t from = raws + raw.at * raw_bytes, to = stages + (uint32_t)turn.at * stage_bytes;
                 split_tile<A_DOWN>(from, to, kTileM, thread);
@@ -1132,12 +1137,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1) split_gemm_kernel(const GemmA
         if (g.bulk_out)
             finish_bulk<kSplit, !A_DOWN && !B_DOWN>(g, maps, warp - 8, lane, tmem, 2u * g.bn, sums_full, sums_empty,
                                                     smem_of(blocks) + (uint32_t)((warp - 8) * g.finish_bytes),
-                                                    smem_of(sh.residual) + 16 * (warp - 8), gave_up);
+                                                    smem_of(sh.residual) + 16 * (warp - 8), waits);
         float* block = blocks + (size_t)(warp - 8) * 1024 * g.places;
         Turn slot;
         for (uint32_t item = blockIdx.x; item < g.items && !g.bulk_out; item += gridDim.x) {
             const Tile t = tile_of(g, item);
-            if (!finish_split<!A_DOWN && !B_DOWN>(g, t, kSplitPhase, slot, tmem, sums_full, sums_empty, gave_up, block, quarter, which,
+            if (!finish_split<!A_DOWN && !B_DOWN>(g, t, kSplitPhase, slot, tmem, sums_full, sums_empty, waits, block, quarter, which,
                                                   lane))
                 break;
         }
@@ -1147,6 +1152,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) split_gemm_kernel(const GemmA
     __syncthreads();
     tc_fence_after();
     if (warp == 1) tmem_free(tmem, (uint32_t)g.columns);
+    if (threadIdx.x == 0 && *waits.gave_up) tell_timeout(g.told);
 }
 
 // ---- rows of whole words ------------------------------------------------------------------------------------------------
@@ -1693,8 +1699,42 @@ static bool finish_maps(FinishMaps* maps, const GemmArgs& g, int64_t splits) {
            (!f.residual || block_map(&maps->residual, f.residual, type, f.residual_stride, g.m, g.n, 1));
 }
 
+static std::atomic<int> g_wait_polls{kWaitPolls};
+constexpr int kToldDevices = 64;
+static std::atomic<unsigned int*> g_told{nullptr};
+
+// The host's words for waits that ran out, one a device, which kernels reach too; null where there is no such memory.
+static unsigned int* told_words() {
+    static unsigned int* words = [] {
+        void* p = nullptr;
+        // a first call may be one that is captured, where allocations are refused unless the thread says it knows
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (cudaHostAlloc(&p, kToldDevices * sizeof(unsigned int), cudaHostAllocPortable | cudaHostAllocMapped) != cudaSuccess) {
+            (void)cudaGetLastError();
+            p = nullptr;
+        }
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (p) std::memset(p, 0, kToldDevices * sizeof(unsigned int));
+        return static_cast<unsigned int*>(p);
+    }();
+    g_told.store(words, std::memory_order_release);
+    return words;
+}
+// Whether a wait has run out in an earlier launch on the current device, as far as is known without waiting: told once.
+static int check_told() {
+    unsigned int* words = g_told.load(std::memory_order_acquire);
+    int device = 0;
+    if (words == nullptr || cudaGetDevice(&device) != cudaSuccess || device >= kToldDevices) return ASHB_OK;
+    volatile unsigned int* word = words + device;
+    if (*word == 0) return ASHB_OK;
+    *word = 0;
+    set_error("a wait inside a kernel of an earlier dense layer ran out: what it returned is incomplete");
+    return ASHB_ERR_TIMEOUT;
+}
+
 template <auto kernel>
-static cudaError_t launch_kernel(const GemmArgs& g, const Plan& p, const CUtensorMap& ma, const CUtensorMap& mb,
+static cudaError_t launch_kernel(GemmArgs g, const Plan& p, const CUtensorMap& ma, const CUtensorMap& mb,
                                  const FinishMaps& maps, cudaStream_t st) {
     // once a kernel and device: a call of the runtime less on every launch
     static std::atomic<uint64_t> told{0};
@@ -1707,6 +1747,9 @@ static cudaError_t launch_kernel(const GemmArgs& g, const Plan& p, const CUtenso
         if (e != cudaSuccess) return e;
         told.fetch_or(bit, std::memory_order_release);
     }
+    unsigned int* words = told_words();
+    g.told = words && device < kToldDevices ? words + device : nullptr;
+    g.polls = g_wait_polls.load(std::memory_order_relaxed);
     kernel<<<(unsigned)std::min<int64_t>(g.items, sm_count()), kGemmThreads, p.shared, st>>>(g, ma, mb, maps);
     return cudaGetLastError();
 }
@@ -1919,6 +1962,7 @@ int ashb_linear_forward(int type, const void* x, int64_t x_stride, const float* 
     if (rows == 0) return ASHB_OK;
     ASHB_REQUIRE(x && weight && y && (!eight || (x_scales && weight_scales)), "null buffer");
     ASHB_REQUIRE((x_stride >= inputs || rows == 1) && weight_stride >= inputs, "rows overlap");
+    if (int rc = check_told()) return rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     GemmArgs g{};
     g.a = Operand{x, x_stride};
@@ -2025,6 +2069,7 @@ int ashb_linear_backward(int type, const void* dy, const void* slope, int slope_
                  "null buffer, or a slope that the slope kind has no use for");
     ASHB_REQUIRE(!dx || weight_stride >= inputs, "rows overlap");
     ASHB_REQUIRE(!dweight || x_stride >= inputs || rows == 1, "rows overlap");
+    if (int rc = check_told()) return rc;
     if (is_small_layer(rows, inputs, outputs)) {
         launch_small_grads(type, SmallGrads{dy, slope, x, weight, dx, dweight, dbias, x_stride, weight_stride, (int)rows, (int)inputs,
                                             (int)outputs, slope_kind, 0}, st);
@@ -2111,7 +2156,19 @@ int ashb_linear_backward(int type, const void* dy, const void* slope, int slope_
 
 int ashb_layer_timeouts(unsigned int* out) {
     ASHB_REQUIRE(out != nullptr, "null output");
+    // of every stream: a copy on the default one does not wait for those that do not wait for it
+    ASHB_CUDA_TRY(cudaDeviceSynchronize());
     ASHB_CUDA_TRY(cudaMemcpyFromSymbol(out, g_layer_timeouts, sizeof(unsigned int)));
+    if (*out != 0) {
+        const unsigned int none = 0;
+        ASHB_CUDA_TRY(cudaMemcpyToSymbol(g_layer_timeouts, &none, sizeof(none)));
+        (void)check_told();
+    }
+    return ASHB_OK;
+}
+
+int ashb_set_layer_wait_limit(int polls) {
+    g_wait_polls.store(polls < 0 ? kWaitPolls : polls, std::memory_order_relaxed);
     return ASHB_OK;
 }
 

@@ -39,17 +39,23 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
 // launch, for the products of one tile, is milliseconds.
 constexpr int kWaitPolls = 1 << 22;
 
+// A CTA's waits: how many polls each may take, and whether one has run out.
+struct Waits {
+    volatile int* gave_up;
+    int polls;
+};
+
 // Waits for phase `parity`.  False once the limit has run out here (`gave_up` is set) or anywhere else in the CTA.
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, const Waits& waits) {
     if (bar_try(bar, parity)) return true;
-    for (int i = 0; i < kWaitPolls; ++i) {
+    for (int i = 0; i < waits.polls; ++i) {
         if (bar_try(bar, parity)) return true;
-        if (*gave_up) return false;
+        if (*waits.gave_up) return false;
     }
-    *gave_up = 1;
+    *waits.gave_up = 1;
     return false;
 }
-// The same after a failure: only the limit ends it.
+// The same for what must end before the CTA does, whatever has failed in it: only the full limit ends it.
 __device__ __forceinline__ void bar_drain(uint32_t bar, uint32_t parity) {
     for (int i = 0; i < kWaitPolls && !bar_try(bar, parity); ++i) {
     }
