@@ -198,3 +198,22 @@ def test_filtered_table():
     want = codes * scale[:, None]
     assert bool(masks[::2].all()) and not bool(masks[1::2].any())
     assert torch.equal(rows[::2], want[::2]) and not bool(rows[1::2].any())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_a_cleared_map_reads_zeros(fmt):
+    """Rows that keys without values are given after clear(), and the buffers themselves, a state's among them."""
+    import ash
+
+    n, width = 500, 20
+    keys, x = keys_of(n, 3, 7), values(n, width, torch.float32, 7)
+    x[::3, 1], x[1::3, 2] = float("inf"), float("nan")
+    m = ash.HashMap(3, width, n, DEV, value_formats=fmt)
+    m.insert(keys, x)
+    m.clear()
+    m.engine.insert_keys(keys)
+    masks, _, rows = m.find(keys, return_values=True)
+    assert bool(masks.all()) and not bool((rows != 0).any())
+    assert not bool((m.items(return_values=True)[2] != 0).any())
+    state = m.state_dict()
+    assert not bool(state["default"].view(torch.uint8).any()) and not bool(state["default_scale"].any())

@@ -157,8 +157,8 @@ class HashMap(ASHModule):
 
     def clear(self) -> None:
         for name, v in self.values.items():
-            if name not in self.value_formats:      # codes read as zeros once their scales are
-                v.zero_()
+            # codes as bytes, their scales beside them: a code that is NaN reads as NaN whatever its scale is
+            (v.view(torch.uint8) if name in self.value_formats else v).zero_()
         self.engine.clear()
 
     def size(self) -> int:
