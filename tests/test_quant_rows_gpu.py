@@ -217,3 +217,25 @@ def test_a_cleared_map_reads_zeros(fmt):
     assert not bool((m.items(return_values=True)[2] != 0).any())
     state = m.state_dict()
     assert not bool(state["default"].view(torch.uint8).any()) and not bool(state["default_scale"].any())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_types_of_rows_stay(fmt):
+    """half(), double() and the like leave the codes and their scales what they are, and the buffers those that the map uses."""
+    import ash
+
+    n, width = 300, 12
+    keys, x = keys_of(n, 3, 9), values(n, width, torch.float32, 9)
+    m = ash.HashMap(3, width, n, DEV, value_formats=fmt)
+    m.insert(keys[:200], x[:200])
+    for change in (lambda: m.half(), lambda: m.double(), lambda: m.bfloat16(), lambda: m.float(),
+                   lambda: torch.nn.ModuleList([m]).half(), lambda: torch.nn.ModuleList([m]).to(torch.float64)):
+        change()
+        assert m.default.dtype == ash.quant.FORMATS[fmt] and m.default_scale.dtype == torch.float32
+        assert m.default is m.values["default"] and m.default_scale is m.values["default_scale"]
+    m.insert(keys[200:], x[200:])
+    codes, scale = plain(x, fmt)
+    assert torch.equal(m.find(keys, return_values=True)[2], codes * scale[:, None])
+    other = ash.HashMap(3, width, n, DEV, value_formats=fmt)
+    other.load_state_dict(m.state_dict())
+    assert torch.equal(other.find(keys, return_values=True)[2], codes * scale[:, None])

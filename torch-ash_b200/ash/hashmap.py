@@ -81,6 +81,16 @@ class HashMap(ASHModule):
         for name, v in new_values.items():
             self.register_buffer(name, v)
 
+    def _apply(self, fn, recurse=True):
+        """half(), double() and the like are about numbers: codes and scales keep their types, and go on being the buffers that
+        the map writes."""
+        kept = {n: self.values[n] for name in self.value_formats for n in (name, name + "_scale")}
+        super()._apply(fn, recurse)
+        for name, v in kept.items():
+            if self._buffers[name] is not v:
+                self._buffers[name] = self.values[name] = v.to(self._buffers[name].device)
+        return self
+
     def _rows(self, name: str) -> QuantizedRows:
         return QuantizedRows(self.values[name], self.values[name + "_scale"])
 
