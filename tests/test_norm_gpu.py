@@ -222,3 +222,106 @@ def test_same_bits_again():
     leaves = [t.requires_grad_(True) for t in (x, w, r)]
     runs = [torch.autograd.grad(ash.rms_norm(x, w, residual=r), leaves, [dy, ds]) for _ in range(3)]
     assert all(torch.equal(a, b) for other in runs[1:] for a, b in zip(runs[0], other))
+
+def far_rows(d, dtype, seed):
+    """Rows whose squares leave the range of float32, with and without smaller values beside them."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    x = torch.randn(9, d, generator=g, device=DEV)
+    big = torch.finfo(dtype).max
+    x[1] *= 1e20
+    x[2] = (x[2] * 1e38).clamp(-3e38, 3e38)
+    x[3] = big
+    x[4] *= 1e-3
+    x[4, d // 2] = big
+    x[6] *= 1e25
+    x[7] = torch.where(x[7] > 0, x[7], -3e19)
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d", [1, 8, 60, 100, 129, 1000, 1024, 4096, 5001, 8192, 9000])
+def test_rows_whose_squares_overflow(d, dtype):
+    """They have a norm like any others, in every form, and gradients."""
+    import ash
+
+    x = far_rows(d, dtype, d)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    w = (1 + 0.2 * torch.randn(d, generator=g, device=DEV)).to(dtype)
+    dy = torch.randn(9, d, generator=g, device=DEV).to(dtype)
+    s, rstd, want = exact(x, w, None)
+    h, f = lb.half(dtype), 2.0**-24
+    rel = f * (steps(d) + 8)
+    # y is (s rstd) w: where s rstd is a float32 subnormal its rounding is half of 2^-149, times w, before y's own
+    tiny = w.to(lb.D).abs() * 2.0**-150
+    own = ((rel + 4 * f) * want.abs() + tiny) * (1 + h) + h * want.abs() + lb.smallest(dtype)
+    lb.assert_within(ash.rms_norm(x, w), want, own, "y")
+    y, total = ash.rms_norm(x, w, residual=torch.zeros_like(x))
+    lb.assert_within(y, want, own, "y of a sum")
+    assert torch.equal(total, x)
+    rows = ash.rms_norm(x, w, quantize=True)
+    scale = (want.abs().amax(1) / 448).clamp_min(2.0**-126)
+    lb.assert_within(rows.scales, scale, scale * f * (steps(d) + 16), "scales")
+    back = rows.codes.to(lb.D) * rows.scales.to(lb.D)[:, None]
+    lb.assert_within(back, want, want.abs() * (2.0**-4 + 4 * rel) + scale[:, None] * (2.0**-10 + 600 * rel), "values")
+    # the factor of a row beyond 2^126 is a subnormal number: half of its last place, 2^-150, on top
+    leaves = [x.requires_grad_(True), w.requires_grad_(True)]
+    gd, wd = dy.to(lb.D), w.detach().to(lb.D)
+    gw, n = gd * wd, s * rstd
+    mean, mag = (gw * n).mean(1, keepdim=True), (gw * n).abs().mean(1, keepdim=True)
+    dx = rstd * (gw - n * mean)
+    er = rel + 2.0**-150 / rstd
+    e = rstd * (gw.abs() * (er + 4 * f) + n.abs() * mag * (4 * er + (steps(d) + 16) * f)) + 4 * f * dx.abs() + 2.0**-148
+    e = e * (1 + h) + h * dx.abs() + lb.smallest(dtype)
+    dw, most = (gd * n).sum(0), ((gd * n).abs() * (er + 80 * f)).sum(0)
+    for create in (False, True):
+        gx, gweight = torch.autograd.grad(ash.rms_norm(x, w), leaves, dy, create_graph=create)
+        lb.assert_within(gx.detach(), dx, e, f"grad x, recorded {create}")
+        lb.assert_within(gweight.detach(), dw, most * (1 + h) + h * dw.abs() + lb.smallest(dtype), f"grad weight, recorded {create}")
+
+
+@pytest.mark.parametrize("d", [8, 100, 129, 4096, 9000])
+def test_rows_whose_squares_vanish(d):
+    """Without an eps a row of tiny values has the norm of any other."""
+    import ash
+
+    g = torch.Generator(device=DEV).manual_seed(d)
+    x = torch.randn(6, d, generator=g, device=DEV)
+    for i, size in enumerate((1.0, 1e-15, 1e-22, 1e-30, 1e-37, 1e-42)):
+        x[i] *= size
+    w = 1 + 0.2 * torch.randn(d, generator=g, device=DEV)
+    _, _, want = exact(x, w, None, 0.0)
+    f = 2.0**-24
+    own = (f * (steps(d) + 8) + 5 * f) * want.abs() + lb.smallest(torch.float32)
+    lb.assert_within(ash.rms_norm(x, w, eps=0.0), want, own, "y")
+    x = x[:4].clone().requires_grad_(True)      # gradients of the smaller ones leave the range
+    dy = torch.randn(4, d, generator=g, device=DEV)
+    s, rstd, _ = exact(x.detach(), w, None, 0.0)
+    gw, n = dy.to(lb.D) * w.to(lb.D), s * rstd
+    dx = rstd * (gw - n * (gw * n).mean(1, keepdim=True))
+    e = rstd * (gw.abs() + n.abs() * (gw * n).abs().mean(1, keepdim=True)) * f * 8 * (steps(d) + 16)
+    for create in (False, True):
+        gx, = torch.autograd.grad(ash.rms_norm(x, w, eps=0.0), x, dy, create_graph=create)
+        lb.assert_within(gx.detach(), dx, e, f"grad x, recorded {create}")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [8, 60, 100, 129, 1000, 4096, 9000])
+def test_an_infinity_or_a_nan_takes_its_row(d, dtype):
+    """All of the row is NaN, in every form and in its gradient; the rows beside it are what they are without it."""
+    import ash
+
+    g = torch.Generator(device=DEV).manual_seed(d)
+    x, w = torch.randn(70, d, generator=g, device=DEV).to(dtype), torch.ones(d, device=DEV, dtype=dtype)
+    plain = ash.rms_norm(x, w)
+    odd = torch.zeros(70, dtype=torch.bool, device=DEV)
+    for row, col, value in ((3, 0, "inf"), (20, d // 2, "-inf"), (21, d - 1, "nan"), (69, d - 1, "inf")):
+        x[row, col] = float(value)
+        odd[row] = True
+    y = ash.rms_norm(x, w)
+    back = ash.dequantize_rows(ash.rms_norm(x, w, quantize=True))
+    assert bool(y[odd].isnan().all()) and bool(back[odd].isnan().all()) and torch.equal(y[~odd], plain[~odd])
+    assert bool(torch.isfinite(back[~odd]).all())
+    x.requires_grad_(True)
+    for create in (False, True):
+        gx, = torch.autograd.grad(ash.rms_norm(x, w).sum(), x, create_graph=create)
+        assert bool(gx[odd].isnan().all()) and bool(torch.isfinite(gx[~odd]).all())

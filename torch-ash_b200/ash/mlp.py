@@ -236,9 +236,12 @@ def _composed_norm_gradients(x, weight, residual, eps, dy, ds):
     """The gradients of x (and the residual) and of the weight, by elementwise operations that autograd records.  Written out:
     asking autograd for those of a composed norm would count what reaches x by way of a residual made from it twice."""
     s, g = x.float() if residual is None else x.float() + residual.float(), dy.float()
-    rstd = torch.rsqrt((s * s).mean(1, keepdim=True) + eps)
-    n, gw = s * rstd, g * weight.float()
-    dx = rstd * (gw - n * (gw * n).mean(1, keepdim=True))
+    # by the row's largest value, or the root of eps if that is larger: squares stay in range, and it cancels
+    size = s.detach().abs().amax(1, keepdim=True).clamp_min(max(math.sqrt(eps), 2.0**-126))
+    t = s / size
+    r = torch.rsqrt((t * t).mean(1, keepdim=True) + eps / size / size)
+    n, gw = t * r, g * weight.float()
+    dx = (gw - n * (gw * n).mean(1, keepdim=True)) * (r / size)
     if ds is not None:
         dx = dx + ds.float()
     return dx.to(x.dtype), (g * n).sum(0).to(weight.dtype)
@@ -250,7 +253,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
     weight``.  Returns y, with a residual ``(y, s)``.
 
     ``quantize``: y comes as ``QuantizedRows`` in e4m3, the operand of ``fused_linear``; that form is for serving and has no
-    gradient.  A row of zeros gives zeros (with an eps of 0 NaN, 0/0); a row that holds an infinity or a NaN gives NaN.
+    gradient.  A row of zeros gives zeros (with an eps of 0 NaN, 0/0); a row that holds an infinity or a NaN gives NaN
+    throughout; one of finite values has its norm, whether their squares are in float32's range or not.
     """
     _check_value(x, "x")
     if x.dim() < 1 or x.shape[-1] < 1:

@@ -4,7 +4,8 @@
 //   s = x + r                                   (r optional; s is an output then)
 //   y = s rstd w,   rstd = (mean(s^2) + eps)^(-1/2)
 //   8 bits: the row's codes and scale by the rules of rowformat.cuh
-//   gradient, with g = dy w:  dx = dr = ds + rstd (g - s rstd^2 mean(g s)),   dw = sum over rows of dy s rstd
+//   gradient, with g = dy w and n = s rstd:  dx = dr = ds + rstd (g - n mean(g n)),   dw = sum over rows of dy n
+// A row that holds an infinity or a NaN is NaN throughout; one whose squares leave float32's range is normed all the same.
 //
 // Everything is memory traffic: each input is read once and each output written once, the row staying in the
 // registers of the lanes that share it between the sum of squares, the largest magnitude and the stores.  Accesses are 16
@@ -66,6 +67,21 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* shared) {
         for (int w = 0; w < TPR / 32; ++w) v = max(v, shared[w]);
     }
     return v;
+}
+
+// Rows whose squares leave the range of float32.  A sum that is not finite, or so small with its eps that squares were lost on
+// the way (2^-100 and less, where a square's last place is 2^-149), is formed again of the row times a power of two that brings
+// its largest value, or the root of eps if that is larger, to 2^40 (as near as 2^127 does): 2^30 squares are far from 2^128, and
+// a value that the factor would make subnormal is 2^-166 of the largest, whose normed value no type holds.
+constexpr float kLeastMean = 0x1p-100f;
+__device__ __forceinline__ bool out_of_range(float mean) { return !(mean >= kLeastMean && mean <= 3.402823466e38f); }     // of eps and all
+__device__ __forceinline__ float row_factor(uint32_t amax, float eps) {
+    const uint32_t field = __float_as_uint(fmaxf(__uint_as_float(amax), sqrtf(eps))) >> 23;      // 0: of a row of zeros too
+    return __uint_as_float(min(294u - min(field, 254u), 254u) << 23);
+}
+// 1 / sqrt(mean + eps) of the row times `factor`; a row that holds an infinity or a NaN has none.
+__device__ __forceinline__ float factored_rstd(uint32_t amax, float squares, int64_t width, float eps, float factor) {
+    return amax >= kInfBits ? __uint_as_float(0x7FC00000u) : 1.0f / sqrtf(squares / (float)width + eps * factor * factor);
 }
 
 // VEC values of a row at p from column `col`, which may begin before the row or end behind it (WINDOW): what is not the row's is
@@ -149,9 +165,33 @@ __global__ void __launch_bounds__(256, NV * VEC <= 16 && !WINDOW ? 8 : 1) norm_f
 #pragma unroll
         for (int k = 0; k < VEC; ++k) squares = fmaf(v[j][k], v[j][k], squares);
     squares = row_sum<TPR>(squares, shared);
-    const float rstd = 1.0f / sqrtf(squares / (float)a.width + a.eps);
-    if (a.rstd != nullptr && live && sub == 0) a.rstd[row] = rstd;
+    const float mean = squares / (float)a.width + a.eps;
+    float rstd = 1.0f / sqrtf(mean), whole = rstd;      // of the values in registers, and of the row
     uint32_t amax = 0;
+    const bool odd = out_of_range(mean);
+    if (TPR > 32 ? odd : __any_sync(0xffffffffu, odd)) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) amax = max(amax, magnitude_bits(v[j][k]));
+        amax = row_max<TPR>(amax, reinterpret_cast<uint32_t*>(shared) + 8);
+        const float factor = odd ? row_factor(amax, a.eps) : 1.0f;
+        squares = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) {
+                v[j][k] *= factor;
+                squares = fmaf(v[j][k], v[j][k], squares);
+            }
+        squares = row_sum<TPR>(squares, shared);
+        if (odd) {
+            rstd = factored_rstd(amax, squares, a.width, a.eps, factor);
+            whole = rstd * factor;
+        }
+        amax = 0;
+    }
+    if (a.rstd != nullptr && live && sub == 0) a.rstd[row] = whole;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const int col = column(j);
@@ -217,11 +257,24 @@ __global__ void __launch_bounds__(256) norm_forward_long_kernel(const NormArgs a
         squares = fmaf(v, v, squares);
     }
     squares = row_sum<256>(squares, shared);
-    const float rstd = 1.0f / sqrtf(squares / (float)a.width + a.eps);
-    if (a.rstd != nullptr && threadIdx.x == 0) a.rstd[row] = rstd;
+    const float mean = squares / (float)a.width + a.eps;
+    float rstd = 1.0f / sqrtf(mean), factor = 1.0f;
     uint32_t amax = 0;
+    if (out_of_range(mean)) {
+        for (int64_t c = threadIdx.x; c < a.width; c += 256) amax = max(amax, magnitude_bits(value(c)));
+        amax = row_max<256>(amax, reinterpret_cast<uint32_t*>(shared) + 8);
+        factor = row_factor(amax, a.eps);
+        squares = 0.0f;
+        for (int64_t c = threadIdx.x; c < a.width; c += 256) {
+            const float v = value(c) * factor;
+            squares = fmaf(v, v, squares);
+        }
+        rstd = factored_rstd(amax, row_sum<256>(squares, shared), a.width, a.eps, factor);
+        amax = 0;
+    }
+    if (a.rstd != nullptr && threadIdx.x == 0) a.rstd[row] = rstd * factor;
     for (int64_t c = threadIdx.x; c < a.width; c += 256) {
-        const float v = value(c), y = v * rstd * to_float(w[c]);
+        const float v = value(c), y = v * factor * rstd * to_float(w[c]);
         amax = max(amax, magnitude_bits(y));
         if constexpr (!QUANT) {
             static_cast<T*>(a.y)[row * a.width + c] = from_float<T>(y);
@@ -234,7 +287,7 @@ __global__ void __launch_bounds__(256) norm_forward_long_kernel(const NormArgs a
         if (threadIdx.x == 0) a.scales[row] = q.scale;
         for (int64_t c = threadIdx.x; c < a.width; c += 256) {
             const float v = value(c);
-            const float u[4] = {v * rstd * to_float(w[c]), 0.0f, 0.0f, 0.0f};
+            const float u[4] = {v * factor * rstd * to_float(w[c]), 0.0f, 0.0f, 0.0f};
             a.codes[row * a.width + c] = (uint8_t)encode4(u, q.inverse, kFormatE4M3);
             if (r) static_cast<T*>(a.sum)[row * a.width + c] = from_float<T>(v);
         }
@@ -291,7 +344,8 @@ __global__ void __launch_bounds__(256, NV * VEC <= 8 ? 4 : NV * VEC <= 16 ? 3 : 
                 load_weights<WINDOW, T, VEC>(w, col, width, u);
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) {
-                    dw[j][k] = fmaf(g[j][k] * s[j][k], rstd, dw[j][k]);
+                    s[j][k] *= rstd;      // before it is multiplied: the normed value is in range whatever s is
+                    dw[j][k] = fmaf(g[j][k], s[j][k], dw[j][k]);
                     g[j][k] *= u[k];
                     dot = fmaf(g[j][k], s[j][k], dot);
                 }
@@ -300,7 +354,7 @@ __global__ void __launch_bounds__(256, NV * VEC <= 8 ? 4 : NV * VEC <= 16 ? 3 : 
         // the sums of two rows in turn go through different words: no second barrier
         dot = row_sum<TPR>(dot, shared + 8 * turn);
         turn ^= 1;
-        const float c = rstd * rstd * (dot / (float)a.width);
+        const float c = dot / (float)a.width;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int col = column(j);
@@ -342,15 +396,15 @@ __global__ void __launch_bounds__(256) norm_backward_long_kernel(const NormGradA
         const float rstd = a.rstd[row];
         float dot = 0.0f;
         for (int64_t c = threadIdx.x; c < a.width; c += 256) {
-            const float sv = to_float(s[c]), dv = to_float(dy[c]);
-            sums[c] = fmaf(dv * sv, rstd, sums[c]);
-            dot = fmaf(dv * to_float(w[c]), sv, dot);
+            const float n = to_float(s[c]) * rstd, dv = to_float(dy[c]);
+            sums[c] = fmaf(dv, n, sums[c]);
+            dot = fmaf(dv * to_float(w[c]), n, dot);
         }
         dot = row_sum<256>(dot, shared + 8 * turn);
         turn ^= 1;
-        const float q = rstd * rstd * (dot / (float)a.width);
+        const float q = dot / (float)a.width;
         for (int64_t c = threadIdx.x; c < a.width; c += 256) {
-            const float d = rstd * fmaf(-to_float(s[c]), q, to_float(dy[c]) * to_float(w[c]));
+            const float d = rstd * fmaf(-to_float(s[c]) * rstd, q, to_float(dy[c]) * to_float(w[c]));
             static_cast<T*>(a.dx)[row * a.width + c] = from_float<T>(ds ? to_float(ds[c]) + d : d);
         }
     }
