@@ -244,3 +244,23 @@ def test_second_order_of_any_type(act, dtype):
         ea = final(egz.T @ x.abs() + (lb.sum_steps(m, torch.float32) + 16) * lb.STEP * ((gz.abs() + egz).T @ x.abs()), a)
         ec = final(edz.T @ v.abs() + (lb.sum_steps(m, dtype) + 16) * lb.STEP * ((dz.abs() + edz).T @ v.abs()), c)
         lb.assert_within(got[1], a + c, final(ea + ec, a + c), f"weight of {act}")
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n", [(4, 8), (2000, 8), (2000, 1), (2000, 40)])
+def test_gelu_of_negative_sums(m, n, dtype):
+    """The tail keeps its leading bits: value and slope relative to the terms that they are made of.  In 16 bits erfc's own
+    formula is good to 2^-15 and the exponential of z^2 / 2 < 72 to 2^-15; in float32 a rounded argument costs z^2 steps."""
+    import ash
+
+    z = torch.linspace(-12, -0.5, m, device=DEV).to(dtype)[:, None].requires_grad_(True)
+    y = ash.fused_linear(z, torch.ones(n, 1, device=DEV, dtype=dtype), activation="gelu")
+    dz, = torch.autograd.grad(y[:, 0].sum(), z)
+    again, = torch.autograd.grad(ash.fused_linear(z, torch.ones(n, 1, device=DEV, dtype=dtype), activation="gelu")[:, 0].sum(), z,
+                                 create_graph=True)
+    zd = z.detach().to(lb.D)
+    c, d = 0.5 * torch.erfc(-zd / 2**0.5), zd * torch.exp(-zd * zd / 2) / (2 * torch.pi) ** 0.5
+    rel = 2.0**-14 if dtype != torch.float32 else (16 + 4 * zd * zd) * 2.0**-24
+    final = lambda e, t: e * (1 + lb.half(dtype)) + lb.half(dtype) * t.abs() + lb.smallest(dtype) + lb.TINY
+    lb.assert_within(y.detach(), (zd * c).expand(m, n), final(rel * (zd * c).abs(), zd * c).expand(m, n), "gelu")
+    for got in (dz, again.detach()):      # the slope is kept in the layer's type, dz and dx are the same value then
+        lb.assert_within(got, c + d, final(rel * (c.abs() + d.abs()), c + d), "its slope")

@@ -84,7 +84,7 @@ def _slope(z: torch.Tensor, activation: str, omega: float) -> torch.Tensor:
         p = torch.sigmoid(z)
         return p * (1 + z * (1 - p))
     if activation == "gelu":
-        return 0.5 * (1 + torch.erf(z * math.sqrt(0.5))) + z * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
+        return 0.5 * torch.erfc(z * -math.sqrt(0.5)) + z * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
     return omega * torch.cos(omega * z)
 
 
