@@ -325,3 +325,32 @@ def test_an_infinity_or_a_nan_takes_its_row(d, dtype):
     for create in (False, True):
         gx, = torch.autograd.grad(ash.rms_norm(x, w).sum(), x, create_graph=create)
         assert bool(gx[odd].isnan().all()) and bool(torch.isfinite(gx[~odd]).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_every_width_has_a_kernel(dtype):
+    """Both sides of every width at which threads a row or accesses a thread change, rows whole and as columns of wider ones."""
+    import ash
+
+    edges = (1, 2, 4, 8, 16, 32, 64, 128, 256, 512, 1024, 2048, 4096, 8192)
+    g = torch.Generator(device=DEV).manual_seed(2)
+    h, f = lb.half(dtype), 2.0**-24
+    for d in sorted({e + o for e in edges for o in (-8, -7, -4, -3, -1, 0, 1) if e + o > 0}):
+        wide = torch.randn(3, d + 1, generator=g, device=DEV).to(dtype)
+        w, dy = (1 + 0.2 * torch.randn(d, generator=g, device=DEV)).to(dtype), torch.randn(3, d, generator=g, device=DEV).to(dtype)
+        for x in (wide[:, :d].clone(), wide[:, 1:]):
+            s, rstd, want = exact(x, w, None)
+            rel = f * (steps(d) + 8)
+            x = x.requires_grad_(True)
+            y = ash.rms_norm(x, w)
+            lb.assert_within(y.detach(), want, (rel + 4 * f) * want.abs() * (1 + h) + h * want.abs() + lb.smallest(dtype), f"y {d}")
+            dx, = torch.autograd.grad(y, x, dy)
+            gw, n = dy.to(lb.D) * w.to(lb.D), s * rstd
+            want = rstd * (gw - n * (gw * n).mean(1, keepdim=True))
+            e = rstd * (gw.abs() + n.abs() * (gw * n).abs().mean(1, keepdim=True)) * 4 * f * (steps(d) + 8)
+            lb.assert_within(dx, want, e * (1 + h) + h * want.abs() + lb.smallest(dtype), f"grad {d}")
+            rows = ash.rms_norm(x.detach(), w, quantize=True)
+            assert torch.equal(ash.quantize_rows(y.detach()).scales.isfinite(), rows.scales.isfinite())
+            back = rows.codes.to(lb.D) * rows.scales.to(lb.D)[:, None]
+            scale = (s * rstd * w.to(lb.D)).abs().amax(1, keepdim=True) / 448
+            lb.assert_within(back, s * rstd * w.to(lb.D), (s * rstd * w.to(lb.D)).abs() * (2.0**-4 + 4 * rel) + scale * (2.0**-10 + 600 * rel), f"codes {d}")

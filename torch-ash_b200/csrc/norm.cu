@@ -415,42 +415,41 @@ constexpr int64_t kLongRow = 8192;
 
 // Threads a row and accesses a thread for a width: as few threads as keep 32 values or less each, so that narrow rows
 // leave no lane idle; the largest NV of a vector width is 32 / VEC.  A window may be a word longer than its row.
+constexpr int64_t kNarrowRow = 64, kWideRow = 1024;      // of eight threads and of a warp at most
 static int threads_of(int64_t width, int vec, bool window) {
     const int64_t most = width + (window ? vec - 1 : 0);
-    return most <= 64 ? 8 : most <= 1024 ? 32 : 256;
+    return most <= kNarrowRow ? 8 : most <= kWideRow ? 32 : 256;
 }
-template <class F>
-static void by_width(int64_t width, int vec, bool window, F&& f) {
-    const int tpr = threads_of(width, vec, window);
+// Whether rows of any width have TPR threads with NV accesses of VEC values, so that only those are compiled.
+constexpr bool is_taken(int vec, int tpr, int nv) {
+    const int64_t above = tpr == 8 ? 0 : tpr == 32 ? kNarrowRow : kWideRow, most = tpr == 8 ? kNarrowRow : tpr == 32 ? kWideRow : kLongRow;
+    const int64_t covers = (int64_t)nv * vec * tpr;
+    return covers > above && (nv == 1 || covers / 2 < most);
+}
+template <int VEC, int TPR, int NV, class F>
+static void by_accesses(int nv, F&& f) {
+    if constexpr (is_taken(VEC, TPR, NV))
+        if (nv == NV) f(std::integral_constant<int, NV>{});
+    if constexpr (NV < 32) by_accesses<VEC, TPR, 2 * NV>(nv, f);
+}
+template <int VEC, bool WINDOW, class F>
+static void by_width(int64_t width, F&& f) {
+    const int tpr = threads_of(width, VEC, WINDOW);
     int nv = 1;
-    while ((int64_t)nv * vec * tpr < width + (window ? vec - 1 : 0)) nv <<= 1;
-    f(tpr, nv);
-}
-
-template <class T, int VEC, int TPR, bool QUANT, bool WINDOW>
-static void launch_forward(const NormArgs& a, int nv, cudaStream_t st) {
-    const unsigned grid = (unsigned)((a.rows + 256 / TPR - 1) / (256 / TPR));
-    switch (nv) {
-        case 1: norm_forward_kernel<T, VEC, TPR, 1, QUANT, WINDOW><<<grid, 256, 0, st>>>(a); break;
-        case 2: norm_forward_kernel<T, VEC, TPR, 2, QUANT, WINDOW><<<grid, 256, 0, st>>>(a); break;
-        case 4: norm_forward_kernel<T, VEC, TPR, 4, QUANT, WINDOW><<<grid, 256, 0, st>>>(a); break;
-        default:
-            if constexpr (VEC <= 4) {
-                if (nv == 8) { norm_forward_kernel<T, VEC, TPR, 8, QUANT, WINDOW><<<grid, 256, 0, st>>>(a); break; }
-            }
-            if constexpr (VEC == 1 && TPR >= 32) {
-                if (nv == 16) { norm_forward_kernel<T, VEC, TPR, 16, QUANT, WINDOW><<<grid, 256, 0, st>>>(a); break; }
-                norm_forward_kernel<T, VEC, TPR, 32, QUANT, WINDOW><<<grid, 256, 0, st>>>(a);
-            }
-    }
+    while ((int64_t)nv * VEC * tpr < width + (WINDOW ? VEC - 1 : 0)) nv <<= 1;
+    const auto with = [&](auto threads) {
+        by_accesses<VEC, decltype(threads)::value, 1>(nv, [&](auto accesses) { f(threads, accesses); });
+    };
+    if (tpr == 8) with(std::integral_constant<int, 8>{});
+    else if (tpr == 32) with(std::integral_constant<int, 32>{});
+    else with(std::integral_constant<int, 256>{});
 }
 
 template <class T, int VEC, bool QUANT, bool WINDOW>
 static void forward_by_width(const NormArgs& a, cudaStream_t st) {
-    by_width(a.width, VEC, WINDOW, [&](int tpr, int nv) {
-        if (tpr == 8) launch_forward<T, VEC, 8, QUANT, WINDOW>(a, nv, st);
-        else if (tpr == 32) launch_forward<T, VEC, 32, QUANT, WINDOW>(a, nv, st);
-        else launch_forward<T, VEC, 256, QUANT, WINDOW>(a, nv, st);
+    by_width<VEC, WINDOW>(a.width, [&](auto threads, auto accesses) {
+        constexpr int TPR = decltype(threads)::value, NV = decltype(accesses)::value;
+        norm_forward_kernel<T, VEC, TPR, NV, QUANT, WINDOW><<<(unsigned)((a.rows + 256 / TPR - 1) / (256 / TPR)), 256, 0, st>>>(a);
     });
 }
 
@@ -491,24 +490,6 @@ static unsigned backward_ctas(int64_t rows, int64_t width) {
     return (unsigned)(groups == 1 ? (ctas + 7) / 8 * 8 : ctas);
 }
 
-template <class T, int VEC, int TPR, bool WINDOW>
-static void launch_backward(const NormGradArgs& a, int nv, unsigned grid, cudaStream_t st) {
-    const size_t smem = (size_t)a.width * 4;
-    switch (nv) {
-        case 1: norm_backward_kernel<T, VEC, TPR, 1, WINDOW><<<grid, 256, smem, st>>>(a); break;
-        case 2: norm_backward_kernel<T, VEC, TPR, 2, WINDOW><<<grid, 256, smem, st>>>(a); break;
-        case 4: norm_backward_kernel<T, VEC, TPR, 4, WINDOW><<<grid, 256, smem, st>>>(a); break;
-        default:
-            if constexpr (VEC <= 4) {
-                if (nv == 8) { norm_backward_kernel<T, VEC, TPR, 8, WINDOW><<<grid, 256, smem, st>>>(a); break; }
-            }
-            if constexpr (VEC == 1 && TPR >= 32) {
-                if (nv == 16) { norm_backward_kernel<T, VEC, TPR, 16, WINDOW><<<grid, 256, smem, st>>>(a); break; }
-                norm_backward_kernel<T, VEC, TPR, 32, WINDOW><<<grid, 256, smem, st>>>(a);
-            }
-    }
-}
-
 template <class T>
 static void backward_typed(const NormGradArgs& a, unsigned grid, void* dw, cudaStream_t st) {
     constexpr int kVec = 16 / sizeof(T);
@@ -519,10 +500,9 @@ static void backward_typed(const NormGradArgs& a, unsigned grid, void* dw, cudaS
         const auto go = [&](auto vec, auto window) {
             constexpr int VEC = decltype(vec)::value;
             constexpr bool WINDOW = decltype(window)::value;
-            by_width(a.width, VEC, WINDOW, [&](int tpr, int nv) {
-                if (tpr == 8) launch_backward<T, VEC, 8, WINDOW>(a, nv, grid, st);
-                else if (tpr == 32) launch_backward<T, VEC, 32, WINDOW>(a, nv, grid, st);
-                else launch_backward<T, VEC, 256, WINDOW>(a, nv, grid, st);
+            by_width<VEC, WINDOW>(a.width, [&](auto threads, auto accesses) {
+                norm_backward_kernel<T, VEC, decltype(threads)::value, decltype(accesses)::value, WINDOW>
+                        <<<grid, 256, (size_t)a.width * 4, st>>>(a);
             });
         };
         if (based && a.width % kVec == 0) go(std::integral_constant<int, kVec>{}, std::false_type{});
