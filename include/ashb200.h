@@ -811,7 +811,8 @@ int ashb_rms_norm_backward(int dtype, const void* dy_dev, const void* dsum_dev, 
  * (values), y [rows][outputs] contiguous; bias [outputs] and residual may be NULL.  type: ASHB_F32, ASHB_F16, ASHB_BF16 --
  * of x, weight, bias, residual and y alike -- or ASHB_E4M3_ROWS: x and weight are e4m3 codes with x_scales [rows] and
  * weight_scales [outputs], bias, residual and y of out_type.  Sums are float32 (float32 operands are multiplied as exact
- * sums of three bf16 parts).  slope (may be NULL): act'(z) [rows][outputs] in y's type, for the backward pass. */
+ * sums of three bf16 parts).  slope (may be NULL): act'(z) [rows][outputs] for the backward pass, in float32; relu's, which is 1
+ * or 0, in y's type. */
 int ashb_linear_forward(int type, const void* x_dev, int64_t x_stride, const float* x_scales_dev, const void* weight_dev,
                         int64_t weight_stride, const float* weight_scales_dev, const void* bias_dev, const void* residual_dev,
                         int64_t residual_stride, int64_t rows, int64_t inputs, int64_t outputs, int activation, float omega,
@@ -823,7 +824,8 @@ int64_t ashb_linear_forward_workspace(int type, const void* x_dev, int64_t x_str
 
 /* Gradients of the same from dy [rows][outputs] (contiguous): dx [rows][inputs], dweight [outputs][inputs] and dbias
  * [outputs], each NULL where not wanted (the residual's is dy).  slope_kind 0: no activation, slope NULL; 1: slope holds
- * act'(z); 2: relu without a residual, slope is the output y.  Sums run in a fixed order.  _workspace: bytes of device
+ * act'(z) in float32; 2: relu, slope is its slope or, without a residual, the output y.  dz = dy act'(z) is rounded to
+ * `type`, whose products are taken of it (not in layers of up to 256 rows and outputs).  Sums run in a fixed order.  _workspace: bytes of device
  * scratch (256-byte aligned). */
 int64_t ashb_linear_backward_workspace(int type, const void* dy_dev, const void* x_dev, int64_t x_stride, const void* weight_dev,
                                        int64_t weight_stride, int64_t rows, int64_t inputs, int64_t outputs, int slope_kind,

@@ -264,3 +264,28 @@ def test_gelu_of_negative_sums(m, n, dtype):
     lb.assert_within(y.detach(), (zd * c).expand(m, n), final(rel * (zd * c).abs(), zd * c).expand(m, n), "gelu")
     for got in (dz, again.detach()):      # the slope is kept in the layer's type, dz and dx are the same value then
         lb.assert_within(got, c + d, final(rel * (c.abs() + d.abs()), c + d), "its slope")
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("act", ["relu", "silu", "gelu", "sin"])
+def test_slopes_are_not_rounded(act, dtype):
+    """One rounding of dz = dy act'(z): with rows of the unit matrix for weights dx is dz, and half a step of its type is all
+    that it may be off by, beside the activation's own error.  Every way that sums leave by, and both backward passes."""
+    import ash
+
+    omega = 2.0 if act == "sin" else 1.0
+    for i, (m, k, n) in enumerate(((4, 8, 8), (200, 8, 8), (3000, 8, 3), (3000, 16, 16), (3000, 33, 9), (64, 4096, 40), (50_000, 64, 64),
+                                   (700, 300, 290), (2000, 1024, 512))):
+        x, _, _, r = make(m, k, n, dtype, 400 + i, residual=act == "relu" and i % 2 == 0)
+        dy = make(m, 1, n, dtype, 500 + i)[3]
+        w = torch.eye(n, k, device=DEV, dtype=dtype)
+        x.requires_grad_(True)
+        dx, = torch.autograd.grad(ash.fused_linear(x, w, activation=act, residual=r, omega=omega), x, dy)
+        z, g = x.detach()[:, :n].to(lb.D), dy.to(lb.D)
+        _, d, _, _ = lb.activation(z, act, omega)
+        assert not bool(dx[:, n:].any())
+        if act == "relu":
+            assert torch.equal(dx[:, :n], torch.where(x[:, :n] > 0, dy, 0))
+            continue
+        own = (8 * lb.STEP if dtype == torch.float32 else 2.0**-19) * (1 + d.abs() + z.abs()) * omega + omega * omega * z.abs() * lb.STEP
+        e = g.abs() * own + 4 * lb.STEP * (g * d).abs()
+        lb.assert_within(dx[:, :n], g * d, e * (1 + lb.half(dtype)) + lb.half(dtype) * (g * d).abs() + lb.smallest(dtype), f"{act} {(m, k, n)}")

@@ -1729,7 +1729,8 @@ def linear_forward(x, weight, bias, activation: str, residual, omega: float, wit
         kind, out_kind = _E4M3_ROWS, _VALUE_TYPES[out_dtype]
         y = x.new_empty((rows, outputs), dtype=out_dtype)
         x_scales, w_scales = _cuda(scales[0], "x.scales"), _cuda(scales[1], "weight.scales")
-    slope = torch.empty_like(y) if with_slope else None
+    # float32, that dz is rounded once; relu's is 1 or 0 in any type
+    slope = None if not with_slope else torch.empty_like(y) if activation == "relu" else y.new_empty((rows, outputs), dtype=torch.float32)
     if rows == 0:
         return y, slope
     at, w_at, workspace, nbytes = x.data_ptr(), weight.data_ptr(), None, 0

@@ -98,7 +98,7 @@ class _FusedLinear(torch.autograd.Function):
         with_slope = activation != "none" and not sign
         y, slope = backend.linear_forward(x, weight, bias, activation, residual, omega, with_slope)
         ctx.activation, ctx.omega = activation, omega
-        ctx.kind = 0 if activation == "none" else 2 if sign else 1
+        ctx.kind = 0 if activation == "none" else 2 if activation == "relu" else 1      # relu: by sign
         ctx.has_bias = bias is not None
         ctx.save_for_backward(x, weight, bias, y if sign else slope)
         return y

@@ -140,6 +140,11 @@ __device__ __forceinline__ float activate_one(float omega, float z, float& slope
     }
 }
 
+// What a slope is kept as for the backward pass: in float32, so that dz is rounded once (in 16 bits as well the gradients of a
+// wide float16 layer are off by 3.7e-4 of their norm, 2.9e-4 so); relu's is one or zero in any type, and read by its sign.
+template <class T, int ACT>
+using SlopeOf = std::conditional_t<ACT == kRelu, T, float>;
+
 // N values in place and their slopes.  Long phases are looked for once for all of them: a branch per value would keep the
 // values from being worked on side by side.
 template <int ACT, bool SLOPE, bool ROUNDED, int N>
@@ -192,7 +197,7 @@ struct Operand {
 struct Finish {          // what becomes of the sums
     const float *a_scales, *b_scales;      // e4m3: of the rows of A and B
     const void *bias, *residual;           // of out's type
-    void *out, *slope;
+    void *out, *slope;                     // slope: SlopeOf
     float* partial;                        // float32 sums instead of out: [splits][m][n]
     int64_t residual_stride;
     int type, activation, wide;            // of out; quadruples are aligned everywhere
@@ -211,6 +216,7 @@ struct GemmArgs {
     int raws;      // split_gemm_kernel: stages of values as they came
     int bulk_out, bufs;      // finishing by bulk copies, from this many blocks in turn
     int64_t finish_bytes;    // of shared memory, a finisher's
+    uint32_t slope_bytes;    // of a block of slopes there
     int polls;               // of a wait
     unsigned int* told;      // the host's word for waits that ran out (may be null)
 };
@@ -342,7 +348,8 @@ __device__ __forceinline__ void finish_wide(const Finish& f, const float* block,
     }
     const int left = (int)min((int64_t)32, m - row0) - sub;      // of this lane's rows, four apart
     T* out = static_cast<T*>(f.out) + (row0 + sub) * n + col;
-    T* slopes = SLOPE ? static_cast<T*>(f.slope) + (row0 + sub) * n + col : nullptr;
+    using S = SlopeOf<T, ACT>;
+    S* slopes = SLOPE ? static_cast<S*>(f.slope) + (row0 + sub) * n + col : nullptr;
     const T* residual = f.residual ? static_cast<const T*>(f.residual) + (row0 + sub + 16) * f.residual_stride + col : nullptr;
     const float* scale = f.b_scales ? f.a_scales + row0 + sub : nullptr;
     // rows sub and sub + 4 of every eight: two places in the block, a round 8 rows on
@@ -387,7 +394,7 @@ __device__ __forceinline__ void finish_wide(const Finish& f, const float* block,
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
             if (in + 4 * p < left) {
-                if (SLOPE) store_n<T, 4>(slopes + 4 * p * n, d[p]);
+                if (SLOPE) store_n<S, 4>(slopes + 4 * p * n, d[p]);
                 store_n<T, 4>(out + 4 * p * n, z[p]);
             }
         }
@@ -406,7 +413,8 @@ __device__ __forceinline__ void finish_narrow(const Finish& f, const float* bloc
     const float b = f.bias ? to_float(static_cast<const T*>(f.bias)[col]) : 0.0f, sb = f.b_scales ? f.b_scales[col] : 1.0f;
     const int left = (int)min((int64_t)32, m - row0);
     T* out = static_cast<T*>(f.out) + row0 * n + col;
-    T* slopes = SLOPE ? static_cast<T*>(f.slope) + row0 * n + col : nullptr;
+    using S = SlopeOf<T, ACT>;
+    S* slopes = SLOPE ? static_cast<S*>(f.slope) + row0 * n + col : nullptr;
     const T* residual = f.residual ? static_cast<const T*>(f.residual) + row0 * f.residual_stride + col : nullptr;
 #pragma unroll 1
     for (int first = 0; first < left; first += 8) {
@@ -423,7 +431,7 @@ __device__ __forceinline__ void finish_narrow(const Finish& f, const float* bloc
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             if (first + i < left) {
-                if (SLOPE) *slopes = from_float<T>(d[i]);
+                if (SLOPE) *slopes = from_float<S>(d[i]);
                 *out = from_float<T>(z[i] + r[i]);
             }
             out += n;
@@ -576,7 +584,8 @@ template <int KIND, class T, int ACT, bool SLOPE>
 __device__ __forceinline__ void bulk_block(const GemmArgs& g, uint32_t sums, uint32_t out, uint32_t slope, uint32_t columns, float row_scale,
                                            int lane) {
     const bool has_residual = g.f.residual != nullptr, has_bias = g.f.bias != nullptr;
-    const uint32_t out_row = out + (uint32_t)lane * (32 * sizeof(T)), slope_row = slope + (uint32_t)lane * (32 * sizeof(T));
+    using S = SlopeOf<T, ACT>;
+    const uint32_t out_row = out + (uint32_t)lane * (32 * sizeof(T)), slope_row = slope + (uint32_t)lane * (32 * sizeof(S));
 #pragma unroll 1
     for (int j = 0; j < 4; ++j) {
         float z[8], d[8];
@@ -601,7 +610,7 @@ __device__ __forceinline__ void bulk_block(const GemmArgs& g, uint32_t sums, uin
             for (int k = 0; k < 8; ++k) z[k] += __uint_as_float(w[k]);
         }
         activate<ACT, SLOPE, sizeof(T) == 2>(g.f.omega, z, d);
-        if (SLOPE) put_eight<T>(slope_row, lane, j, d);
+        if (SLOPE) put_eight<S>(slope_row, lane, j, d);
         if (has_residual) add_eight<T>(out_row, lane, j, z);
         put_eight<T>(out_row, lane, j, z);
     }
@@ -634,7 +643,7 @@ __device__ __forceinline__ void finish_bulk(const GemmArgs& g, const FinishMaps&
                                             uint32_t arrivals, const Waits& waits) {
     const int quarter = threadIdx.x >> 5 & 3, n_blocks = (g.bn + 31) >> 5;
     const uint32_t block = g.f.partial || g.f.type == ASHB_F32 ? 4096u : 2048u;
-    const uint32_t columns = scratch + block * g.bufs * (g.f.slope ? 2 : 1);
+    const uint32_t slopes = scratch + block * g.bufs, columns = slopes + g.slope_bytes * g.bufs;
     const bool fetches = FORWARD && g.f.residual != nullptr;
     // the next place among the groups' blocks, and how many tiles on it is
     const auto settle = [&](uint32_t& item, int& blk) {
@@ -665,7 +674,7 @@ __device__ __forceinline__ void finish_bulk(const GemmArgs& g, const FinishMaps&
         const int tiles = settle(next_item, next_blk);
         Tile next = t;
         if (tiles && next_item < g.items) next = tile_of(g, next_item);
-        const uint32_t out = scratch + block * buf.at, slope = out + block * g.bufs;
+        const uint32_t out = scratch + block * buf.at, slope = slopes + g.slope_bytes * buf.at;
         const Turn here = buf;
         float row_scale = 1.0f;
         bool next_under_way = false;
@@ -1230,10 +1239,11 @@ __global__ void __launch_bounds__(256) join_layer_kernel(const Finish f, const f
         const float r = f.residual ? to_float(static_cast<const T*>(f.residual)[row * f.residual_stride + col]) : 0.0f;
         by_activation(f.activation, [&](auto act) {
             constexpr int ACT = decltype(act)::value;
-            if (f.slope) activate<ACT, true, kRounded>(f.omega, z, d);
-            else activate<ACT, false, kRounded>(f.omega, z, d);
+            if (f.slope) {
+                activate<ACT, true, kRounded>(f.omega, z, d);
+                static_cast<SlopeOf<T, ACT>*>(f.slope)[i] = from_float<SlopeOf<T, ACT>>(d[0]);
+            } else activate<ACT, false, kRounded>(f.omega, z, d);
         });
-        if (f.slope) static_cast<T*>(f.slope)[i] = from_float<T>(d[0]);
         static_cast<T*>(f.out)[i] = from_float<T>(z[0] + r);
     }
 }
@@ -1302,10 +1312,11 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const GemmArgs g, bool wi
             const int64_t at = lane * g.n + n;
             by_activation(f.activation, [&](auto act) {
                 constexpr int ACT = decltype(act)::value;
-                if (f.slope) activate<ACT, true, ROUNDED>(f.omega, z, d);
-                else activate<ACT, false, ROUNDED>(f.omega, z, d);
+                if (f.slope) {
+                    activate<ACT, true, ROUNDED>(f.omega, z, d);
+                    static_cast<SlopeOf<OUT, ACT>*>(f.slope)[at] = from_float<SlopeOf<OUT, ACT>>(d[0]);
+                } else activate<ACT, false, ROUNDED>(f.omega, z, d);
             });
-            if (f.slope) static_cast<OUT*>(f.slope)[at] = from_float<OUT>(d[0]);
             static_cast<OUT*>(f.out)[at] = from_float<OUT>(z[0] + r);
         }
     }
@@ -1386,21 +1397,38 @@ __global__ void __launch_bounds__(256) few_outputs_kernel(const GemmArgs g, bool
             const int64_t at = (row0 + i) * outputs + n;
             by_activation(f.activation, [&](auto act) {
                 constexpr int ACT = decltype(act)::value;
-                if (f.slope) activate<ACT, true, ROUNDED>(f.omega, z, d);
-                else activate<ACT, false, ROUNDED>(f.omega, z, d);
+                if (f.slope) {
+                    activate<ACT, true, ROUNDED>(f.omega, z, d);
+                    static_cast<SlopeOf<T, ACT>*>(f.slope)[at] = from_float<SlopeOf<T, ACT>>(d[0]);
+                } else activate<ACT, false, ROUNDED>(f.omega, z, d);
             });
-            if (f.slope) static_cast<T*>(f.slope)[at] = from_float<T>(d[0]);
             static_cast<T*>(f.out)[at] = from_float<T>(z[0] + r);
         }
     }
 }
 
 // ---- dz and its column sums -------------------------------------------------------------------------------------------
-// dz = dy * slope (slope kind 1) or dy where the output is positive (kind 2: relu without a residual); column sums of it
-// (kind 0: of dy) over the rows of a CTA go to partial[CTA][outputs].  A row has as many lanes as it has accesses, 32 at
-// most; blockIdx.x picks the columns of wider rows.
-template <class T, int VEC>
-__global__ void __launch_bounds__(256) slope_kernel(const T* __restrict__ dy, const T* __restrict__ slope, int kind,
+// dz = dy * slope (slope kind 1, float32) or dy where slope is positive (kind 2: relu's slope or, without a residual, its
+// output); column sums of it (kind 0: of dy) over the rows of a CTA go to partial[CTA][outputs].  dz is rounded to the layer's
+// type, being an operand of two products of that type: in two parts it would double them.  A row has as many lanes as it has
+// accesses, 32 at most; blockIdx.x picks the columns of wider rows.
+template <int N>
+__device__ __forceinline__ void load_floats(const float* __restrict__ p, float (&v)[N]) {
+    if constexpr (N == 8) {
+        float a[4], b[4];
+        load_n<float, 4>(p, a);
+        load_n<float, 4>(p + 4, b);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            v[j] = a[j];
+            v[j + 4] = b[j];
+        }
+    } else {
+        load_n<float, N>(p, v);
+    }
+}
+template <class T, int VEC, int SLOPE_KIND>
+__global__ void __launch_bounds__(256) slope_kernel(const T* __restrict__ dy, const std::conditional_t<SLOPE_KIND == 1, float, T>* __restrict__ slope,
                                                     int64_t rows, int64_t n, int lanes, T* __restrict__ dz,
                                                     int64_t dz_stride, float* __restrict__ partial) {
     __shared__ float sums[256 * VEC];
@@ -1414,10 +1442,11 @@ __global__ void __launch_bounds__(256) slope_kernel(const T* __restrict__ dy, co
         for (int64_t r = (int64_t)blockIdx.y * groups + group; r < rows; r += (int64_t)gridDim.y * groups) {
             float g[VEC], s[VEC];
             load_n<T, VEC>(dy + r * n + col, g);
-            if (kind != 0) {
-                load_n<T, VEC>(slope + r * n + col, s);
+            if (SLOPE_KIND != 0) {
+                if constexpr (SLOPE_KIND == 1) load_floats<VEC>(slope + r * n + col, s);
+                else load_n<T, VEC>(slope + r * n + col, s);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) g[j] = kind == 1 ? g[j] * s[j] : s[j] > 0.0f ? g[j] : 0.0f;
+                for (int j = 0; j < VEC; ++j) g[j] = SLOPE_KIND == 1 ? g[j] * s[j] : s[j] > 0.0f ? g[j] : 0.0f;
                 if (dz != nullptr) store_n<T, VEC>(dz + r * dz_stride + col, g);
             }
 #pragma unroll
@@ -1462,7 +1491,7 @@ __global__ void __launch_bounds__(256) small_grads_kernel(const SmallGrads s) {
     const int tile = is_dx ? blockIdx.x : blockIdx.x - s.dx_tiles, across = (s.inputs + 31) / 32;
     const int first = tile / across * 32, k0 = tile % across * 32;      // rows of x, or outputs; inputs
     const int length = is_dx ? s.outputs : s.rows;
-    const T *dy = static_cast<const T*>(s.dy), *slope = static_cast<const T*>(s.slope);
+    const T* dy = static_cast<const T*>(s.dy);
     const T* other = static_cast<const T*>(is_dx ? s.weight : s.dw ? s.x : nullptr);
     const int64_t stride = is_dx ? s.weight_stride : s.x_stride;
     const bool sums = !is_dx && k0 == 0 && s.db != nullptr;
@@ -1477,8 +1506,8 @@ __global__ void __launch_bounds__(256) small_grads_kernel(const SmallGrads s) {
             if (row < s.rows && out < s.outputs) {
                 const int64_t e = (int64_t)row * s.outputs + out;
                 a[i] = to_float(dy[e]);
-                if (s.kind == 1) a[i] *= to_float(slope[e]);
-                else if (s.kind == 2) a[i] = to_float(slope[e]) > 0.0f ? a[i] : 0.0f;
+                if (s.kind == 1) a[i] *= static_cast<const float*>(s.slope)[e];
+                else if (s.kind == 2) a[i] = to_float(static_cast<const T*>(s.slope)[e]) > 0.0f ? a[i] : 0.0f;
             }
             if (other != nullptr && at + r < length && k0 + tx < s.inputs) b[i] = to_float(other[(at + r) * stride + k0 + tx]);
         }
@@ -1600,12 +1629,12 @@ static void plan_slots(Plan* p, int columns) {
 
 // A finisher's shared memory: blocks that leave by bulk copies, and their columns' biases and scales, or a block (two, where
 // sums of several phases wait in them) whose values are stored.
-static size_t finisher_bytes(const Plan& p, int block, bool slope) {
-    return p.bulk_out ? (size_t)(block * p.bufs * (slope ? 2 : 1) + 1024) : (size_t)4096 * p.places;
+static size_t finisher_bytes(const Plan& p, int block, int slope) {
+    return p.bulk_out ? (size_t)((block + slope) * p.bufs + 1024) : (size_t)4096 * p.places;
 }
 
-// Stages and finishers once it is known how results are stored.  block: bytes of one that leaves by bulk copies.
-static void plan_shared(Plan* p, int64_t blocks, int block, bool slope) {
+// Stages and finishers once it is known how results are stored.  block, slope: bytes of one that leaves by bulk copies.
+static void plan_shared(Plan* p, int64_t blocks, int block, int slope) {
     const size_t room = kSharedLimit - 2048;
     plan_slots(p, p->bn);
     p->places = 1;
@@ -1625,7 +1654,7 @@ static void plan_shared(Plan* p, int64_t blocks, int block, bool slope) {
 }
 
 // The same of split_gemm_kernel.  Blocks are half as long as the plan counts them.
-static void plan_split(Plan* p, bool a_down, bool b_down, int64_t k, bool slope) {
+static void plan_split(Plan* p, bool a_down, bool b_down, int64_t k, int slope) {
     const int64_t blocks = ceil_div(k, kSplitBlock);
     plan_slots(p, 2 * p->bn);
     p->split_blocks *= 2;
@@ -1637,7 +1666,7 @@ static void plan_split(Plan* p, bool a_down, bool b_down, int64_t k, bool slope)
     const size_t b = 3 * (b_down ? split_bytes<true>(p->bn) : split_bytes<false>(p->bn));
     const size_t raw_a = kTileM * 128, raw_b = (size_t)p->bn * 128, all = kSharedLimit - 2048;
     // B stays where two stages of A's parts and three of its values fit beside it and the smallest finishers
-    const size_t least = 8 * (size_t)(p->bulk_out ? 4096 * (slope ? 2 : 1) + 1024 : 4096 * p->places);
+    const size_t least = 8 * (size_t)(p->bulk_out ? 4096 + slope + 1024 : 4096 * p->places);
     p->b_stays = p->b_stays && b * blocks + 2 * a + 3 * raw_a + least <= all;
     const size_t operands = p->b_stays ? b * blocks + 2 * a + 3 * raw_a : 2 * (a + b + raw_a + raw_b);
     // two blocks of a finisher, else one, else blocks that are stored value by value
@@ -1706,7 +1735,7 @@ static bool finish_maps(FinishMaps* maps, const GemmArgs& g, int64_t splits) {
     const Finish& f = g.f;
     const int type = f.partial ? ASHB_F32 : f.type;
     return block_map(&maps->out, f.partial ? (const void*)f.partial : f.out, type, g.n, g.m, g.n, splits) &&
-           (!f.slope || block_map(&maps->slope, f.slope, type, g.n, g.m, g.n, 1)) &&
+           (!f.slope || block_map(&maps->slope, f.slope, f.activation == kRelu ? type : ASHB_F32, g.n, g.m, g.n, 1)) &&
            (!f.residual || block_map(&maps->residual, f.residual, type, f.residual_stride, g.m, g.n, 1));
 }
 
@@ -1826,8 +1855,10 @@ static int run_product(GemmArgs g, int type, Plan p, cudaStream_t st) {
     FinishMaps maps{};
     p.bulk_out = finish_maps(&maps, g, p.splits);
     constexpr int64_t kBlock = kBlockK<KIND>;
-    if (KIND == kSplit) plan_split(&p, A_DOWN, B_DOWN, g.k, g.f.slope != nullptr);
-    else plan_shared(&p, ceil_div(g.k, kBlock), g.f.partial || g.f.type == ASHB_F32 ? 4096 : 2048, g.f.slope != nullptr);
+    const int block = g.f.partial || g.f.type == ASHB_F32 ? 4096 : 2048, slope = !g.f.slope ? 0 : g.f.activation == kRelu ? block : 4096;
+    if (KIND == kSplit) plan_split(&p, A_DOWN, B_DOWN, g.k, slope);
+    else plan_shared(&p, ceil_div(g.k, kBlock), block, slope);
+    g.slope_bytes = (uint32_t)slope;
     g.bulk_out = p.bulk_out;
     g.bufs = p.bufs;
     g.finish_bytes = p.finish_bytes;
@@ -1887,13 +1918,21 @@ static int64_t slope_rows(int type, int64_t rows, int64_t n) {
     return std::max(plan_slope(type, rows, n, true).down, plan_slope(type, rows, n, false).down);
 }
 
+template <class T, int SLOPE_KIND>
+static void launch_slope_kind(const SlopePlan& p, const void* dy, const void* slope, int64_t rows, int64_t n, void* dz, int64_t dz_stride,
+                              float* partial, cudaStream_t st) {
+    const dim3 grid(p.across, p.down);
+    const T* g = static_cast<const T*>(dy);
+    const auto* s = static_cast<const std::conditional_t<SLOPE_KIND == 1, float, T>*>(slope);
+    if (p.vec > 1) slope_kernel<T, 16 / sizeof(T), SLOPE_KIND><<<grid, 256, 0, st>>>(g, s, rows, n, p.lanes, static_cast<T*>(dz), dz_stride, partial);
+    else slope_kernel<T, 1, SLOPE_KIND><<<grid, 256, 0, st>>>(g, s, rows, n, p.lanes, static_cast<T*>(dz), dz_stride, partial);
+}
 template <class T>
 static void launch_slope(const SlopePlan& p, const void* dy, const void* slope, int kind, int64_t rows, int64_t n, void* dz,
                          int64_t dz_stride, float* partial, cudaStream_t st) {
-    const dim3 grid(p.across, p.down);
-    const T *g = static_cast<const T*>(dy), *s = static_cast<const T*>(slope);
-    if (p.vec > 1) slope_kernel<T, 16 / sizeof(T)><<<grid, 256, 0, st>>>(g, s, kind, rows, n, p.lanes, static_cast<T*>(dz), dz_stride, partial);
-    else slope_kernel<T, 1><<<grid, 256, 0, st>>>(g, s, kind, rows, n, p.lanes, static_cast<T*>(dz), dz_stride, partial);
+    if (kind == 0) launch_slope_kind<T, 0>(p, dy, nullptr, rows, n, dz, dz_stride, partial, st);
+    else if (kind == 1) launch_slope_kind<T, 1>(p, dy, slope, rows, n, dz, dz_stride, partial, st);
+    else launch_slope_kind<T, 2>(p, dy, slope, rows, n, dz, dz_stride, partial, st);
 }
 
 // What a layer's own product needs: copies of operands whose rows are no whole words, and the parts of split sums.
@@ -1994,8 +2033,8 @@ int ashb_linear_forward(int type, const void* x, int64_t x_stride, const float* 
     f.omega = omega;
     const uintptr_t four = (uintptr_t)(4 * value_bytes(out_type));
     f.wide = outputs % 4 == 0 && (!residual || residual_stride % 4 == 0) &&
-             (((uintptr_t)y | (uintptr_t)slope | (uintptr_t)bias | (uintptr_t)residual) & (four - 1)) == 0 &&
-             ((uintptr_t)f.b_scales & 15) == 0;
+             (((uintptr_t)y | (uintptr_t)bias | (uintptr_t)residual) & (four - 1)) == 0 &&
+             (((uintptr_t)f.b_scales | (uintptr_t)slope) & 15) == 0;
     if (rows <= kFewRows) {
         const bool wide = is_whole(type, x, rows == 1 ? 0 : x_stride) && is_whole(type, weight, weight_stride) &&
                           inputs * operand_bytes(type) % 16 == 0;
