@@ -262,7 +262,7 @@ def test_gelu_of_negative_sums(m, n, dtype):
     rel = 2.0**-14 if dtype != torch.float32 else (16 + 4 * zd * zd) * 2.0**-24
     final = lambda e, t: e * (1 + lb.half(dtype)) + lb.half(dtype) * t.abs() + lb.smallest(dtype) + lb.TINY
     lb.assert_within(y.detach(), (zd * c).expand(m, n), final(rel * (zd * c).abs(), zd * c).expand(m, n), "gelu")
-    for got in (dz, again.detach()):      # the slope is kept in the layer's type, dz and dx are the same value then
+    for got in (dz, again.detach()):      # dz is rounded to the layer's type, and dx is the same value
         lb.assert_within(got, c + d, final(rel * (c.abs() + d.abs()), c + d), "its slope")
 
 @pytest.mark.parametrize("dtype", TYPES)

@@ -114,7 +114,7 @@ class _FusedLinear(torch.autograd.Function):
                 dz = torch.where(slope.detach() > 0, grad, 0)
             elif ctx.kind == 1:
                 # The formula in float32, and of the float32 sum, as the slope is without recording: a sum rounded to 16 bits
-                # first is off by 2^-9 of itself, times omega in a sine's phase (omega 30, bf16: 9 % of the slope, against 0.2 %).
+                # first is off by up to 2^-8 of itself, times omega in a sine's phase (omega 30, bf16: 9 % of the slope, against 0.2 %).
                 # The casts keep 16-bit factors what they are; the product of float32 rows is the price.
                 z = fused_linear(x.float(), weight.float(), None if bias is None else bias.float())
                 dz = (grad.float() * _slope(z, ctx.activation, ctx.omega)).to(grad.dtype)

@@ -12,10 +12,10 @@
 //
 // Types.  f16 and bf16 are multiplied as they are, e4m3 with the scales of its rows applied to the sums.  float32 values
 // are split exactly into three bf16 parts, v = hi + mid + lo (8 bits each), and six of the nine products are formed:
-// what is left out is below 2^-22 of a term (two products of parts of 2^-7 and 2^-16).  Their sums are kept apart, hi hi in one accumulator and the five small
-// ones in another, and both are added to float32 registers, rounded to nearest, every 512 values: the tensor cores
-// truncate as they accumulate, which over thousands of steps would be seen in 32 bits.  (An infinity in float32 operands
-// becomes NaN: its mid part is infinity less infinity.)
+// what is left out is below 2^-22 of a term (two products of parts of 2^-7 and 2^-16).  Their sums are kept apart, hi hi in one
+// accumulator and the five small ones in another, and both are added to float32 registers, rounded to nearest, every 512 values:
+// the tensor cores truncate as they accumulate, which over thousands of steps would be seen in 32 bits.  (An infinity in float32
+// operands becomes NaN: its mid part is infinity less infinity.)
 //
 // Shape of a CTA, one per SM and looping over tiles of 128 x bn: one thread fills a ring of shared-memory stages by tiled bulk
 // copies, one warp issues the products, and eight or twelve warps finish the tiles before, whose sums are in tensor memory.
@@ -24,8 +24,9 @@
 // A layer's rows are many and few values wide as often as not: then the kernel is bound by memory, and a weight tile that
 // serves every tile of a CTA is loaded once (`b_stays`).
 //
-// Measured (B200, 6547 GB/s and 1657 TFLOP/s bf16 measured): 8192 x 4096 -> 4096 bf16 with gelu and residual 204 us, 81 % of
-// those; e4m3 111 us; a sine layer of 1M float32 rows 64 -> 64 136 us, 3.8 TB/s; without an activation 97 us, 5.3 TB/s, bf16 53 us.
+// Measured (B200, 6547 GB/s and 1657 TFLOP/s bf16 measured; kernels alone, back to back): 8192 x 4096 -> 4096 bf16 with gelu and
+// residual 204 us, 81 % of those; e4m3 111 us; a sine layer of 1M float32 rows 64 -> 64 143 us, 3.6 TB/s; without an activation
+// 98 us, 5.2 TB/s, bf16 57 us.  Calls that do not follow one another in a burst: 241, 137 and 151 us.
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -62,7 +63,7 @@ __device__ __noinline__ void tell_timeout(unsigned int* told) {
 // ---- activations -----------------------------------------------------------------------------------------------------
 // Short and without branches, so that a block's 32 values a lane are straight code.  ROUNDED: the results are rounded to 16
 // bits, and the hardware's exponential will do: e^x is off by (2 + 1.2 |x|) 2^-23 of itself, which is less than half a step of
-// float16 (2^-12) wherever e^x is neither 0 nor infinite.  The quotient of silu is 0 below -87.3, where its value is 2^-119.
+// float16 (2^-11) wherever e^x is neither 0 nor infinite.  The quotient of silu is 0 below -87.3, where its value is 2^-119.
 
 // sin(x + turn pi / 2), turn 0 or 1.  Reduction by a multiple k of pi in two parts (W. J. Cody, W. Waite, Software Manual for
 // the Elementary Functions, 1980): k times the first part is a multiple of x's last place, so the first step is exact.
@@ -1552,7 +1553,7 @@ static bool is_small_layer(int64_t rows, int64_t inputs, int64_t outputs) {
 static void launch_small_grads(int type, SmallGrads s, cudaStream_t st) {
     const int across = (s.inputs + 31) / 32;
     s.dx_tiles = s.dx ? (s.rows + 31) / 32 * across : 0;
-    // dW's tiles, or those of the first inputs alone where only the columns' sums are wanted: they come first in a row of tiles
+    // dW's tiles; where only the columns' sums are wanted too, of which those at the first inputs do the work
     const int dw_tiles = s.dw || s.db ? (s.outputs + 31) / 32 * across : 0;
     const unsigned blocks = (unsigned)(s.dx_tiles + dw_tiles);
     if (blocks == 0) return;

@@ -10,8 +10,8 @@
 // Everything is memory traffic: each input is read once and each output written once, the row staying in the
 // registers of the lanes that share it between the sum of squares, the largest magnitude and the stores.  Accesses are 16
 // bytes.  Rows that are no multiples of that are taken through windows: the row's lanes walk the 16-byte words that hold it,
-// whose first and last it shares with its neighbours and stores value by value (12383 rows of 3230 bf16 values with gradients
-// 518 us with accesses of one value, 309 so).  Sums are
+// whose first and last it shares with its neighbours and stores value by value (12383 rows of 3230 bf16 values with a residual and
+// gradients 518 us with accesses of one value, 310 so).  Sums are
 // float32; s enters the statistics before it is rounded to its type, the backward pass reads it rounded.  A row has
 // 8, 32 or 256 threads by its width; rows wider than 8192 are read again for each of their passes.
 // The weight's gradient is summed by a thread over the rows of its CTA, then over the CTAs in their order by a second
@@ -121,7 +121,7 @@ __device__ __forceinline__ void load_weights(const T* __restrict__ w, int col, i
 }
 
 // VEC values an access (one where rows have strides or buffers are not aligned for more), NV accesses a thread.
-// Eight CTAs an SM where registers allow it: 8192 rows of 4096 bf16 values with residual and 8-bit output 42 us (5.6 TB/s), 46 with
+// Eight CTAs an SM where registers allow it: 8192 rows of 4096 bf16 values with residual and 8-bit output 43 us (5.5 TB/s), 46 with
 // the six that the compiler left room for, 54 with the weights fetched ahead of the sum in registers of their own.
 template <class T, int VEC, int TPR, int NV, bool QUANT, bool WINDOW>
 __global__ void __launch_bounds__(256, NV * VEC <= 16 && !WINDOW ? 8 : 1) norm_forward_kernel(const NormArgs a) {
@@ -294,7 +294,9 @@ __global__ void __launch_bounds__(256) norm_forward_long_kernel(const NormArgs a
     }
 }
 
-// Rows in turn, so that a thread keeps the weight's gradient of its columns in registers.  Through windows the columns of a
+// Rows in turn, so that a thread keeps the weight's gradient of its columns in registers.  With 32 columns a thread, and through
+// windows with 16, s, g, ds and dw spill (16-bit rows of 513 to 1024 values 200 bytes a thread, as windows 360): fewer columns would
+// take a second CTA's or warp's sums per row.  Through windows the columns of a
 // thread depend on where its row begins in a 16-byte word: a group takes rows that begin alike, `period` apart.
 template <class T, int VEC, int TPR, int NV, bool WINDOW>
 __global__ void __launch_bounds__(256, NV * VEC <= 8 ? 4 : NV * VEC <= 16 ? 3 : 2) norm_backward_kernel(const NormGradArgs a) {
