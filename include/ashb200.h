@@ -55,6 +55,7 @@ extern "C" {
 typedef struct ashb_map ashb_map;
 
 const char* ashb_last_error_string(void);
+/* 2: slopes of 16-bit layers are float32 (1: of the layer's type). */
 int ashb_version(void);
 
 /* ---------------------------------------------------------------- hash engine */
@@ -825,8 +826,8 @@ int64_t ashb_linear_forward_workspace(int type, const void* x_dev, int64_t x_str
 /* Gradients of the same from dy [rows][outputs] (contiguous): dx [rows][inputs], dweight [outputs][inputs] and dbias
  * [outputs], each NULL where not wanted (the residual's is dy).  slope_kind 0: no activation, slope NULL; 1: slope holds
  * act'(z) in float32; 2: relu, slope is its slope or, without a residual, the output y.  dz = dy act'(z) is rounded to
- * `type`, whose products are taken of it (not in layers of up to 256 rows and outputs).  Sums run in a fixed order.  _workspace: bytes of device
- * scratch (256-byte aligned). */
+ * `type`, whose products are taken of it (not in layers of up to 256 rows and outputs).  Sums run in a fixed order.
+ * _workspace: bytes of device scratch (256-byte aligned). */
 int64_t ashb_linear_backward_workspace(int type, const void* dy_dev, const void* x_dev, int64_t x_stride, const void* weight_dev,
                                        int64_t weight_stride, int64_t rows, int64_t inputs, int64_t outputs, int slope_kind,
                                        int want_dx, int want_dweight, int want_dbias);
@@ -836,8 +837,9 @@ int ashb_linear_backward(int type, const void* dy_dev, const void* slope_dev, in
                          int64_t workspace_bytes, void* stream);
 
 /* In how many CTAs of the layer kernels a wait ran out on the current device since this was last asked (0 in a healthy
- * run); what such a launch returned is incomplete.  Waits for the device.  The calls above look without waiting: the first
- * one after it is known, with arguments that are otherwise good, launches nothing and returns ASHB_ERR_TIMEOUT, once. */
+ * run); what such a launch returned is incomplete.  Waits for the device.  ashb_linear_forward and
+ * ashb_linear_backward look without waiting: the first such call after it is known, with arguments that are otherwise
+ * good, launches nothing and returns ASHB_ERR_TIMEOUT, once. */
 int ashb_layer_timeouts(unsigned int* out);
 
 /* ---------------------------------------------------------------- runtime knobs */

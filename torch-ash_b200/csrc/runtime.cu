@@ -106,7 +106,7 @@ int ashb_measure_random_reads(const void* buffer, int64_t bytes, int64_t n_reads
 
 const char* ashb_last_error_string(void) { return ashb::g_error; }
 
-int ashb_version(void) { return 1; }
+int ashb_version(void) { return 2; }
 
 int ashb_set_l2_fetch_granularity(int bytes) {
     ASHB_REQUIRE(bytes == 32 || bytes == 64 || bytes == 128, "granularity must be 32, 64 or 128 bytes");
